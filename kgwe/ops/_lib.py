@@ -73,6 +73,16 @@ _SIGS = {
                                 c_int, c_int, c_int, c_int, c_void_p]),
     "kgwe_wgrad_splits": (c_int, [c_int, c_int, c_int]),
     "kgwe_wgrad_workspace": (c_int64, [c_int, c_int, c_int]),
+    "kgwe_norm_rope_fwd": (c_int, [c_void_p, c_int64, *[c_void_p] * 11, *[c_int] * 8, c_float, c_int, c_void_p]),
+    "kgwe_norm_rope_bwd_blocks": (c_int, [c_int, c_int, c_int, c_int]),
+    "kgwe_norm_rope_bwd": (c_int, [c_void_p, c_int64, *[c_void_p] * 12, *[c_int] * 6, c_float, c_int, c_void_p]),
+    "kgwe_packed_plan_jobs": (c_int, [c_int, c_int]),
+    "kgwe_packed_plan": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
+                                 c_void_p]),
+    "kgwe_packed_attn_fwd": (c_int, [*[c_void_p, c_int64, c_int64] * 5, c_int, c_void_p, c_void_p, c_void_p,
+                                     c_void_p, *[c_int] * 6, c_float, c_int, c_int, c_void_p]),
+    "kgwe_packed_attn_bwd": (c_int, [*[c_void_p, c_int64, c_int64] * 3, *[c_void_p] * 9, *[c_int] * 6, c_float,
+                                     c_int, c_int, c_void_p]),
 }
 _OPTIONAL_SIGS = {
     "kgwe_flash_attn_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -135,6 +145,20 @@ def ptr(t: torch.Tensor | None) -> int | None:
 def check(rc: int, what: str) -> None:
     if rc != 0:
         raise RuntimeError(f"{what} failed with code {rc}")
+
+
+# Type codes of the kernels that take more than one 16-bit type (native/ops/half_types.h).
+HALF_TYPES = {torch.bfloat16: 0, torch.float16: 1}
+
+
+def rows16(t: torch.Tensor) -> torch.Tensor:
+    """t itself where its last dimension is dense and every row starts on 16
+    bytes (what the strided kernels read), else a contiguous copy."""
+    ok = (t.stride(-1) == 1 and all(s % 8 == 0 and s >= 0 for s in t.stride()[:-1]) and t.data_ptr() % 16 == 0)
+    if ok:
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def use_hip(*tensors: torch.Tensor) -> bool:

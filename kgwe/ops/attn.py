@@ -6,6 +6,9 @@ Dispatch order on a GPU:
   2. otherwise (head_dim != 128, or forced) PyTorch SDPA (ROCm flash
      backend) with the GQA heads expanded.
 On CPU the fp32 reference is used.
+
+``attention_packed`` is the same for sequences of different lengths packed on
+one token axis (``native/ops/packed_attn.hip``).
 """
 from __future__ import annotations
 
@@ -15,7 +18,8 @@ import torch
 import torch.nn.functional as F
 
 from . import reference as ref
-from ._lib import check, has_symbol, lib, ptr, stream, use_hip
+from ._lib import HALF_TYPES, check, has_symbol, lib, ptr, rows16, stream, use_hip
+from .packed import PackedBatch
 
 
 class _FlashAttn(torch.autograd.Function):
@@ -89,3 +93,94 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
         vt = vt.repeat_interleave(hq // hkv, dim=1)
     o = F.scaled_dot_product_attention(qt, kt, vt, is_causal=causal)
     return o.transpose(1, 2)
+
+
+# --------------------------------------------------------------------------
+# Packed sequences
+# --------------------------------------------------------------------------
+def _packed_fwd(q, k, v, batch, causal, prefix, want_lse):
+    T, Hq, D = q.shape
+    Hkv = k.shape[1]
+    o = torch.empty(T, Hq, D, device=q.device, dtype=q.dtype)
+    lse = torch.empty(Hq, T, device=q.device, dtype=torch.float32) if want_lse else None
+    pk, pv = prefix if prefix is not None else (None, None)
+    P = pk.shape[1] if pk is not None else 0
+    views = [x for t in (q, k, v) for x in (ptr(t), t.stride(0), t.stride(1))]
+    for t in (pk, pv):  # [Hkv, P, D]: row stride, head stride
+        views += [ptr(t), t.stride(1), t.stride(0)] if P else [None, 0, 0]
+    with torch.cuda.device(q.device):
+        check(lib().kgwe_packed_attn_fwd(*views, P, ptr(o), ptr(lse), ptr(batch.cu), ptr(batch.jobs),
+                                         batch.jobs.shape[0], batch.n, T, Hq, Hkv, D, 1.0 / math.sqrt(D),
+                                         int(causal), HALF_TYPES[q.dtype], stream(q)), "packed_attn_fwd")
+    return o, lse
+
+
+class _PackedAttn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, batch, causal):
+        o, lse = _packed_fwd(q, k, v, batch, causal, None, True)
+        ctx.save_for_backward(q, k, v, o, lse)
+        ctx.batch, ctx.causal = batch, causal
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, lse = ctx.saved_tensors
+        batch = ctx.batch
+        T, Hq, D = q.shape
+        Hkv = k.shape[1]
+        do = do.contiguous()
+        if do.data_ptr() % 16:
+            do = do.clone()
+        dq = torch.empty(T, Hq, D, device=q.device, dtype=q.dtype)
+        dk = torch.empty(T, Hkv, D, device=q.device, dtype=q.dtype)
+        dv = torch.empty_like(dk)
+        delta = torch.empty_like(lse)
+        views = [x for t in (q, k, v) for x in (ptr(t), t.stride(0), t.stride(1))]
+        with torch.cuda.device(q.device):
+            check(lib().kgwe_packed_attn_bwd(*views, ptr(o), ptr(lse), ptr(do), ptr(delta), ptr(dq), ptr(dk), ptr(dv),
+                                             ptr(batch.cu), ptr(batch.jobs), batch.jobs.shape[0], batch.n, T, Hq, Hkv,
+                                             D, 1.0 / math.sqrt(D), int(ctx.causal), HALF_TYPES[q.dtype], stream(q)),
+                  "packed_attn_bwd")
+        return dq, dk, dv, None, None
+
+
+def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: PackedBatch, causal: bool = True,
+                     prefix: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+    """Attention of every sequence of a packed batch with itself: q [T, Hq, D],
+    k / v [T, Hkv, D] -> [T, Hq, D], T = ``batch.total``; differentiable.
+
+    prefix: (keys, values), each [Hkv, P, D], that every row sees before its
+    own sequence (a prompt shared by the batch); forward only.  Padding rows
+    (behind the last sequence) give zeros and get zero gradients, whatever they
+    hold.  On a GPU: bf16 or fp16, D 64 or 128; q / k / v may be views with
+    dense 16-byte aligned rows (slices of a fused projection), others are
+    copied.  A NaN or infinity in v reaches the rows that see it and may reach
+    up to 63 rows before it in its own sequence, never another sequence."""
+    if not (q.dim() == k.dim() == v.dim() == 3 and q.shape[0] == k.shape[0] == batch.total and k.shape == v.shape
+            and q.shape[2] == k.shape[2] and k.shape[1] > 0 and q.shape[1] > 0 and q.shape[1] % k.shape[1] == 0):
+        raise ValueError(f"attention_packed: q [T, Hq, D], k / v [T, Hkv, D] with T = {batch.total} and Hq % Hkv == 0, "
+                         f"got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    tensors = [q, k, v]
+    if prefix is not None:
+        pk, pv = prefix
+        if not (pk.dim() == 3 and pk.shape == pv.shape and pk.shape[0] == k.shape[1] and pk.shape[2] == k.shape[2]):
+            raise ValueError("attention_packed: prefix keys and values must be [Hkv, P, D]")
+        tensors += [pk, pv]
+        if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+            raise ValueError("attention_packed: a shared prefix has no gradient; call it under torch.no_grad()")
+    if any(t.dtype != q.dtype or t.device != q.device for t in tensors) or batch.device != q.device:
+        raise ValueError("attention_packed: tensors and batch must share one type and device")
+    if not use_hip(q):
+        return ref.attention_packed(q, k, v, batch.lengths.tolist(), causal, prefix)
+    if q.dtype not in HALF_TYPES or q.shape[2] not in (64, 128):
+        raise ValueError("attention_packed: bf16 or fp16 with head_dim 64 or 128")
+    if batch.total == 0:
+        return q.clone()
+    q, k, v = rows16(q), rows16(k), rows16(v)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+        return _PackedAttn.apply(q, k, v, batch, causal)
+    if prefix is not None:
+        prefix = (rows16(prefix[0]), rows16(prefix[1])) if prefix[0].shape[1] else None
+    return _packed_fwd(q, k, v, batch, causal, prefix, False)[0]

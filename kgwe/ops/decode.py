@@ -20,7 +20,8 @@ import math
 
 import torch
 
-from ._lib import check, lib, ptr, stream, use_hip
+from . import reference as ref
+from ._lib import HALF_TYPES, check, lib, ptr, rows16, stream, use_hip
 
 
 def _require(cond: bool, msg: str) -> None:
@@ -85,6 +86,53 @@ def rope_append(qkv: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, sin: to
     check(lib().kgwe_decode_rope_append(ptr(qkv), ptr(pos), ptr(cos), ptr(sin), ptr(q), ptr(kc), ptr(vc),
                                         B, hq, hkv, d, kc.shape[2], stream(qkv)), "decode_rope_append")
     return q
+
+
+def norm_rope_append(qkv: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, kc: torch.Tensor,
+                     vc: torch.Tensor, hq: int, hkv: int, d: int, q_weight: torch.Tensor | None = None,
+                     k_weight: torch.Tensor | None = None, eps: float = 1e-5, offset: int = 0,
+                     rows: torch.Tensor | None = None, keep_kv: bool = False):
+    """``functional.norm_rope_qkv`` + the append of k / v to a cache in one
+    launch: row t of qkv [T,(hq+2hkv)d] goes to kc/vc [R,hkv,Smax,d] at
+    (rows[t], pos[t]) (int32; no ``rows``: row t), rotated at pos[t] + offset.
+    Returns q [T,hq,d], with ``keep_kv`` (q, k, v).  One new token per row in a
+    decode step, or all rows of a packed prompt.  A row of qkv whose place is
+    outside the cache (position -1: padding) writes nothing; two rows must not
+    name one place.  Forward only."""
+    from .functional import check_norm_rope  # noqa: PLC0415
+
+    T = qkv.shape[0]
+    _require(kc.shape == vc.shape and kc.dim() == 4 and kc.shape[1] == hkv and kc.shape[3] == d
+             and kc.dtype == vc.dtype == qkv.dtype and kc.is_contiguous() and vc.is_contiguous()
+             and kc.device == vc.device == qkv.device and kc.data_ptr() != vc.data_ptr(),
+             "norm_rope_append: caches must be contiguous [R, hkv, Smax, d] of qkv's type")
+    check_norm_rope("norm_rope_append", qkv, pos, cos, sin, hq, hkv, d, q_weight, k_weight, offset,
+                    kc.shape[2] + offset)
+    _require(rows is not None or T <= kc.shape[0], "norm_rope_append: more rows than the cache has")
+    _require(rows is None or (rows.dtype == torch.int32 and rows.shape == (T,) and rows.device == qkv.device),
+             "norm_rope_append: rows int32 [T]")
+    if not use_hip(qkv):
+        q, k, v = ref.norm_rope_qkv(qkv, cos, sin, pos, hq, hkv, d, q_weight, k_weight, eps, offset)
+        at = torch.arange(T, device=qkv.device) if rows is None else rows.long()
+        ok = (pos >= 0) & (pos < kc.shape[2]) & (at >= 0) & (at < kc.shape[0])
+        kc[at[ok], :, pos[ok].long()] = k[ok]
+        vc[at[ok], :, pos[ok].long()] = v[ok]
+        return (q, k, v) if keep_kv else q
+    q = torch.empty(T, hq, d, device=qkv.device, dtype=qkv.dtype)
+    k = torch.empty(T, hkv, d, device=qkv.device, dtype=qkv.dtype) if keep_kv else None
+    v = torch.empty_like(k) if keep_kv else None
+    if T > 0 and kc.numel() > 0:
+        _require(kc.data_ptr() % 16 == 0 and vc.data_ptr() % 16 == 0, "norm_rope_append: caches must be 16-byte aligned")
+        qkv = rows16(qkv)
+        qw, kw = (None, None) if q_weight is None else (rows16(q_weight), rows16(k_weight))
+        cos, sin, pos = rows16(cos.contiguous()), rows16(sin.contiguous()), pos.contiguous()
+        rows = None if rows is None else rows.contiguous()
+        with torch.cuda.device(qkv.device):
+            check(lib().kgwe_norm_rope_fwd(ptr(qkv), qkv.stride(0), ptr(pos), ptr(cos), ptr(sin), ptr(qw), ptr(kw),
+                                           ptr(q), ptr(k), ptr(v), ptr(kc), ptr(vc), ptr(rows), T, offset,
+                                           cos.shape[0], hq, hkv, d, kc.shape[2], kc.shape[0], eps,
+                                           HALF_TYPES[qkv.dtype], stream(qkv)), "norm_rope_append")
+    return (q, k, v) if keep_kv else q
 
 
 class DecodeAttention:

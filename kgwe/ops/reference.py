@@ -66,6 +66,49 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     return o.transpose(1, 2).to(q.dtype)
 
 
+def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths: list, causal: bool = True,
+                     prefix: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+    """q [T, Hq, D], k/v [T, Hkv, D], sequences one after the other; rows behind
+    the last one give zeros.  prefix: [Hkv, P, D] keys and values seen by all."""
+    G, scale = q.shape[1] // k.shape[1], q.shape[2] ** -0.5
+    out, at = [], 0
+    for n in lengths:
+        qs, ks, vs = (t[at:at + n].float().transpose(0, 1) for t in (q, k, v))
+        P = 0
+        if prefix is not None:
+            P = prefix[0].shape[1]
+            ks, vs = torch.cat([prefix[0].float(), ks], 1), torch.cat([prefix[1].float(), vs], 1)
+        s = qs @ ks.repeat_interleave(G, 0).transpose(1, 2) * scale
+        if causal:
+            s = s.masked_fill(torch.ones(n, P + n, dtype=torch.bool, device=q.device).triu(P + 1), float("-inf"))
+        out.append((s.softmax(-1) @ vs.repeat_interleave(G, 0)).transpose(0, 1).to(q.dtype))
+        at += n
+    out.append(torch.zeros_like(q[at:]))
+    return torch.cat(out)
+
+
+def norm_rope_qkv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, hq: int,
+                  hkv: int, d: int, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
+                  eps: float = 1e-5, offset: int = 0):
+    """RMS norm of every q and k head (weights [d]; None: no norm), rotation at
+    positions + offset; rows whose position is outside the tables give zeros."""
+    T = qkv.shape[0]
+    at = positions.long() + offset
+    live = (positions >= 0) & (at < cos.shape[0])
+    x = qkv.view(T, hq + 2 * hkv, d).float().masked_fill(~live[:, None, None], 0.0)
+    at = at.clamp(0, cos.shape[0] - 1)
+    c, s = cos[at].float()[:, None], sin[at].float()[:, None]
+
+    def turn(t, w):
+        if w is not None:
+            t = t * torch.rsqrt(t.pow(2).mean(-1, keepdim=True) + eps) * w.float()
+        a, b = t[..., :d // 2], t[..., d // 2:]
+        y = torch.cat([a * c - b * s, b * c + a * s], dim=-1)
+        return y.masked_fill(~live[:, None, None], 0.0).to(qkv.dtype)
+
+    return turn(x[:, :hq], q_weight), turn(x[:, hq:hq + hkv], k_weight), x[:, hq + hkv:].to(qkv.dtype)
+
+
 def adamw_(p, g, m, v, lr, b1, b2, eps, wd, step):
     m.mul_(b1).add_(g, alpha=1 - b1)
     v.mul_(b2).addcmul_(g, g, value=1 - b2)

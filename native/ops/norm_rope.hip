@@ -1,0 +1,400 @@
+// Norm of every query and key head + position rotation in one pass over the
+// fused projection's output, with its gradient, for rows at given positions.
+//
+// qkv [T, (Hq + 2 Hkv) D] (row stride given) -> q [T, Hq, D], k, v [T, Hkv, D]:
+//   n = x * rsqrt(mean(x^2) + eps) * w        per head, w [D] (absent: n = x)
+//   y[i]       = n[i] cos[p, i] - n[i + D/2] sin[p, i]         i < D/2
+//   y[i + D/2] = n[i + D/2] cos[p, i] + n[i] sin[p, i]
+// with p = pos[t] + offset and fp32 tables.  v is copied.  A row whose p is
+// outside the tables (a packed batch marks its padding rows with position -1)
+// gives zeros and takes no gradient.  Everything between the load and the
+// store is fp32: ONE rounding per output, where norm and rotation as two
+// passes round twice.
+//
+// Optionally the same launch appends k and v to a head-major cache
+// [rows, Hkv, Smax, D] at (cache_row[t], pos[t]).
+//
+// Gradient, with g = the rotation's transpose applied to dy and r = 1 / rms:
+//   dx = r (w g - x r^2 mean(w g x)),   dw = sum over rows and heads of g x r.
+//
+// Both passes are bound by HBM: a thread holds one 8-wide chunk of a head's
+// first half and the matching chunk of its second half (the pair that the
+// rotation mixes), D / 16 neighbouring lanes hold a head, and the mean is a
+// shuffle tree over them.
+#include <algorithm>
+
+#include "half_types.h"
+
+using namespace kgwe;
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kDwBlocks = 1024;  // partial sums of dw: one [2, D] row per workgroup
+
+// Sum over the L lanes that hold one head.
+template <int L>
+__device__ __forceinline__ float head_sum(float v) {
+#pragma unroll
+  for (int off = L / 2; off > 0; off >>= 1) v += __shfl_xor(v, off, kWave);
+  return v;
+}
+
+__device__ __forceinline__ void load_table(const float* __restrict__ p, float (&out)[8]) {
+  const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    out[j] = a[j];
+    out[4 + j] = b[j];
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void up8(bf16x8 v, float (&out)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) out[j] = T::up(v[j]);
+}
+
+template <class T>
+__device__ __forceinline__ bf16x8 down8(const float (&in)[8]) {
+  bf16x8 v;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = T::down(in[j]);
+  return v;
+}
+
+__device__ __forceinline__ bf16x8 ld8(const unsigned short* p) { return *reinterpret_cast<const bf16x8*>(p); }
+__device__ __forceinline__ void st8(unsigned short* p, bf16x8 v) { *reinterpret_cast<bf16x8*>(p) = v; }
+
+struct FwdArgs {
+  const unsigned short* qkv;
+  int64_t row_stride;
+  const int* pos;
+  const float* cosT;
+  const float* sinT;
+  const unsigned short* wq;  // null: no norm
+  const unsigned short* wk;
+  unsigned short* q;
+  unsigned short* k;         // null: k and v go to the cache only
+  unsigned short* v;
+  unsigned short* kc;        // null: no cache
+  unsigned short* vc;
+  const int* cache_row;      // null: row t
+  int T, offset, table_rows, Hq, Hkv, Smax, cache_rows;
+  float eps;
+};
+
+// L = D / 16 lanes per head.
+template <class T, int L>
+__global__ __launch_bounds__(kThreads) void norm_rope_fwd_kernel(FwdArgs a) {
+  constexpr int D = 16 * L, half = D / 2;
+  const int Ht = a.Hq + 2 * a.Hkv;
+  const int64_t n = static_cast<int64_t>(a.T) * Ht * L;
+  // Every lane of a wave runs the same number of rounds (the shuffles need all
+  // lanes of a head, and a wave holds whole heads: 64 % L == 0).
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < n;
+       i += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int64_t th = i / L;
+    const int c = static_cast<int>(i % L) * 8;
+    const int64_t t = th / Ht;
+    const int head = static_cast<int>(th - t * Ht);
+    const int cp = a.pos[t];
+    const int64_t p = static_cast<int64_t>(cp) + a.offset;
+    const bool live = cp >= 0 && p < a.table_rows;
+    const unsigned short* in = a.qkv + t * a.row_stride + static_cast<int64_t>(head) * D + c;
+    const bf16x8 lo = live ? ld8(in) : bf16x8{}, hi = live ? ld8(in + half) : bf16x8{};
+    const bool is_q = head < a.Hq, is_v = head >= a.Hq + a.Hkv;
+    bf16x8 ylo = lo, yhi = hi;
+    float x0[8], x1[8];
+    up8<T>(lo, x0);
+    up8<T>(hi, x1);
+    if (a.wq != nullptr) {
+      float ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss += x0[j] * x0[j] + x1[j] * x1[j];
+      ss = head_sum<L>(ss);
+      const float r = 1.f / sqrtf(ss * (1.f / D) + a.eps);
+      const unsigned short* w = is_q ? a.wq : a.wk;
+      float w0[8], w1[8];
+      up8<T>(ld8(w + c), w0);
+      up8<T>(ld8(w + half + c), w1);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x0[j] *= r * w0[j];
+        x1[j] *= r * w1[j];
+      }
+    }
+    if (live && !is_v) {
+      float cs[8], sn[8], y0[8], y1[8];
+      load_table(a.cosT + p * half + c, cs);
+      load_table(a.sinT + p * half + c, sn);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        y0[j] = x0[j] * cs[j] - x1[j] * sn[j];
+        y1[j] = x1[j] * cs[j] + x0[j] * sn[j];
+      }
+      ylo = down8<T>(y0);
+      yhi = down8<T>(y1);
+    }
+    unsigned short* out = nullptr;
+    if (is_q) out = a.q + (t * a.Hq + head) * D;
+    else if (a.k != nullptr) out = (is_v ? a.v : a.k) + (t * a.Hkv + (head - a.Hq - (is_v ? a.Hkv : 0))) * D;
+    if (out != nullptr) {
+      st8(out + c, ylo);
+      st8(out + half + c, yhi);
+    }
+    if (a.kc != nullptr && !is_q && live && cp < a.Smax) {
+      const int row = a.cache_row != nullptr ? a.cache_row[t] : static_cast<int>(t);
+      if (row >= 0 && row < a.cache_rows) {  // never write outside the cache
+        unsigned short* dst = (is_v ? a.vc : a.kc) +
+            ((static_cast<int64_t>(row) * a.Hkv + (head - a.Hq - (is_v ? a.Hkv : 0))) * a.Smax + cp) * D;
+        st8(dst + c, ylo);
+        st8(dst + half + c, yhi);
+      }
+    }
+  }
+}
+
+struct BwdArgs {
+  const unsigned short* qkv;  // the forward's input (norm only)
+  int64_t row_stride;
+  const int* pos;
+  const float* cosT;
+  const float* sinT;
+  const unsigned short* wq;
+  const unsigned short* wk;
+  const unsigned short* dq;
+  const unsigned short* dk;
+  const unsigned short* dv;
+  unsigned short* dqkv;
+  float* part;                // [grid, 2, D] sums of dw (norm only)
+  int T, offset, table_rows, Hq, Hkv;
+  float eps;
+};
+
+template <class T, int L, bool NORM>
+__global__ __launch_bounds__(kThreads) void norm_rope_bwd_kernel(BwdArgs a) {
+  constexpr int D = 16 * L, half = D / 2;
+  const int Ht = a.Hq + 2 * a.Hkv;
+  const int64_t n = static_cast<int64_t>(a.T) * Ht * L;
+  // The stride is a multiple of L, so a thread always holds the same chunk of
+  // a head and sums its share of dw in registers.
+  const int c = static_cast<int>(threadIdx.x % L) * 8;
+  float wq0[8], wq1[8], wk0[8], wk1[8], aq[16], ak[16];
+  if (NORM) {
+    up8<T>(ld8(a.wq + c), wq0);
+    up8<T>(ld8(a.wq + half + c), wq1);
+    up8<T>(ld8(a.wk + c), wk0);
+    up8<T>(ld8(a.wk + half + c), wk1);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) aq[j] = ak[j] = 0.f;
+  }
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < n;
+       i += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int64_t th = i / L;
+    const int64_t t = th / Ht;
+    const int head = static_cast<int>(th - t * Ht);
+    const int cp = a.pos[t];
+    const int64_t p = static_cast<int64_t>(cp) + a.offset;
+    const bool live = cp >= 0 && p < a.table_rows;
+    const bool is_q = head < a.Hq, is_v = head >= a.Hq + a.Hkv;
+    const unsigned short* dy = is_q ? a.dq + (t * a.Hq + head) * D
+        : (is_v ? a.dv : a.dk) + (t * a.Hkv + (head - a.Hq - (is_v ? a.Hkv : 0))) * D;
+    const bf16x8 lo = live ? ld8(dy + c) : bf16x8{}, hi = live ? ld8(dy + half + c) : bf16x8{};
+    unsigned short* out = a.dqkv + (t * Ht + head) * static_cast<int64_t>(D);
+    float g0[8], g1[8];
+    {
+      float y0[8], y1[8], cs[8], sn[8];
+      up8<T>(lo, y0);
+      up8<T>(hi, y1);
+      if (live && !is_v) {
+        load_table(a.cosT + p * half + c, cs);
+        load_table(a.sinT + p * half + c, sn);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) cs[j] = 1.f, sn[j] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        g0[j] = y0[j] * cs[j] + y1[j] * sn[j];
+        g1[j] = y1[j] * cs[j] - y0[j] * sn[j];
+      }
+    }
+    if (NORM) {  // v heads run along with their own loads idle: the shuffles want whole waves
+      const unsigned short* in = a.qkv + t * a.row_stride + static_cast<int64_t>(head) * D + c;
+      const bool use = live && !is_v;
+      float x0[8], x1[8];
+      up8<T>(use ? ld8(in) : bf16x8{}, x0);
+      up8<T>(use ? ld8(in + half) : bf16x8{}, x1);
+      float ss = 0.f, gx = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        ss += x0[j] * x0[j] + x1[j] * x1[j];
+        gx += g0[j] * (is_q ? wq0[j] : wk0[j]) * x0[j] + g1[j] * (is_q ? wq1[j] : wk1[j]) * x1[j];
+      }
+      ss = head_sum<L>(ss);
+      gx = head_sum<L>(gx);
+      if (use) {
+        const float r = 1.f / sqrtf(ss * (1.f / D) + a.eps);
+        const float m = gx * (1.f / D) * r * r;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float s0 = g0[j] * x0[j] * r, s1 = g1[j] * x1[j] * r;
+          if (is_q) aq[j] += s0, aq[8 + j] += s1;
+          else ak[j] += s0, ak[8 + j] += s1;
+          g0[j] = r * (g0[j] * (is_q ? wq0[j] : wk0[j]) - x0[j] * m);
+          g1[j] = r * (g1[j] * (is_q ? wq1[j] : wk1[j]) - x1[j] * m);
+        }
+      }
+    }
+    st8(out + c, is_v ? lo : down8<T>(g0));
+    st8(out + half + c, is_v ? hi : down8<T>(g1));
+  }
+  if (NORM) {
+    // Lanes of one chunk (same lane % L), then the four waves, in a fixed order.
+    __shared__ float red[kThreads / kWave][2][D];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+#pragma unroll
+      for (int off = kWave / 2; off >= L; off >>= 1) {
+        aq[j] += __shfl_xor(aq[j], off, kWave);
+        ak[j] += __shfl_xor(ak[j], off, kWave);
+      }
+    }
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    if (lane < L) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        red[wave][0][c + j] = aq[j];
+        red[wave][0][half + c + j] = aq[8 + j];
+        red[wave][1][c + j] = ak[j];
+        red[wave][1][half + c + j] = ak[8 + j];
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * D; i += kThreads) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < kThreads / kWave; ++w) s += red[w][i / D][i % D];
+      a.part[static_cast<int64_t>(blockIdx.x) * 2 * D + i] = s;
+    }
+  }
+}
+
+// dw[2, D] = sum of the workgroups' partials: 16 columns x 16 row groups per
+// workgroup, the groups joined through LDS in a fixed order.
+template <class T>
+__global__ __launch_bounds__(kThreads) void norm_rope_dw_kernel(const float* __restrict__ part, int blocks,
+                                                                int D, unsigned short* __restrict__ dwq,
+                                                                unsigned short* __restrict__ dwk) {
+  __shared__ float red[16][17];
+  const int col = threadIdx.x % 16, grp = threadIdx.x / 16;
+  const int i = blockIdx.x * 16 + col;  // 2 * D is a multiple of 16
+  float s = 0.f;
+  for (int b = grp; b < blocks; b += 16) s += part[static_cast<int64_t>(b) * 2 * D + i];
+  red[grp][col] = s;
+  __syncthreads();
+  if (grp == 0) {
+    float t = 0.f;
+#pragma unroll
+    for (int g = 0; g < 16; ++g) t += red[g][col];
+    (i < D ? dwq[i] : dwk[i - D]) = T::down(t);
+  }
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+inline bool shape_ok(int T, int Hq, int Hkv, int D, int dtype, int64_t row_stride) {
+  return T > 0 && Hq > 0 && Hkv > 0 && Hq <= 4096 && Hkv <= 4096 && (D == 32 || D == 64 || D == 128 || D == 256) &&
+         (dtype == kTypeBf16 || dtype == kTypeFp16) && row_stride % 8 == 0;
+}
+
+inline int grid_for(int64_t items, int most) {
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((items + kThreads - 1) / kThreads, most)));
+}
+
+template <class T>
+int fwd(const FwdArgs& a, int D, hipStream_t s) {
+  const int grid = grid_for(static_cast<int64_t>(a.T) * (a.Hq + 2 * a.Hkv) * (D / 16), 1 << 20);
+  switch (D) {
+    case 32: hipLaunchKernelGGL((norm_rope_fwd_kernel<T, 2>), dim3(grid), dim3(kThreads), 0, s, a); break;
+    case 64: hipLaunchKernelGGL((norm_rope_fwd_kernel<T, 4>), dim3(grid), dim3(kThreads), 0, s, a); break;
+    case 128: hipLaunchKernelGGL((norm_rope_fwd_kernel<T, 8>), dim3(grid), dim3(kThreads), 0, s, a); break;
+    case 256: hipLaunchKernelGGL((norm_rope_fwd_kernel<T, 16>), dim3(grid), dim3(kThreads), 0, s, a); break;
+    default: return -1;
+  }
+  return KGWE_CHECK_LAUNCH();
+}
+
+template <class T, int L>
+int bwd_launch(const BwdArgs& a, int grid, hipStream_t s) {
+  if (a.wq != nullptr)
+    hipLaunchKernelGGL((norm_rope_bwd_kernel<T, L, true>), dim3(grid), dim3(kThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL((norm_rope_bwd_kernel<T, L, false>), dim3(grid), dim3(kThreads), 0, s, a);
+  return KGWE_CHECK_LAUNCH();
+}
+
+template <class T>
+int bwd(const BwdArgs& a, int D, int grid, unsigned short* dwq, unsigned short* dwk, hipStream_t s) {
+  int rc = -1;
+  switch (D) {
+    case 32: rc = bwd_launch<T, 2>(a, grid, s); break;
+    case 64: rc = bwd_launch<T, 4>(a, grid, s); break;
+    case 128: rc = bwd_launch<T, 8>(a, grid, s); break;
+    case 256: rc = bwd_launch<T, 16>(a, grid, s); break;
+  }
+  if (rc || a.wq == nullptr) return rc;
+  hipLaunchKernelGGL((norm_rope_dw_kernel<T>), dim3(2 * D / 16), dim3(kThreads), 0, s, a.part, grid, D, dwq, dwk);
+  return KGWE_CHECK_LAUNCH();
+}
+
+}  // namespace
+
+// wq / wk null: rotation alone.  k / v null: the rotated keys and the values go
+// to the cache only (kc, vc then required).  cache_row null: row t of the cache.
+KGWE_API int kgwe_norm_rope_fwd(const void* qkv, int64_t row_stride, const int* pos, const float* cos_t,
+                                const float* sin_t, const void* wq, const void* wk, void* q, void* k, void* v,
+                                void* kc, void* vc, const int* cache_row, int T, int offset, int table_rows,
+                                int Hq, int Hkv, int D, int Smax, int cache_rows, float eps, int dtype,
+                                hipStream_t s) {
+  if (!shape_ok(T, Hq, Hkv, D, dtype, row_stride) || offset < 0 || table_rows <= 0) return -1;
+  if ((wq == nullptr) != (wk == nullptr) || (k == nullptr) != (v == nullptr) || (kc == nullptr) != (vc == nullptr) ||
+      (k == nullptr && kc == nullptr) || q == nullptr || (kc != nullptr && (Smax <= 0 || cache_rows <= 0)))
+    return -1;
+  if (!aligned16(qkv) || !aligned16(wq) || !aligned16(wk) || !aligned16(q) || !aligned16(k) || !aligned16(v) ||
+      !aligned16(kc) || !aligned16(vc) || !aligned16(cos_t) || !aligned16(sin_t))
+    return -1;
+  using u16 = unsigned short;
+  const FwdArgs a{static_cast<const u16*>(qkv), row_stride, pos, cos_t, sin_t, static_cast<const u16*>(wq),
+                  static_cast<const u16*>(wk), static_cast<u16*>(q), static_cast<u16*>(k), static_cast<u16*>(v),
+                  static_cast<u16*>(kc), static_cast<u16*>(vc), cache_row, T, offset, table_rows, Hq, Hkv, Smax,
+                  cache_rows, eps};
+  return dtype == kTypeBf16 ? fwd<Bf16>(a, D, s) : fwd<Fp16>(a, D, s);
+}
+
+// Workgroups of the gradient's launch = rows [2, D] of its fp32 workspace.
+KGWE_API int kgwe_norm_rope_bwd_blocks(int T, int Hq, int Hkv, int D) {
+  if (T <= 0 || Hq <= 0 || Hkv <= 0 || D < 16) return 0;
+  return grid_for(static_cast<int64_t>(T) * (Hq + 2 * Hkv) * (D / 16), kDwBlocks);
+}
+
+// dq, dk, dv contiguous; dqkv contiguous [T, (Hq + 2 Hkv) D].  With norms also
+// part [blocks, 2, D] fp32 and dwq, dwk [D] (always both).
+KGWE_API int kgwe_norm_rope_bwd(const void* qkv, int64_t row_stride, const int* pos, const float* cos_t,
+                                const float* sin_t, const void* wq, const void* wk, const void* dq, const void* dk,
+                                const void* dv, void* dqkv, float* part, void* dwq, void* dwk, int T, int offset,
+                                int table_rows, int Hq, int Hkv, int D, float eps, int dtype, hipStream_t s) {
+  if (!shape_ok(T, Hq, Hkv, D, dtype, row_stride) || offset < 0 || table_rows <= 0) return -1;
+  if ((wq == nullptr) != (wk == nullptr) || (wq != nullptr && (!part || !dwq || !dwk || !qkv))) return -1;
+  if (!aligned16(qkv) || !aligned16(wq) || !aligned16(wk) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) ||
+      !aligned16(dqkv) || !aligned16(cos_t) || !aligned16(sin_t))
+    return -1;
+  using u16 = unsigned short;
+  const BwdArgs a{static_cast<const u16*>(qkv), row_stride, pos, cos_t, sin_t, static_cast<const u16*>(wq),
+                  static_cast<const u16*>(wk), static_cast<const u16*>(dq), static_cast<const u16*>(dk),
+                  static_cast<const u16*>(dv), static_cast<u16*>(dqkv), part, T, offset, table_rows, Hq, Hkv, eps};
+  const int grid = kgwe_norm_rope_bwd_blocks(T, Hq, Hkv, D);
+  return dtype == kTypeBf16 ? bwd<Bf16>(a, D, grid, static_cast<u16*>(dwq), static_cast<u16*>(dwk), s)
+                            : bwd<Fp16>(a, D, grid, static_cast<u16*>(dwq), static_cast<u16*>(dwk), s);
+}

@@ -1,0 +1,517 @@
+// Attention over packed sequences (one token axis, sequences one after the
+// other), grouped heads, causal or not, forward and gradient, for 16-bit
+// inputs with fp32 accumulation; head dimension 64 or 128.
+//
+//   o_i = sum_j p_ij v_j,  p_ij = softmax_j(s q_i k_j) over the keys j of row
+//   i's own sequence (j <= i when causal), after an optional prefix whose keys
+//   and values every sequence sees.  A row that sees nothing (padding) is 0.
+//   dV_j = sum_i p_ij dO_i          dP_ij = dO_i v_j      D_i = dO_i o_i
+//   dS = p (dP - D)   dQ_i = s sum_j dS_ij k_j   dK_j = s sum_i dS_ij q_i
+//
+// One workgroup = 4 waves = 128 rows of one sequence and head (a job of the
+// batch's plan, longest sweep first); q, k, v are read through their strides,
+// so slices of a fused projection need no copy.  Tiles of 64 keys go HBM ->
+// LDS by DMA, double buffered, one barrier per tile; a tile that straddles the
+// sequence's end is loaded with zeros past it, so what the next sequence (or
+// nothing) holds there never enters.
+#include "attn_tile.h"
+
+using namespace kgwe;
+
+namespace {
+
+typedef unsigned short u16;
+constexpr int kRows = 128;    // rows of a job (packed_plan.hip)
+constexpr int kTile = 64;     // keys per tile
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct View {
+  const u16* p;
+  int64_t row, head;  // strides in elements
+};
+
+struct Batch {
+  const int* cu;    // [N + 2]
+  const int2* jobs;
+  int N, T, Hq, Hkv;
+};
+
+// Job and head of this workgroup: all heads of a job are neighbours, and on
+// Hq % 8 == 0 each of the 8 XCDs (workgroups go round them) takes a contiguous
+// run of heads, so the heads that share keys share an L2.
+__device__ __forceinline__ bool pick(const Batch& b, int heads, int* seq, int* blk, int* head) {
+  const int j = blockIdx.x / heads, p = blockIdx.x - j * heads;
+  *head = heads % 8 == 0 ? (p % 8) * (heads / 8) + p / 8 : p;
+  const int2 jb = b.jobs[j];
+  *seq = __builtin_amdgcn_readfirstlane(jb.x);
+  *blk = __builtin_amdgcn_readfirstlane(jb.y);
+  return *seq >= 0;
+}
+
+// Running max kept until a tile's max passes it by this much (log2 units), so
+// P stays below 2^4 and O is rescaled on few tiles.
+constexpr float kDefer = 4.f;
+
+struct FwdArgs {
+  Batch b;
+  View q, k, v, pk, pv;
+  u16* o;      // [T, Hq, D]
+  float* lse;  // [Hq, T], log2 units; null: not wanted
+  int P, causal;
+  float c;     // scale * log2 e
+};
+
+template <class T, int D, bool PREFIX>
+__global__ __launch_bounds__(256, 2) void packed_fwd_kernel(FwdArgs a) {
+  constexpr int NB = D / 32, NT = D / 16;
+  constexpr int kImg = kTile * D * 2;
+  // One array per stage: the compiler orders an LDS read after every DMA in
+  // flight that it cannot prove to go to another object.
+  __shared__ __attribute__((aligned(1024))) char K0[kImg], V0[kImg], K1[kImg], V1[kImg];
+  int seq, blk, h;
+  if (!pick(a.b, a.b.Hq, &seq, &blk, &h)) return;
+  const int hkv = h / (a.b.Hq / a.b.Hkv);
+  const int row0 = __builtin_amdgcn_readfirstlane(a.b.cu[seq]);
+  const int len = __builtin_amdgcn_readfirstlane(a.b.cu[seq + 1]) - row0;  // query rows
+  const int klen = seq < a.b.N ? len : 0;                                  // padding rows see nothing
+  const int plen = PREFIX && seq < a.b.N ? a.P : 0;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lq = lane & 31, hh = lane >> 5;
+  const int q0 = blk * kRows + w * 32, qrow = q0 + lq;
+  const bool mine = q0 < len;  // wave-uniform: this wave has rows
+
+  bf16x8 qf[NT];
+  {
+    const u16* qp = a.q.p + (static_cast<int64_t>(row0) + qrow) * a.q.row + h * a.q.head;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      qf[t] = qrow < len ? *reinterpret_cast<const bf16x8*>(qp + 16 * t + 8 * hh) : bf16x8{};
+  }
+  f32x16 oacc[NB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i) oacc[i] = f32x16{};
+  float m = -INFINITY, l = 0.f;
+
+  const int ntp = (plen + kTile - 1) / kTile;
+  const int kv_end = a.causal ? min(klen, blk * kRows + kRows) : klen;
+  const int nt = ntp + (kv_end + kTile - 1) / kTile;
+  const TileDma<D, kTile> dma(w, lane);
+  const TileAddr<D> ad(lane);
+  const u16* kb = a.k.p + static_cast<int64_t>(row0) * a.k.row + hkv * a.k.head;
+  const u16* vb = a.v.p + static_cast<int64_t>(row0) * a.v.row + hkv * a.v.head;
+  const u16* pkb = PREFIX ? a.pk.p + hkv * a.pk.head : nullptr;
+  const u16* pvb = PREFIX ? a.pv.p + hkv * a.pv.head : nullptr;
+
+  auto load = [&](char* Kd, char* Vd, int t) {
+    const bool pre = PREFIX && t < ntp;
+    const int k0 = (pre ? t : t - ntp) * kTile;
+    const int rows = min(kTile, (pre ? plen : klen) - k0);
+    const int64_t krow = pre ? a.pk.row : a.k.row, vrow = pre ? a.pv.row : a.v.row;
+    const int kbytes = static_cast<int>(2 * krow), vbytes = static_cast<int>(2 * vrow);
+    dma.load(row_buffer((pre ? pkb : kb) + k0 * krow, rows, kbytes), kbytes, Kd);
+    dma.load(row_buffer((pre ? pvb : vb) + k0 * vrow, rows, vbytes), vbytes, Vd);
+  };
+
+  auto tile = [&](const char* Kc, const char* Vc, char* Kn, char* Vn, int t) {
+    if (t + 1 < nt) load(Kn, Vn, t + 1);  // lands during this tile's work
+    const bool pre = PREFIX && t < ntp;
+    const int k0 = (pre ? t : t - ntp) * kTile;
+    const bool causal = a.causal && !pre;
+    if (mine && (!causal || k0 <= q0 + 31)) {  // else: the tile is past this wave's diagonal
+      // S^T = K Q^T: key on the accumulator's rows, query on the lane
+      f32x16 s[2];
+      s[0] = s[1] = f32x16{};
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int u = 0; u < NT; ++u) s[st] = mfma32<T>(ad.rows(Kc, 32 * st, u), qf[u], s[st]);
+      const int kend = pre ? plen : klen;
+      const bool edge = (causal && k0 + kTile - 1 > q0) || k0 + kTile > kend;  // wave-uniform
+      if (edge) {
+        const int last = causal ? min(kend - 1, qrow) : kend - 1;  // last key this row sees
+#pragma unroll
+        for (int st = 0; st < 2; ++st)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (k0 + 32 * st + tile_row(r, hh) > last) s[st][r] = -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[st][r]);
+      mx = half_max(mx) * a.c;
+      const float m_new = mx > m + kDefer ? mx : m;
+      const float m_use = m_new == -INFINITY ? 0.f : m_new;
+      if (__any(m_new > m)) {
+        const float alpha = exp2_fast(m - m_use);
+        l *= alpha;
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) oacc[i][r] *= alpha;
+      }
+      m = m_new;
+      // P = 2^(S c - m) in pairs; the accumulator tile is the next product's operand as it is
+      u32x4 pb[4];
+      float r0 = 0.f, r1 = 0.f;
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          const float p0 = exp2_fast(fmaf(s[st][r], a.c, -m_use));
+          const float p1 = exp2_fast(fmaf(s[st][r + 1], a.c, -m_use));
+          r0 += p0;
+          r1 += p1;
+          pb[2 * st + (r >> 3)][(r & 7) >> 1] = pack2<T>(p0, p1);
+        }
+      l += r0 + r1;  // this lane half's keys; the halves meet in the epilogue
+      // O^T += V^T P
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int db = 0; db < NB; ++db) oacc[db] = mfma32<T>(ad.cols(Vc, 16 * u, db), as_op(pb[u]), oacc[db]);
+    }
+    dma_join();
+  };
+
+  if (nt > 0) {
+    load(K0, V0, 0);
+    // The Q loads end before the loop: sunk into it, they would make the
+    // first products of every tile wait for the next tile's DMA.
+#pragma unroll
+    for (int t = 0; t < NT; ++t) asm volatile("" ::"v"(qf[t]));
+    dma_join();
+    for (int t = 0; t < nt; t += 2) {
+      tile(K0, V0, K1, V1, t);
+      if (t + 1 < nt) tile(K1, V1, K0, V0, t + 1);
+    }
+  }
+  const float lt = half_add(l);
+  const bool ok = qrow < len;
+  const int64_t orow = static_cast<int64_t>(row0) + qrow;
+  store_row<T, NB>(a.o + (orow * a.b.Hq + h) * D, oacc, lt == 0.f ? 0.f : 1.f / lt, hh, ok);
+  if (a.lse != nullptr && ok && hh == 0)
+    a.lse[static_cast<int64_t>(h) * a.b.T + orow] = lt == 0.f ? -INFINITY : m + log2f(lt);
+}
+
+struct BwdArgs {
+  Batch b;
+  View q, k, v;
+  const u16* o;       // [T, Hq, D]
+  const u16* dout;    // [T, Hq, D]
+  const float* lse;   // [Hq, T]
+  float* delta;       // [Hq, T]: written by the dQ kernel, read by the dK / dV kernel
+  u16* dq;            // [T, Hq, D]
+  u16* dk;            // [T, Hkv, D]
+  u16* dv;
+  int causal;
+  float c, scale;
+};
+
+// dQ: the forward's geometry (query on the lane).  Recomputes S^T and dP^T and
+// accumulates dQ^T += K^T dS^T, K^T read transposed from the K image.
+template <class T, int D>
+__global__ __launch_bounds__(256, 2) void packed_dq_kernel(BwdArgs a) {
+  constexpr int NB = D / 32, NT = D / 16;
+  constexpr int kImg = kTile * D * 2;
+  __shared__ __attribute__((aligned(1024))) char K0[kImg], V0[kImg], K1[kImg], V1[kImg];
+  int seq, blk, h;
+  if (!pick(a.b, a.b.Hq, &seq, &blk, &h)) return;
+  const int hkv = h / (a.b.Hq / a.b.Hkv);
+  const int row0 = __builtin_amdgcn_readfirstlane(a.b.cu[seq]);
+  const int len = __builtin_amdgcn_readfirstlane(a.b.cu[seq + 1]) - row0;
+  const int klen = seq < a.b.N ? len : 0;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lq = lane & 31, hh = lane >> 5;
+  const int q0 = blk * kRows + w * 32, qrow = q0 + lq;
+  const bool mine = q0 < len;
+  const bool ok = qrow < len;
+  const int64_t row = static_cast<int64_t>(row0) + qrow;
+
+  bf16x8 qf[NT], df[NT];
+  float dsum = 0.f;
+  {
+    const u16* qp = a.q.p + row * a.q.row + h * a.q.head;
+    const int64_t off = (row * a.b.Hq + h) * D;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      qf[t] = ok ? *reinterpret_cast<const bf16x8*>(qp + 16 * t + 8 * hh) : bf16x8{};
+      df[t] = ok ? *reinterpret_cast<const bf16x8*>(a.dout + off + 16 * t + 8 * hh) : bf16x8{};
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const bf16x8 ov = ok ? *reinterpret_cast<const bf16x8*>(a.o + off + 16 * t + 8 * hh) : bf16x8{};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dsum = fmaf(T::up(df[t][e]), T::up(ov[e]), dsum);
+    }
+  }
+  const int64_t li = static_cast<int64_t>(h) * a.b.T + row;
+  const float lse = ok ? a.lse[li] : 0.f;
+  const float delta = half_add(dsum);
+  if (hh == 0 && ok) a.delta[li] = delta;
+  f32x16 acc[NB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i) acc[i] = f32x16{};
+
+  const int kv_end = a.causal ? min(klen, blk * kRows + kRows) : klen;
+  const int nt = (kv_end + kTile - 1) / kTile;
+  const TileDma<D, kTile> dma(w, lane);
+  const TileAddr<D> ad(lane);
+  const u16* kb = a.k.p + static_cast<int64_t>(row0) * a.k.row + hkv * a.k.head;
+  const u16* vb = a.v.p + static_cast<int64_t>(row0) * a.v.row + hkv * a.v.head;
+  const int kbytes = static_cast<int>(2 * a.k.row), vbytes = static_cast<int>(2 * a.v.row);
+  auto load = [&](char* Kd, char* Vd, int t) {
+    const int k0 = t * kTile, rows = min(kTile, klen - k0);
+    dma.load(row_buffer(kb + k0 * a.k.row, rows, kbytes), kbytes, Kd);
+    dma.load(row_buffer(vb + k0 * a.v.row, rows, vbytes), vbytes, Vd);
+  };
+  auto tile = [&](const char* Kc, const char* Vc, char* Kn, char* Vn, int t) {
+    if (t + 1 < nt) load(Kn, Vn, t + 1);
+    const int k0 = t * kTile;
+    if (mine && (!a.causal || k0 <= q0 + 31)) {
+      const bool edge = (a.causal && k0 + kTile - 1 > q0) || k0 + kTile > klen;
+      const int last = a.causal ? min(klen - 1, qrow) : klen - 1;
+      // Two 32-key halves in turn: one S^T / dP^T pair live at a time.
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        f32x16 s = f32x16{}, p;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) p[r] = -delta;  // dP - D without a subtraction
+#pragma unroll
+        for (int u = 0; u < NT; ++u) {
+          s = mfma32<T>(ad.rows(Kc, 32 * st, u), qf[u], s);
+          p = mfma32<T>(ad.rows(Vc, 32 * st, u), df[u], p);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) p[r] *= exp2_fast(fmaf(s[r], a.c, -lse));
+        if (edge) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (k0 + 32 * st + tile_row(r, hh) > last) p[r] = 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          u32x4 sw;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sw[j] = pack2<T>(p[8 * u + 2 * j], p[8 * u + 2 * j + 1]);
+#pragma unroll
+          for (int db = 0; db < NB; ++db)
+            acc[db] = mfma32<T>(ad.cols(Kc, 32 * st + 16 * u, db), as_op(sw), acc[db]);
+        }
+      }
+    }
+    dma_join();
+  };
+  if (nt > 0) {
+    load(K0, V0, 0);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) asm volatile("" ::"v"(qf[t]), "v"(df[t]));
+    asm volatile("" ::"v"(lse), "v"(delta));
+    dma_join();
+    for (int t = 0; t < nt; t += 2) {
+      tile(K0, V0, K1, V1, t);
+      if (t + 1 < nt) tile(K1, V1, K0, V0, t + 1);
+    }
+  }
+  store_row<T, NB>(a.dq + (row * a.b.Hq + h) * D, acc, a.scale, hh, ok);
+}
+
+constexpr int kQt = 32;  // query rows per step of the dK / dV sweep
+
+// dK, dV: 128 keys of one sequence and key head, 32 per wave (key on the
+// lane), swept by every query head of the group and every query tile that sees
+// them, last tile first.  P and dS feed the next products as they are; Q and
+// dO are read by rows for S and dP and by columns for dV and dK.
+template <class T, int D>
+__global__ __launch_bounds__(256, 2) void packed_dkv_kernel(BwdArgs a) {
+  constexpr int NB = D / 32, NT = D / 16;
+  constexpr int kImg = kQt * D * 2;
+  __shared__ __attribute__((aligned(1024))) char Q0[kImg], O0[kImg], Q1[kImg], O1[kImg];
+  __shared__ __attribute__((aligned(1024))) char Vw[kRows * D * 2];
+  __shared__ __attribute__((aligned(256))) float L0[64], L1[64];  // lse and delta of a tile's 32 rows
+  int seq, blk, hkv;
+  if (!pick(a.b, a.b.Hkv, &seq, &blk, &hkv)) return;
+  const int G = a.b.Hq / a.b.Hkv;
+  const int row0 = __builtin_amdgcn_readfirstlane(a.b.cu[seq]);
+  const int len = __builtin_amdgcn_readfirstlane(a.b.cu[seq + 1]) - row0;
+  const int qlen = seq < a.b.N ? len : 0;  // nothing looks at padding
+  const int nblk = (len + kRows - 1) / kRows;
+  const int kb = nblk - 1 - blk;  // the job table's order, mirrored: the first keys sweep longest
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lk = lane & 31, hh = lane >> 5;
+  const int key0 = kb * kRows + w * 32, key = key0 + lk;
+  const bool ok = key < len;
+  const int64_t krow = static_cast<int64_t>(row0) + key;
+
+  const TileDma<D, kQt> dma(w, lane);
+  const TileAddr<D> ad(lane);
+  const int vbytes = static_cast<int>(2 * a.v.row), qbytes = static_cast<int>(2 * a.q.row);
+  const int obytes = 2 * a.b.Hq * D;
+  {
+    const TileDma<D, kRows> vdma(w, lane);
+    const int v0 = kb * kRows;
+    vdma.load(row_buffer(a.v.p + (static_cast<int64_t>(row0) + v0) * a.v.row + hkv * a.v.head, min(kRows, len - v0),
+                         vbytes), vbytes, Vw);
+  }
+  bf16x8 kf[NT];
+  {
+    const u16* kp = a.k.p + krow * a.k.row + hkv * a.k.head;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) kf[t] = ok ? *reinterpret_cast<const bf16x8*>(kp + 16 * t + 8 * hh) : bf16x8{};
+  }
+  f32x16 dka[NB], dva[NB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i) dka[i] = dva[i] = f32x16{};
+
+  const int nq = (qlen + kQt - 1) / kQt;
+  const int first = a.causal ? kb * (kRows / kQt) : 0;
+  const int total = max(0, nq - first) * G;
+  auto load = [&](char* Qd, char* Od, float* Ld, int qt, int g) {
+    const int h = hkv * G + g, s0 = qt * kQt, rows = min(kQt, qlen - s0);
+    const int64_t r = static_cast<int64_t>(row0) + s0;
+    dma.load(row_buffer(a.q.p + r * a.q.row + h * a.q.head, rows, qbytes), qbytes, Qd);
+    dma.load(row_buffer(a.dout + (r * a.b.Hq + h) * D, rows, obytes), obytes, Od);
+    if (w < 2 && lane < 32) {  // wave 0: lse, wave 1: delta
+      const float* src = (w == 0 ? a.lse : a.delta) + static_cast<int64_t>(h) * a.b.T + r;
+      dma_lane<4>(row_buffer(src, rows, 4), 4 * lane, Ld + 32 * w);
+    }
+  };
+  int qt = nq - 1, g = 0;
+  auto step = [&](const char* Qc, const char* Oc, const float* Lc, char* Qn, char* On, float* Ln, bool more) {
+    const int g2 = g + 1 == G ? 0 : g + 1, qt2 = g2 == 0 ? qt - 1 : qt;
+    if (more) load(Qn, On, Ln, qt2, g2);
+    const int qb = qt * kQt;
+    if (key0 < len && (!a.causal || qb + kQt - 1 >= key0)) {  // else every query here precedes our keys
+      f32x16 s = f32x16{}, p;
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4) {
+        const f32x4 de = *reinterpret_cast<const f32x4*>(Lc + 32 + 8 * g4 + 4 * hh);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[4 * g4 + j] = -de[j];
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        s = mfma32<T>(ad.rows(Qc, 0, t), kf[t], s);
+        p = mfma32<T>(ad.rows(Oc, 0, t), ad.rows(Vw, 32 * w, t), p);
+      }
+      const bool edge = a.causal && key0 + 31 > qb;
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4) {
+        const f32x4 ls = *reinterpret_cast<const f32x4*>(Lc + 8 * g4 + 4 * hh);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = 4 * g4 + j;
+          float e = exp2_fast(fmaf(s[r], a.c, -ls[j]));
+          float ds = e * p[r];
+          if (edge && key > qb + tile_row(r, hh)) e = ds = 0.f;
+          s[r] = e;
+          p[r] = ds;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        u32x4 pw, sw;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          pw[j] = pack2<T>(s[8 * u + 2 * j], s[8 * u + 2 * j + 1]);
+          sw[j] = pack2<T>(p[8 * u + 2 * j], p[8 * u + 2 * j + 1]);
+        }
+#pragma unroll
+        for (int db = 0; db < NB; ++db) {
+          dva[db] = mfma32<T>(ad.cols(Oc, 16 * u, db), as_op(pw), dva[db]);
+          dka[db] = mfma32<T>(ad.cols(Qc, 16 * u, db), as_op(sw), dka[db]);
+        }
+      }
+    }
+    dma_join();
+    g = g2;
+    qt = qt2;
+  };
+  if (total > 0) {
+    load(Q0, O0, L0, qt, g);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) asm volatile("" ::"v"(kf[t]));
+    dma_join();
+    for (int it = 0; it < total; it += 2) {
+      step(Q0, O0, L0, Q1, O1, L1, it + 1 < total);
+      if (it + 1 < total) step(Q1, O1, L1, Q0, O0, L0, it + 2 < total);
+    }
+  } else {
+    dma_join();  // the V image's DMA ends before the workgroup does
+  }
+  const int64_t off = (krow * a.b.Hkv + hkv) * D;
+  store_row<T, NB>(a.dk + off, dka, a.scale, hh, ok);
+  store_row<T, NB>(a.dv + off, dva, 1.f, hh, ok);
+}
+
+// Strides fit the kernels' 32-bit offsets inside a tile of 128 rows.
+inline bool view_ok(const void* p, int64_t row, int64_t head) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && row % 8 == 0 && head % 8 == 0 && row >= 0 && head >= 0 &&
+         row <= (1 << 22);
+}
+
+inline bool shape_ok(int N, int T, int J, int Hq, int Hkv, int D, int dtype) {
+  return N >= 0 && T > 0 && J > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && (D == 64 || D == 128) &&
+         (dtype == kTypeBf16 || dtype == kTypeFp16) && static_cast<int64_t>(J) * Hq < (1LL << 31) &&
+         static_cast<int64_t>(Hq) * D < (1 << 22);
+}
+
+template <class T, int D>
+int fwd(const FwdArgs& a, int J, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(J) * a.b.Hq);
+  if (a.P > 0) hipLaunchKernelGGL((packed_fwd_kernel<T, D, true>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((packed_fwd_kernel<T, D, false>), grid, dim3(256), 0, s, a);
+  return KGWE_CHECK_LAUNCH();
+}
+
+template <class T, int D>
+int bwd(const BwdArgs& a, int J, hipStream_t s) {
+  hipLaunchKernelGGL((packed_dq_kernel<T, D>), dim3(static_cast<unsigned>(J) * a.b.Hq), dim3(256), 0, s, a);
+  if (int rc = KGWE_CHECK_LAUNCH()) return rc;
+  hipLaunchKernelGGL((packed_dkv_kernel<T, D>), dim3(static_cast<unsigned>(J) * a.b.Hkv), dim3(256), 0, s, a);
+  return KGWE_CHECK_LAUNCH();
+}
+
+}  // namespace
+
+// Row / head strides in elements.  cu [N + 2] and jobs [J, 2] from
+// kgwe_packed_plan for the same N and T.  Prefix keys / values [Hkv, P, D] by
+// strides (P = 0: none).  o contiguous [T, Hq, D]; lse [Hq, T] or null.
+KGWE_API int kgwe_packed_attn_fwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
+                                  int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const void* pk,
+                                  int64_t pk_row, int64_t pk_head, const void* pv, int64_t pv_row, int64_t pv_head,
+                                  int P, void* o, float* lse, const int* cu, const int* jobs, int J, int N, int T,
+                                  int Hq, int Hkv, int D, float scale, int causal, int dtype, hipStream_t s) {
+  if (!shape_ok(N, T, J, Hq, Hkv, D, dtype) || P < 0) return -1;
+  if (!view_ok(q, q_row, q_head) || !view_ok(k, k_row, k_head) || !view_ok(v, v_row, v_head)) return -1;
+  if (P > 0 && (!pk || !pv || !view_ok(pk, pk_row, pk_head) || !view_ok(pv, pv_row, pv_head))) return -1;
+  if (reinterpret_cast<uintptr_t>(o) & 15) return -1;
+  const FwdArgs a{{cu, reinterpret_cast<const int2*>(jobs), N, T, Hq, Hkv},
+                  {static_cast<const u16*>(q), q_row, q_head}, {static_cast<const u16*>(k), k_row, k_head},
+                  {static_cast<const u16*>(v), v_row, v_head}, {static_cast<const u16*>(pk), pk_row, pk_head},
+                  {static_cast<const u16*>(pv), pv_row, pv_head}, static_cast<u16*>(o), lse, P, causal,
+                  scale * kLog2e};
+  if (dtype == kTypeBf16) return D == 64 ? fwd<Bf16, 64>(a, J, s) : fwd<Bf16, 128>(a, J, s);
+  return D == 64 ? fwd<Fp16, 64>(a, J, s) : fwd<Fp16, 128>(a, J, s);
+}
+
+// o, lse: the forward's; dout contiguous [T, Hq, D]; delta fp32 [Hq, T]
+// workspace; dq [T, Hq, D], dk, dv [T, Hkv, D] contiguous, every row written.
+KGWE_API int kgwe_packed_attn_bwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
+                                  int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const void* o,
+                                  const float* lse, const void* dout, float* delta, void* dq, void* dk, void* dv,
+                                  const int* cu, const int* jobs, int J, int N, int T, int Hq, int Hkv, int D,
+                                  float scale, int causal, int dtype, hipStream_t s) {
+  if (!shape_ok(N, T, J, Hq, Hkv, D, dtype) || !lse || !delta) return -1;
+  if (!view_ok(q, q_row, q_head) || !view_ok(k, k_row, k_head) || !view_ok(v, v_row, v_head)) return -1;
+  for (const void* p : {o, dout, static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv)})
+    if (!p || (reinterpret_cast<uintptr_t>(p) & 15)) return -1;
+  const BwdArgs a{{cu, reinterpret_cast<const int2*>(jobs), N, T, Hq, Hkv},
+                  {static_cast<const u16*>(q), q_row, q_head}, {static_cast<const u16*>(k), k_row, k_head},
+                  {static_cast<const u16*>(v), v_row, v_head}, static_cast<const u16*>(o),
+                  static_cast<const u16*>(dout), lse, delta, static_cast<u16*>(dq), static_cast<u16*>(dk),
+                  static_cast<u16*>(dv), causal, scale * kLog2e, scale};
+  if (dtype == kTypeBf16) return D == 64 ? bwd<Bf16, 64>(a, J, s) : bwd<Bf16, 128>(a, J, s);
+  return D == 64 ? bwd<Fp16, 64>(a, J, s) : bwd<Fp16, 128>(a, J, s);
+}
