@@ -43,12 +43,12 @@ HIP_FLAGS = [
     # does not know the feature; harmless.)
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
 ]
-# Per-source extras.  flash_attn.hip: no SLP vectorisation — hipcc otherwise
+# Per-source extras.  The attention kernels: no SLP vectorisation — hipcc otherwise
 # packs the softmax's adjacent f32 adds / multiplies into v_pk_*_f32, which
 # costs more than two plain VALU ops when issued beside MFMAs
 # (MI355X_MICROARCH.md); outputs are bit-identical, fwd / bwd +0.5-1 %
 # (`tools/gpu.sh fa-variants`, variant "noslp").
-HIP_FILE_FLAGS = {"flash_attn.hip": ["-fno-slp-vectorize"], "packed_attn.hip": ["-fno-slp-vectorize"]}
+HIP_FILE_FLAGS = {f: ["-fno-slp-vectorize"] for f in ("flash_attn.hip", "packed_attn.hip", "prefix_attn.hip")}
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-Wextra",
              "-Wno-unused-parameter"]
 

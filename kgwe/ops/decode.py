@@ -5,6 +5,10 @@
 * ``decode_attention`` — split-K GQA attention of one query token per
   sequence over the cache (HBM-bound; one workgroup per (sequence, kv head,
   key chunk) serves all query heads of the group);
+* ``norm_rope_append`` — the same append with the norms of q / k heads, also
+  for all rows of a packed prompt;
+* ``PrefixDecodeAttention`` — the decode attention of a batch whose sequences
+  share a prefix, read once for all of them (``native/ops/prefix_attn.hip``);
 * ``gemv`` — the decode step's projections as weight-streaming skinny GEMMs
   with the layer's RMSNorm (+ residual add), SwiGLU and greedy argmax fused
   in: M <= 8 rows on the vector ALU (``native/ops/gemv.hip``), 8 < M <= 32 —
@@ -62,6 +66,22 @@ def decode_attention_reference(q, kc, vc, lens):
         v = vc[b, :, :n].float().repeat_interleave(hq // hkv, dim=0)
         sc = torch.einsum("hd,hnd->hn", q[b].float(), k) / math.sqrt(d)
         out[b] = torch.einsum("hn,hnd->hd", sc.softmax(-1), v).to(q.dtype)
+    return out
+
+
+def prefix_attention_reference(q, pk, pv, kc, vc, lens):
+    """q [B,Hq,D], prefix [Hkv,P,D], caches [B,Hkv,Smax,D], lens [B] -> [B,Hq,D]
+    (fp32 math; a row without any key gives zeros)."""
+    B, hq, d = q.shape
+    hkv, smax = kc.shape[1], kc.shape[2]
+    out = torch.zeros_like(q)
+    for b in range(B):
+        n = min(max(int(lens[b]), 0), smax)
+        k = torch.cat([pk.float(), kc[b, :, :n].float()], 1).repeat_interleave(hq // hkv, dim=0)
+        v = torch.cat([pv.float(), vc[b, :, :n].float()], 1).repeat_interleave(hq // hkv, dim=0)
+        if k.shape[1]:
+            sc = torch.matmul(k, q[b].float()[:, :, None])[..., 0] / math.sqrt(d)
+            out[b] = torch.matmul(sc.softmax(-1)[:, None], v)[:, 0].to(q.dtype)
     return out
 
 
@@ -190,6 +210,57 @@ class DecodeAttention:
         check(lib().kgwe_decode_attn_rope(ptr(qkv), ptr(cos), ptr(sin), ptr(kc), ptr(vc), ptr(lens),
                                           ptr(self.work), ptr(out), B, hq, hkv, d, self.smax, self.splits,
                                           1.0 / math.sqrt(d), stream(qkv)), "decode_attn_rope")
+        return out
+
+
+class PrefixDecodeAttention:
+    """Decode attention of B sequences that share a prefix of ``prefix_len``
+    keys: row b attends to the prefix's keys / values [Hkv, P, D] and to the
+    first lens[b] entries of its own cache [B, Hkv, Smax, D] (lens of 0: the
+    prefix alone).  The prefix is read once for the whole batch.
+
+    Sized once; nothing depends on lens on the host, so a call can be captured
+    in a hipGraph and replayed at any length.  Each call has a workspace of its
+    own, so one object may be used on several streams and in several graphs.
+    Rows that see no key at all give zeros.  On a GPU: bf16 or fp16, head_dim
+    64 or 128, Hq / Hkv at most 32."""
+
+    def __init__(self, B: int, hq: int, hkv: int, d: int, smax: int, prefix_len: int, device,
+                 dtype: torch.dtype = torch.bfloat16):
+        _require(B > 0 and hkv > 0 and hq > 0 and hq % hkv == 0 and d > 0 and smax >= 0 and prefix_len >= 0
+                 and smax + prefix_len > 0,
+                 "prefix attention: B, heads and head_dim positive, Hq % Hkv == 0, room for at least one key")
+        self.B, self.hq, self.hkv, self.d, self.smax, self.prefix_len = B, hq, hkv, d, smax, prefix_len
+        self.dtype = dtype
+        self.hip = torch.device(device).type == "cuda"
+        if self.hip:
+            _require(dtype in HALF_TYPES, "prefix attention: bf16 or fp16")
+            self.words = int(lib().kgwe_prefix_attn_workspace(B, hq, hkv, d, prefix_len, smax))
+            _require(self.words >= 0, "prefix attention: head_dim 64 or 128 and Hq / Hkv at most 32")
+
+    def __call__(self, q: torch.Tensor, pk: torch.Tensor, pv: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor,
+                 lens: torch.Tensor) -> torch.Tensor:
+        B, hq, hkv, d, smax, P = self.B, self.hq, self.hkv, self.d, self.smax, self.prefix_len
+        _require(q.shape == (B, hq, d), "prefix attention: q must be [B, Hq, D]")
+        _require(pk.shape == pv.shape == (hkv, P, d), "prefix attention: prefix must be [Hkv, P, D]")
+        _require(kc.shape == vc.shape == (B, hkv, smax, d), "prefix attention: cache shape")
+        _require(lens.dtype == torch.int32 and lens.shape == (B,), "prefix attention: lens int32 [B]")
+        _require(all(t.dtype == self.dtype for t in (q, pk, pv, kc, vc))
+                 and all(t.device == q.device for t in (pk, pv, kc, vc, lens)) and q.is_cuda == self.hip,
+                 "prefix attention: one type and one device")
+        if not self.hip:
+            return prefix_attention_reference(q, pk, pv, kc, vc, lens)
+        _require(kc.is_contiguous() and vc.is_contiguous() and kc.data_ptr() % 16 == 0 and vc.data_ptr() % 16 == 0,
+                 "prefix attention: caches must be contiguous and 16-byte aligned")
+        q, pk, pv, lens = rows16(q.contiguous()), rows16(pk), rows16(pv), lens.contiguous()
+        if P > 0 and pk.stride() != pv.stride():  # one pair of strides for both
+            pk, pv = rows16(pk.contiguous()), rows16(pv.contiguous())
+        out = torch.empty_like(q)
+        with torch.cuda.device(q.device):
+            work = torch.empty(self.words, device=q.device, dtype=torch.float32)
+            check(lib().kgwe_prefix_attn(ptr(q), ptr(pk), ptr(pv), max(pk.stride(1), d), pk.stride(0), ptr(kc),
+                                         ptr(vc), ptr(lens), ptr(work), ptr(out), B, hq, hkv, d, P, smax,
+                                         1.0 / math.sqrt(d), HALF_TYPES[q.dtype], stream(q)), "prefix_attn")
         return out
 
 

@@ -1,0 +1,452 @@
+// Attention of one query token per sequence where all sequences of the batch
+// share a prefix: keys = the prefix's [Hkv, P, D], held once, then the
+// sequence's own cache [B, Hkv, Smax, D] up to lens[b].
+//
+//   out[b, h] = sum_j softmax_j(s q[b, h] k_j) v_j,  j over prefix + own keys
+//
+// The bound is HBM: the prefix's keys and values have to be read once per
+// step, not once per sequence.  The rows of one key head, B x G of them (G =
+// Hq / Hkv), are therefore one matrix: a workgroup takes a chunk of the
+// prefix's keys for 128 rows (or for all of them, where there are at most 32)
+// on the matrix cores, another one a chunk of one sequence's own keys for its
+// G rows; a second small launch joins the chunks' (max, sum, output) states.
+// Where prefix and cache are short, one workgroup per (sequence, key head)
+// walks both and nothing is joined.
+//
+// Chunk counts depend on capacities only (P, Smax, B), never on lens, so a
+// step can be captured in a graph and replayed at any length; a workgroup
+// whose chunk lies past its sequence's end leaves at once.
+#include <algorithm>
+
+#include "attn_tile.h"
+
+using namespace kgwe;
+
+namespace {
+
+typedef unsigned short u16;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kDefer = 4.f;  // as in packed_attn.hip
+constexpr int kWide = 64;      // keys per tile of the 128-row form, shared by 4 waves
+constexpr int kSlim = 32;      // keys per tile of the 32-row form, one wave's own
+
+struct Args {
+  const u16* q;   // [B, Hq, D]
+  const u16 *pk, *pv;
+  int64_t p_row, p_head;
+  const u16 *kc, *vc;  // [B, Hkv, Smax, D]
+  const int* lens;
+  u16* out;            // [B, Hq, D]
+  float *part_o, *part_ml;  // [B * Hq, slots, D], [B * Hq, slots, 2]
+  int B, Hq, Hkv, P, Smax;
+  int p_chunk, p_splits, o_chunk, o_splits;  // splits 0: no workgroups of that kind
+  int direct;          // one workgroup walks prefix and own keys and writes out
+  float c;
+};
+
+// State of 32 query rows (row on the lane) over the keys seen so far.
+template <class T, int D>
+struct State {
+  static constexpr int NB = D / 32, NT = D / 16;
+  f32x16 o[NB];
+  float m, l;
+  __device__ __forceinline__ State() : m(-INFINITY), l(0.f) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) o[i] = f32x16{};
+  }
+  // Scores of NS x 32 keys (key on the accumulator's rows), of which the first
+  // `valid` count -> P as the next product's operand.
+  template <int NS>
+  __device__ __forceinline__ void soften(f32x16 (&s)[NS], int valid, float c, int hh, u32x4 (&pb)[2 * NS]) {
+    if (valid < 32 * NS) {
+#pragma unroll
+      for (int st = 0; st < NS; ++st)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (32 * st + tile_row(r, hh) >= valid) s[st][r] = -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int st = 0; st < NS; ++st)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[st][r]);
+    mx = half_max(mx) * c;
+    const float m_new = mx > m + kDefer ? mx : m;
+    const float m_use = m_new == -INFINITY ? 0.f : m_new;
+    if (__any(m_new > m)) {
+      const float alpha = exp2_fast(m - m_use);
+      l *= alpha;
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
+    }
+    m = m_new;
+    float r0 = 0.f, r1 = 0.f;
+#pragma unroll
+    for (int st = 0; st < NS; ++st)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) {
+        const float p0 = exp2_fast(fmaf(s[st][r], c, -m_use)), p1 = exp2_fast(fmaf(s[st][r + 1], c, -m_use));
+        r0 += p0;
+        r1 += p1;
+        pb[2 * st + (r >> 3)][(r & 7) >> 1] = pack2<T>(p0, p1);
+      }
+    l += r0 + r1;
+  }
+};
+
+template <class T, int D>
+__device__ __forceinline__ void load_q(const u16* qrow, bool ok, int hh, bf16x8 (&qf)[D / 16]) {
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t)
+    qf[t] = ok ? *reinterpret_cast<const bf16x8*>(qrow + 16 * t + 8 * hh) : bf16x8{};
+}
+
+// Keys of a walk: n0 rows at k0 / v0, then n1 rows at k1 / v1 (row strides in bytes).
+struct Walk {
+  const u16 *k0, *v0, *k1, *v1;
+  int n0, n1, row0, row1;
+};
+
+template <class T, int D>
+__global__ __launch_bounds__(256, 2) void prefix_attn_kernel(Args a) {
+  constexpr int NB = D / 32, NT = D / 16;
+  constexpr int kImg = kWide * D * 2;  // = two waves' slim tiles
+  __shared__ __attribute__((aligned(1024))) char K0[kImg], V0[kImg], K1[kImg], V1[kImg];
+  __shared__ float ml[4][32][2], joined[32][2];  // (max, sum) of each wave's rows; of all four
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lq = lane & 31, hh = lane >> 5;
+  const int G = a.Hq / a.Hkv, rows_all = a.B * G, slots = a.p_splits + a.o_splits;
+  const bool wide = !a.direct && rows_all > 32;
+  const int tiles = wide ? (rows_all + 127) / 128 : 1;
+  const TileAddr<D> ad(lane);
+
+  // ---- which work: chunk of the prefix (all row tiles of one chunk on one XCD), or of a sequence's own keys
+  const int units = a.p_splits * a.Hkv;
+  const int prefix_wgs = (units + 7) / 8 * 8 * tiles;
+  int i = blockIdx.x;
+  int slot, kvh, nrows, first_row = 0, b = 0;  // first_row: of the rows b * G + g
+  Walk wk{};
+  wk.row0 = static_cast<int>(2 * a.p_row);
+  wk.row1 = 2 * D;
+  if (!a.direct && i < prefix_wgs) {
+    const int base = i / (8 * tiles), rem = i - base * 8 * tiles;
+    const int unit = base * 8 + rem % 8;
+    if (unit >= units) return;
+    slot = unit / a.Hkv;
+    kvh = unit - slot * a.Hkv;
+    first_row = rem / 8 * 128;
+    nrows = min(rows_all - first_row, wide ? 128 : 32);
+    const int64_t at = kvh * a.p_head + static_cast<int64_t>(slot) * a.p_chunk * a.p_row;
+    wk.k0 = a.pk + at;
+    wk.v0 = a.pv + at;
+    wk.n0 = min(a.p_chunk, a.P - slot * a.p_chunk);
+  } else {
+    if (!a.direct) i -= prefix_wgs;
+    const int per = a.direct ? 1 : a.o_splits;
+    const int split = i % per;
+    kvh = i / per % a.Hkv;
+    b = i / per / a.Hkv;
+    first_row = b * G;
+    nrows = G;
+    slot = a.direct ? 0 : a.p_splits + split;
+    const int len = min(max(a.lens[b], 0), a.Smax);
+    const int start = a.direct ? 0 : split * a.o_chunk;
+    wk.n1 = __builtin_amdgcn_readfirstlane(a.direct ? len : min(a.o_chunk, len - start));
+    if (!a.direct && wk.n1 <= 0 && slots > 1) return;
+    wk.n1 = max(wk.n1, 0);
+    const int64_t at = ((static_cast<int64_t>(b) * a.Hkv + kvh) * a.Smax + start) * D;
+    wk.k1 = a.kc + at;
+    wk.v1 = a.vc + at;
+    if (a.direct) {
+      wk.k0 = a.pk + kvh * a.p_head;
+      wk.v0 = a.pv + kvh * a.p_head;
+      wk.n0 = a.P;
+    }
+  }
+  const bool final = a.direct || slots == 1;
+
+  bf16x8 qf[NT];
+  State<T, D> st;
+
+  if (wide && wk.n0 > 0) {
+    // 128 rows, 32 per wave, on tiles of 64 keys that the waves share.
+    const int r = first_row + 32 * w + lq, rb = r / G;
+    const bool ok = 32 * w + lq < nrows;
+    const int64_t qi = static_cast<int64_t>(rb) * a.Hq + kvh * G + (r - rb * G);
+    load_q<T, D>(a.q + qi * D, ok, hh, qf);
+    const bool mine = 32 * w < nrows;
+    const TileDma<D, kWide> dma(w, lane);
+    const int nt = (wk.n0 + kWide - 1) / kWide;
+    auto load = [&](char* Kd, char* Vd, int t) {
+      const int rows = min(kWide, wk.n0 - t * kWide);
+      const int64_t at = static_cast<int64_t>(t) * kWide * a.p_row;
+      dma.load(row_buffer(wk.k0 + at, rows, wk.row0), wk.row0, Kd);
+      dma.load(row_buffer(wk.v0 + at, rows, wk.row0), wk.row0, Vd);
+    };
+    auto tile = [&](const char* Kc, const char* Vc, char* Kn, char* Vn, int t) {
+      if (t + 1 < nt) load(Kn, Vn, t + 1);
+      if (mine) {
+        f32x16 s[2];
+        s[0] = s[1] = f32x16{};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int u = 0; u < NT; ++u) s[h] = mfma32<T>(ad.rows(Kc, 32 * h, u), qf[u], s[h]);
+        u32x4 pb[4];
+        st.template soften<2>(s, wk.n0 - t * kWide, a.c, hh, pb);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int db = 0; db < NB; ++db) st.o[db] = mfma32<T>(ad.cols(Vc, 16 * u, db), as_op(pb[u]), st.o[db]);
+      }
+      dma_join();
+    };
+    load(K0, V0, 0);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) asm volatile("" ::"v"(qf[t]));
+    dma_join();
+    for (int t = 0; t < nt; t += 2) {
+      tile(K0, V0, K1, V1, t);
+      if (t + 1 < nt) tile(K1, V1, K0, V0, t + 1);
+    }
+    const float lt = half_add(st.l);
+    if (final) {
+      store_row<T, NB>(a.out + qi * D, st.o, lt == 0.f ? 0.f : 1.f / lt, hh, ok);
+    } else if (ok) {
+      float* po = a.part_o + (qi * slots + slot) * D;
+#pragma unroll
+      for (int db = 0; db < NB; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          f32x4 v;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = st.o[db][4 * g + j];
+          *reinterpret_cast<f32x4*>(po + 32 * db + 8 * g + 4 * hh) = v;
+        }
+      if (hh == 0) {
+        a.part_ml[(qi * slots + slot) * 2] = st.m;
+        a.part_ml[(qi * slots + slot) * 2 + 1] = lt;
+      }
+    }
+    return;
+  }
+
+  // At most 32 rows: every wave walks tiles of its own (tile index = wave mod
+  // 4) with its own K and V buffer and no barrier: the next K tile is on its
+  // way from the S product on, the next V tile from the O product on.
+  {
+    const int r = first_row + lq, rb = r / G;
+    const int64_t qi = static_cast<int64_t>(rb) * a.Hq + kvh * G + (r - rb * G);
+    load_q<T, D>(a.q + qi * D, lq < nrows, hh, qf);
+  }
+  const TileDma<D, kSlim, 1> dma(0, lane);
+  const int t0 = (wk.n0 + kSlim - 1) / kSlim, nt = t0 + (wk.n1 + kSlim - 1) / kSlim;
+  auto load = [&](bool keys, char* dst, int t) {
+    const bool own = t >= t0;
+    const int at = (own ? t - t0 : t) * kSlim, rows = min(kSlim, (own ? wk.n1 : wk.n0) - at);
+    const int row = own ? wk.row1 : wk.row0;
+    const u16* base = own ? (keys ? wk.k1 : wk.v1) : (keys ? wk.k0 : wk.v0);
+    dma.load(row_buffer(base + static_cast<int64_t>(at) * (row / 2), rows, row), row, dst);
+  };
+  constexpr int kDma = TileDma<D, kSlim, 1>::kN;
+  auto walk = [&](char* Kb, char* Vb) {
+    if (w >= nt) return;
+    load(true, Kb, w);
+    load(false, Vb, w);
+    for (int t = w; t < nt; t += 4) {
+      const bool more = t + 4 < nt;
+      f32x16 s[1];
+      s[0] = f32x16{};
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kDma) : "memory");  // K has landed, V may be on its way
+#pragma unroll
+      for (int u = 0; u < NT; ++u) s[0] = mfma32<T>(ad.rows(Kb, 0, u), qf[u], s[0]);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read: its buffer is free
+      if (more) load(true, Kb, t + 4);
+      u32x4 pb[2];
+      st.template soften<1>(s, t >= t0 ? wk.n1 - (t - t0) * kSlim : wk.n0 - t * kSlim, a.c, hh, pb);
+      if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kDma) : "memory");  // V has landed, the next K may be on its way
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int db = 0; db < NB; ++db) st.o[db] = mfma32<T>(ad.cols(Vb, 16 * u, db), as_op(pb[u]), st.o[db]);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (more) load(false, Vb, t + 4);
+    }
+  };
+  // Each wave pair in an LDS object of its own, known at compile time.
+  if (w < 2) walk(K0 + (w & 1) * (kImg / 2), V0 + (w & 1) * (kImg / 2));
+  else walk(K1 + (w & 1) * (kImg / 2), V1 + (w & 1) * (kImg / 2));
+
+  // Join the four waves through LDS: a common max, then the scaled outputs.
+  const float lw = half_add(st.l);
+  if (hh == 0) {
+    ml[w][lq][0] = st.m;
+    ml[w][lq][1] = lw;
+  }
+  __syncthreads();  // also: every wave is done with the tile buffers
+  float M = -INFINITY, L = 0.f;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) M = fmaxf(M, ml[v][lq][0]);
+  const float M_use = M == -INFINITY ? 0.f : M;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) L += ml[v][lq][1] * exp2_fast(ml[v][lq][0] - M_use);
+  {
+    // Row lq of this wave's [32][D] fp32 region, its 16-byte pieces XOR-swizzled
+    // by the row (rows are a multiple of all banks apart).
+    constexpr int kPieces = D / 4;
+    char* reg = w == 0 ? K0 : w == 1 ? V0 : w == 2 ? K1 : V1;
+    const float mul = exp2_fast(st.m - M_use);
+    if (lq < nrows) {
+#pragma unroll
+      for (int db = 0; db < NB; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          f32x4 v;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = st.o[db][4 * g + j] * mul;
+          const int piece = 8 * db + 2 * g + hh;
+          *reinterpret_cast<f32x4*>(reg + lq * D * 4 + 16 * (piece ^ (lq & (kPieces - 1)))) = v;
+        }
+      if (w == 0 && hh == 0) {
+        joined[lq][0] = M;
+        joined[lq][1] = L;
+      }
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < nrows * kPieces; e += 256) {
+      const int row = e / kPieces, piece = e - row * kPieces;
+      const int off = row * D * 4 + 16 * (piece ^ (row & (kPieces - 1)));
+      const f32x4 v = (*reinterpret_cast<const f32x4*>(K0 + off) + *reinterpret_cast<const f32x4*>(V0 + off)) +
+                      (*reinterpret_cast<const f32x4*>(K1 + off) + *reinterpret_cast<const f32x4*>(V1 + off));
+      const int rr = first_row + row, rb = rr / G;
+      const int64_t qi = static_cast<int64_t>(rb) * a.Hq + kvh * G + (rr - rb * G);
+      const float Lr = joined[row][1];
+      if (final) {
+        const float inv = Lr == 0.f ? 0.f : 1.f / Lr;
+        u16x4 y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = T::down(v[j] * inv);
+        *reinterpret_cast<u16x4*>(a.out + qi * D + 4 * piece) = y;
+      } else {
+        *reinterpret_cast<f32x4*>(a.part_o + (qi * slots + slot) * D + 4 * piece) = v;
+        if (piece == 0) {
+          a.part_ml[(qi * slots + slot) * 2] = joined[row][0];
+          a.part_ml[(qi * slots + slot) * 2 + 1] = Lr;
+        }
+      }
+    }
+  }
+}
+
+// Join the slots of one (b, h) per wave: the prefix's, then those of the own
+// chunks that hold keys.
+template <class T, int D>
+__global__ __launch_bounds__(256) void prefix_join_kernel(Args a) {
+  constexpr int E = D / 64;  // outputs per lane
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (row >= a.B * a.Hq) return;
+  const int b = row / a.Hq, slots = a.p_splits + a.o_splits;
+  const int len = min(max(a.lens[b], 0), a.Smax);
+  const int n = a.p_splits + (a.o_splits > 0 ? (len + a.o_chunk - 1) / a.o_chunk : 0);
+  const float* ml = a.part_ml + static_cast<int64_t>(row) * slots * 2;
+  const float* po = a.part_o + static_cast<int64_t>(row) * slots * D + E * lane;
+  float M = -INFINITY;
+  for (int s = lane; s < n; s += 64) M = fmaxf(M, ml[2 * s]);
+  M = wave_max(M);
+  if (M == -INFINITY) M = 0.f;
+  float L = 0.f, o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < n; ++s) {
+    const float f = exp2_fast(ml[2 * s] - M);
+    L += f * ml[2 * s + 1];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] += f * po[static_cast<int64_t>(s) * D + e];
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+  for (int e = 0; e < E; ++e) a.out[static_cast<int64_t>(row) * D + E * lane + e] = T::down(o[e] * inv);
+}
+
+// Chunks.  Numbers of workgroups are per (key head, row tile) or (key head,
+// sequence); the chip holds 512 of them (2 per CU).
+struct Plan {
+  int direct, p_chunk, p_splits, o_chunk, o_splits;
+};
+
+Plan make_plan(int B, int Hq, int Hkv, int P, int Smax) {
+  Plan p{};
+  const int rows = B * (Hq / Hkv), tiles = rows > 32 ? (rows + 127) / 128 : 1;
+  p.direct = P + Smax <= 512;
+  if (p.direct) return p;
+  auto split = [](int64_t n, int units, int least, int* chunk, int* splits) {
+    *splits = 0;
+    *chunk = least;
+    if (n <= 0) return;
+    const int64_t want = std::max<int64_t>(1, 512 / units);
+    const int64_t c = std::max<int64_t>(least, ((n + want - 1) / want + 63) / 64 * 64);
+    *chunk = static_cast<int>(c);
+    *splits = static_cast<int>((n + c - 1) / c);
+  };
+  split(P, Hkv * tiles, rows > 32 ? 256 : 128, &p.p_chunk, &p.p_splits);
+  split(Smax, B * Hkv, 256, &p.o_chunk, &p.o_splits);
+  return p;
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <class T, int D>
+int launch(Args a, hipStream_t s) {
+  const int G = a.Hq / a.Hkv, rows = a.B * G, tiles = !a.direct && rows > 32 ? (rows + 127) / 128 : 1;
+  const int64_t grid = a.direct ? static_cast<int64_t>(a.B) * a.Hkv
+                                : static_cast<int64_t>((a.p_splits * a.Hkv + 7) / 8 * 8) * tiles +
+                                      static_cast<int64_t>(a.B) * a.Hkv * a.o_splits;
+  if (grid <= 0 || grid > 0x7fffffff) return -1;
+  hipLaunchKernelGGL((prefix_attn_kernel<T, D>), dim3(static_cast<unsigned>(grid)), dim3(256), 0, s, a);
+  int rc = KGWE_CHECK_LAUNCH();
+  if (rc || a.direct || a.p_splits + a.o_splits == 1) return rc;
+  hipLaunchKernelGGL((prefix_join_kernel<T, D>), dim3((a.B * a.Hq + 3) / 4), dim3(256), 0, s, a);
+  return KGWE_CHECK_LAUNCH();
+}
+
+inline bool shape_ok(int B, int Hq, int Hkv, int D, int P, int Smax) {
+  return B > 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= 32 && (D == 64 || D == 128) && P >= 0 &&
+         Smax >= 0 && P + static_cast<int64_t>(Smax) > 0 && P < (1 << 30) && Smax < (1 << 30) &&
+         static_cast<int64_t>(B) * Hq < (1 << 24);
+}
+
+}  // namespace
+
+// fp32 words of workspace that a call needs (0: none), -1: unsupported shape.
+KGWE_API int64_t kgwe_prefix_attn_workspace(int B, int Hq, int Hkv, int D, int P, int Smax) {
+  if (!shape_ok(B, Hq, Hkv, D, P, Smax)) return -1;
+  const Plan p = make_plan(B, Hq, Hkv, P, Smax);
+  const int slots = p.p_splits + p.o_splits;
+  return p.direct || slots == 1 ? 0 : static_cast<int64_t>(B) * Hq * slots * (D + 2);
+}
+
+// q, out contiguous [B, Hq, D]; prefix [Hkv, P, D] by strides (elements, both
+// tensors alike); caches contiguous [B, Hkv, Smax, D]; lens int32 [B], cut to
+// [0, Smax].  The workspace needs no clearing and is the call's own.
+KGWE_API int kgwe_prefix_attn(const void* q, const void* pk, const void* pv, int64_t p_row, int64_t p_head,
+                              const void* kc, const void* vc, const int* lens, float* work, void* out, int B, int Hq,
+                              int Hkv, int D, int P, int Smax, float scale, int dtype, hipStream_t s) {
+  if (!shape_ok(B, Hq, Hkv, D, P, Smax) || (dtype != kTypeBf16 && dtype != kTypeFp16)) return -1;
+  if (P > 0 && (!pk || !pv || !aligned16(pk) || !aligned16(pv) || p_row % 8 || p_head % 8 || p_row < D ||
+                p_row > (1 << 22) || p_head < 0))
+    return -1;
+  if (!aligned16(q) || !aligned16(out) || !aligned16(kc) || !aligned16(vc) || !aligned16(work)) return -1;
+  const Plan p = make_plan(B, Hq, Hkv, P, Smax);
+  const int slots = p.p_splits + p.o_splits;
+  if (!p.direct && slots > 1 && !work) return -2;
+  float* ml = work + static_cast<int64_t>(B) * Hq * slots * D;
+  const Args a{static_cast<const u16*>(q), static_cast<const u16*>(pk), static_cast<const u16*>(pv), p_row, p_head,
+               static_cast<const u16*>(kc), static_cast<const u16*>(vc), lens, static_cast<u16*>(out), work, ml, B,
+               Hq, Hkv, P, Smax, p.p_chunk, p.p_splits, p.o_chunk, p.o_splits, p.direct, scale * kLog2e};
+  if (dtype == kTypeBf16) return D == 64 ? launch<Bf16, 64>(a, s) : launch<Bf16, 128>(a, s);
+  return D == 64 ? launch<Fp16, 64>(a, s) : launch<Fp16, 128>(a, s);
+}

@@ -395,3 +395,90 @@ def test_norm_rope_gpu_refusals():
         norm_rope_qkv(torch.zeros(2, 3 * 64, device="cuda", dtype=torch.bfloat16), cos, sin, pos.cpu(), 1, 1, 64)
     empty = norm_rope_qkv(torch.zeros(0, 3 * 64, device="cuda", dtype=torch.bfloat16), cos, sin, pos[:0], 1, 1, 64)
     assert [t.shape for t in empty] == [(0, 1, 64)] * 3
+
+
+# ------------------------------------------------------------------ single tokens behind a shared prefix
+def _exact_prefix(q, pk, pv, kc, vc, lens):
+    h, tiny = HALF[q.dtype], TINY[q.dtype]
+    out, tol = torch.zeros_like(q, dtype=torch.float64), torch.zeros_like(q, dtype=torch.float64)
+    G = q.shape[1] // kc.shape[1]
+    for b, n in enumerate(lens.tolist()):
+        for j in range(kc.shape[1]):
+            k = torch.cat([pk[j], kc[b, j, :n]]).double()
+            v = torch.cat([pv[j], vc[b, j, :n]]).double()
+            if not len(k):
+                continue
+            r = slice(j * G, (j + 1) * G)
+            p = torch.softmax(q[b, r].double() @ k.T / math.sqrt(q.shape[2]), 1)
+            out[b, r] = p @ v
+            tol[b, r] = h * out[b, r].abs() + (h + SLOP) * (p @ v.abs()) + tiny * (1 + len(k) * v.abs().max())
+    return out, tol
+
+
+@pytest.mark.parametrize("B,hq,hkv,d,smax,P,lens", [
+    (1, 4, 2, 64, 16, 7, [0]), (3, 32, 8, 128, 300, 100, [0, 300, 33]),      # one workgroup walks both
+    (4, 8, 2, 64, 700, 129, [1, 700, 256, 0]), (2, 14, 2, 128, 64, 1000, [64, 3]),  # at most 32 rows a key head
+    (40, 8, 4, 128, 300, 515, [0, 300, 257, 256] * 10), (33, 4, 4, 64, 16, 4000, [16, 0, 5] * 11),
+    (70, 12, 4, 64, 260, 1030, [260, 1] * 35), (9, 32, 1, 128, 600, 300, [600, 0, 1] * 3),  # row tiles of 128
+    (3, 4, 4, 64, 900, 0, [0, 900, 5]), (5, 64, 8, 64, 0, 600, [0] * 5), (2, 4, 4, 128, 0, 9, [0, 0]),
+])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_prefix_attention(B, hq, hkv, d, smax, P, lens, dtype):
+    g = torch.Generator(device="cuda").manual_seed(B + P)
+    q = _rnd(g, B, hq, d, dtype=dtype)
+    room = torch.full((2, hkv, P + 5, d), float("nan"), device="cuda", dtype=dtype)  # the prefix inside a longer buffer
+    room[:, :, :P] = _rnd(g, 2, hkv, P, d, dtype=dtype)
+    kc, vc = _rnd(g, B, hkv, smax, d, dtype=dtype), _rnd(g, B, hkv, smax, d, dtype=dtype)
+    ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    for b, n in enumerate(lens):  # what lies past a row's length is never looked at
+        kc[b, :, n:], vc[b, :, n:] = float("nan"), float("inf")
+    att = dec.PrefixDecodeAttention(B, hq, hkv, d, smax, P, "cuda", dtype=dtype)
+    got = att(q, room[0, :, :P], room[1, :, :P], kc, vc, ln)
+    _within(got, *_exact_prefix(q, room[0, :, :P], room[1, :, :P], kc, vc, ln), "o")
+    # other strides, lengths out of range, again: the same bits
+    ln2 = torch.where(ln == smax, ln + 77, torch.where(ln == 0, ln - 3, ln)).to(torch.int32)
+    again = att(q, room[0, :, :P].contiguous(), room[1, :, :P], kc, vc, ln2)
+    assert torch.equal(got, again)
+
+
+def test_prefix_attention_growing_scores_and_replays():
+    g = torch.Generator(device="cuda").manual_seed(3)
+    B, hq, hkv, d, smax, P = 20, 16, 4, 64, 600, 2000
+    q = _rnd(g, B, hq, d, scale=3.0)
+    grow = torch.linspace(0.1, 5, P, device="cuda")[None, :, None]
+    pk, pv = (torch.randn(hkv, P, d, device="cuda", generator=g) * grow).bfloat16(), _rnd(g, hkv, P, d)
+    kc, vc = _rnd(g, B, hkv, smax, d), _rnd(g, B, hkv, smax, d)
+    lens = torch.full((B,), 600, dtype=torch.int32, device="cuda")
+    att = dec.PrefixDecodeAttention(B, hq, hkv, d, smax, P, "cuda")
+    _within(att(q, pk, pv, kc, vc, lens), *_exact_prefix(q, pk, pv, kc, vc, lens), "o")
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    outs = []
+    for graph in graphs:  # two graphs of one object
+        with torch.cuda.graph(graph):
+            outs.append(att(q, pk, pv, kc, vc, lens))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for n in (600, 0, 1, 333):
+        lens.fill_(n)
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):  # replayed at the same time
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        want = att(q, pk, pv, kc, vc, lens)
+        assert all(torch.equal(o, want) for o in outs), n
+
+
+def test_prefix_attention_gpu_refusals():
+    for bad in ((1, 4, 2, 32, 8, 8), (1, 66, 2, 64, 8, 8)):
+        with pytest.raises(ValueError):
+            dec.PrefixDecodeAttention(*bad, "cuda")
+    with pytest.raises(ValueError):
+        dec.PrefixDecodeAttention(1, 4, 2, 64, 8, 8, "cuda", dtype=torch.float32)
+    att = dec.PrefixDecodeAttention(1, 4, 2, 64, 8, 8, "cuda")
+    z = lambda *s: torch.zeros(*s, device="cuda", dtype=torch.bfloat16)  # noqa: E731
+    with pytest.raises(ValueError):
+        att(z(1, 4, 64), z(2, 8, 64), z(2, 8, 64), z(1, 2, 8, 64), z(1, 2, 64, 8).transpose(2, 3),
+            torch.zeros(1, dtype=torch.int32, device="cuda"))
+    with pytest.raises(ValueError):
+        att(z(1, 4, 64), z(2, 8, 64), z(2, 8, 64), z(1, 2, 8, 64), z(1, 2, 8, 64), torch.zeros(1, dtype=torch.int32))

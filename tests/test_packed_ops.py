@@ -149,3 +149,30 @@ def test_norm_rope_reference_gradient_matches_differences():
     want = (qkv.grad * step[0]).sum() + (w.grad * step[1]).sum()
     assert abs(diff - want) < 2e-2 * max(1.0, abs(want))
     assert not qkv.grad[2].any()
+
+
+def test_prefix_attention_reference_is_decode_attention_behind_a_prefix():
+    B, hq, hkv, d, smax, P = 3, 4, 2, 16, 9, 5
+    g = torch.Generator().manual_seed(2)
+    q, pk, pv = (torch.randn(*s, generator=g) for s in ((B, hq, d), (hkv, P, d), (hkv, P, d)))
+    kc, vc = torch.randn(B, hkv, smax, d, generator=g), torch.randn(B, hkv, smax, d, generator=g)
+    lens = torch.tensor([0, 4, 9], dtype=torch.int32)
+    got = dec.PrefixDecodeAttention(B, hq, hkv, d, smax, P, "cpu", dtype=torch.float32)(q, pk, pv, kc, vc, lens)
+    whole = [torch.cat([p.expand(B, -1, -1, -1), c], 2) for p, c in ((pk, kc), (pv, vc))]
+    assert torch.allclose(got, dec.decode_attention_reference(q, *whole, lens + P), atol=1e-5)
+    none = dec.PrefixDecodeAttention(B, hq, hkv, d, smax, 0, "cpu", dtype=torch.float32)(
+        q, pk[:, :0], pv[:, :0], kc, vc, lens)
+    assert not none[0].any()  # a row without any key
+
+
+def test_prefix_attention_refusals():
+    for bad in ((0, 4, 2, 64, 8, 8), (1, 3, 2, 64, 8, 8), (1, 4, 2, 64, 0, 0), (1, 4, 2, 64, -1, 8)):
+        with pytest.raises(ValueError):
+            dec.PrefixDecodeAttention(*bad, "cpu")
+    att = dec.PrefixDecodeAttention(1, 4, 2, 16, 8, 5, "cpu", dtype=torch.float32)
+    q, p, c = torch.zeros(1, 4, 16), torch.zeros(2, 5, 16), torch.zeros(1, 2, 8, 16)
+    lens = torch.zeros(1, dtype=torch.int32)
+    for args in ((q[:, :2], p, p, c, c, lens), (q, p[:, :4], p[:, :4], c, c, lens), (q, p, p, c[:, :, :7], c[:, :, :7], lens),
+                 (q, p, p, c, c, lens.long()), (q, p.double(), p, c, c, lens), (q, p, p, c, c, lens[:0])):
+        with pytest.raises(ValueError):
+            att(*args)
