@@ -7,7 +7,9 @@ sampling) and by ``__graft_entry__.smoke``.
 """
 from __future__ import annotations
 
+import math
 import os
+import random
 import sys
 import time
 from dataclasses import dataclass
@@ -15,7 +17,7 @@ from dataclasses import dataclass
 import torch
 
 from ..models import llama
-from ..ops import FusedAdamW
+from ..ops import FusedAdamW, PackedBatch
 from ..parallel import dist as kdist
 from ..parallel.checkpoint import Checkpointer
 from ..parallel.fsdp import shard_model
@@ -37,6 +39,10 @@ class TrainConfig:
     # "none": single process, no process group.
     parallel: str = "zero"
     data: str = "random"  # "random": fresh uniform tokens each step; "fixed": one batch
+    # > 0: the step's micro_batch * seq_len tokens are documents of up to so many
+    # tokens packed on one axis (attention stays inside a document); 0: a
+    # rectangular batch
+    doc_len: int = 0
     seed: int = 1234
     ckpt_dir: str | None = None  # sharded checkpoints (kgwe.parallel.checkpoint); resume if present
     ckpt_every: int = 0          # steps between checkpoints (0: only at the end of run())
@@ -86,6 +92,8 @@ class Trainer:
         self._gen = torch.Generator(device=dev).manual_seed(tc.seed + info.rank)
         self.tokens = torch.empty((tc.micro_batch, tc.seq_len + 1), dtype=torch.long, device=dev)
         self.tokens.random_(0, self.cfg.vocab_size, generator=self._gen)
+        if tc.doc_len < 0 or tc.doc_len == 1:
+            raise ValueError("doc_len: 0, or at least 2 tokens")
         self.last_loss: torch.Tensor | None = None
         self.global_step = 0
         self.ckpt = None
@@ -112,11 +120,32 @@ class Trainer:
         if self.tc.data == "random":
             self.tokens.random_(0, self.cfg.vocab_size, generator=self._gen)
 
+    def doc_lengths(self) -> list[int]:
+        """Document lengths of the current step, log-uniform in [2, doc_len],
+        that fill the token axis; the same for the same seed, rank and step."""
+        rng = random.Random((self.tc.seed, self.info.rank, self.global_step).__repr__())
+        left, out = self.tokens_per_step, []
+        while left > 0:
+            n = min(left, round(math.exp(rng.uniform(math.log(2), math.log(self.tc.doc_len)))))
+            out.append(n)
+            left -= n
+        return out
+
+    def _packed_loss(self) -> torch.Tensor:
+        """Next-token loss of documents packed on one axis: the last token of a
+        document predicts nothing."""
+        tok = self.tokens[:, :-1].reshape(-1)
+        batch = PackedBatch(self.doc_lengths(), device=tok.device)
+        labels = torch.cat([tok[1:], tok[:1]])
+        labels[batch.last_rows.long()] = -100
+        return self.model(tok, labels, batch)
+
     def step(self) -> torch.Tensor:
         self.next_batch()
-        inp = self.tokens[:, :-1]
-        lab = self.tokens[:, 1:]
-        loss = self.model(inp, lab)
+        if self.tc.doc_len:
+            loss = self._packed_loss()
+        else:
+            loss = self.model(self.tokens[:, :-1], self.tokens[:, 1:])
         loss.backward()
         if self.dp is not None:
             self.dp.step()
@@ -176,12 +205,14 @@ def main(argv=None) -> int:
     ap.add_argument("--micro-batch", type=int, default=4)
     ap.add_argument("--steps", type=int, default=100)
     ap.add_argument("--lr", type=float, default=3e-4)
+    ap.add_argument("--doc-len", type=int, default=0,
+                    help="pack documents of up to this many tokens on one axis (0: one sequence per row)")
     ap.add_argument("--ckpt-dir", default=None)
     ap.add_argument("--ckpt-every", type=int, default=0)
     a = ap.parse_args(argv)
     info = kdist.init(force_group=True)
     tr = Trainer(TrainConfig(model=a.model, seq_len=a.seq_len, micro_batch=a.micro_batch, lr=a.lr,
-                             ckpt_dir=a.ckpt_dir, ckpt_every=a.ckpt_every), info)
+                             doc_len=a.doc_len, ckpt_dir=a.ckpt_dir, ckpt_every=a.ckpt_every), info)
     loss = train(tr, a.steps)
     log(info, f"done at step {tr.global_step}: loss {loss:.4f}")
     kdist.shutdown()

@@ -13,6 +13,12 @@ pods"; reference README.md:31 "7x GPU density").
   and replayed — a 1B-parameter decode step is ~200 kernels, launch-bound
   without a graph.
 
+* packed prefill (``prefill_packed``): prompts of different lengths in one
+  pass over one token axis, each into its own cache row;
+* shared prefix (``Generator(prefix=...)``): the prompt that all rows have in
+  common is prefilled once at construction; its keys and values are held once
+  and read once per step for the whole batch.
+
 KV cache: one bf16 tensor [L, B, Hkv, Smax, D] (head-major, so one
 (sequence, kv head) is a contiguous slab the decode kernel streams).
 """
@@ -24,11 +30,17 @@ from ..ops import attn as attn_ops
 from ..ops import decode as dec
 from ..ops import functional as K
 from ..ops import reference as ref
+from ..ops.packed import PackedBatch
 from .llama import Llama
 
 
 class Generator:
-    def __init__(self, model: Llama, batch: int, max_seq: int, keep_logits: bool = False):
+    """Decodes ``batch`` rows with room for ``max_seq`` positions each.
+
+    prefix: token ids (1-D tensor or list) that every row starts with; rows'
+    prompts, positions and ``max_seq`` then count from its end."""
+
+    def __init__(self, model: Llama, batch: int, max_seq: int, keep_logits: bool = False, prefix=None):
         self.m = model
         self.keep_logits = keep_logits
         self.logits = None
@@ -39,9 +51,17 @@ class Generator:
         self.B, self.smax = batch, max_seq
         hq, hkv, d = c.n_heads, c.n_kv_heads, c.head_dim
         self.kv = torch.zeros(2, c.n_layers, batch, hkv, max_seq, d, device=self.dev, dtype=p.dtype)
-        self.cos, self.sin = ref.rope_tables(max_seq, d, c.rope_theta, self.dev)
+        prefix = torch.as_tensor([] if prefix is None else prefix, dtype=torch.long, device=self.dev)
+        if prefix.dim() != 1:
+            raise ValueError("prefix: one row of token ids")
+        self.prefix_len = P = prefix.numel()
+        self.cos, self.sin = ref.rope_tables(P + max_seq, d, c.rope_theta, self.dev)
         self.cos, self.sin = self.cos.float().contiguous(), self.sin.float().contiguous()
-        self.attn = dec.DecodeAttention(batch, hq, hkv, d, max_seq, self.dev)
+        if P:
+            self.attn = dec.PrefixDecodeAttention(batch, hq, hkv, d, max_seq, P, self.dev, dtype=p.dtype)
+        else:
+            self.attn = dec.DecodeAttention(batch, hq, hkv, d, max_seq, self.dev)
+        self.prefix_kv = self._prefill_prefix(prefix) if P else None  # [2, L, Hkv, P, D]
         self.tok = torch.zeros(batch, dtype=torch.long, device=self.dev)
         self.pos = torch.zeros(batch, dtype=torch.int32, device=self.dev)
         self.lens = torch.zeros(batch, dtype=torch.int32, device=self.dev)
@@ -64,6 +84,63 @@ class Generator:
 
     # ------------------------------------------------------------ prefill
     @torch.no_grad()
+    def _prefill_prefix(self, tokens: torch.Tensor) -> torch.Tensor:
+        """Keys and values of the shared prefix, all layers: [2, L, Hkv, P, D]."""
+        c, P = self.cfg, tokens.numel()
+        kv = torch.zeros(2, c.n_layers, 1, c.n_kv_heads, P, c.head_dim, device=self.dev, dtype=self.kv.dtype)
+        self._packed_pass(tokens, PackedBatch([P], device=self.dev), torch.zeros(P, dtype=torch.int32, device=self.dev),
+                          kv, None)
+        return kv[:, :, 0]
+
+    def _packed_pass(self, tokens, batch: PackedBatch, cache_rows, kv, prefix_kv) -> torch.Tensor:
+        """One pass over a packed batch: row t's keys and values go to cache row
+        cache_rows[t] of kv [2, L, R, Hkv, S, D] at its position.  Returns the
+        final hidden states [T, dim]."""
+        c, m = self.cfg, self.m
+        hq, hkv, d = c.n_heads, c.n_kv_heads, c.head_dim
+        T, P = batch.total, 0 if prefix_kv is None else prefix_kv.shape[3]
+        h = m.tok_embeddings(tokens)
+        residual = None
+        for i, layer in enumerate(m.layers):
+            at = layer.attention
+            xn, residual = K.rmsnorm(h, layer.attention_norm, c.norm_eps, residual=residual)
+            q, k, v = dec.norm_rope_append(K.linear(xn, at.wqkv), batch.positions, self.cos, self.sin, kv[0, i], kv[1, i],
+                                           hq, hkv, d, at.q_norm, at.k_norm, c.norm_eps, offset=P, rows=cache_rows,
+                                           keep_kv=True)
+            o = attn_ops.attention_packed(q, k, v, batch, prefix=None if prefix_kv is None else tuple(prefix_kv[:, i]))
+            xn, residual = K.rmsnorm(K.linear(o.view(T, -1), at.wo), layer.ffn_norm, c.norm_eps, residual=residual)
+            h = layer.feed_forward(xn)
+        h, _ = K.rmsnorm(h, m.norm, c.norm_eps, residual=residual)
+        return h
+
+    @torch.no_grad()
+    def prefill_packed(self, prompts: list, rows: list[int]) -> torch.Tensor:
+        """Prompts of different lengths (lists or 1-D tensors of token ids) in
+        ONE pass -> next token of each [n]; prompt i fills cache positions
+        [0, len) of batch row rows[i].  The other rows are left as they are."""
+        prompts = [torch.as_tensor(p, dtype=torch.long) for p in prompts]
+        lens = [p.numel() for p in prompts]
+        if not prompts or len(prompts) != len(rows) or len(set(rows)) != len(rows) or any(
+                p.dim() != 1 for p in prompts) or not all(0 < n < self.smax for n in lens) or not all(
+                0 <= r < self.B for r in rows):
+            raise ValueError(f"prefill_packed: one prompt of 1 .. {self.smax - 1} tokens for each of some of the "
+                             f"{self.B} rows, got lengths {lens} for rows {list(rows)}")
+        tokens = torch.cat([p.to(self.dev) for p in prompts])
+        batch = PackedBatch(lens, device=self.dev)
+        at = torch.tensor(rows, dtype=torch.int32).to(self.dev)
+        hidden = self._packed_pass(tokens, batch, at[batch.seq_ids.long()], self.kv, self.prefix_kv)
+        at = at.long()
+        logits = K.linear(hidden[batch.last_rows.long()], self.m.output)
+        if self.keep_logits and list(rows) == list(range(self.B)):
+            self.logits = logits.clone()
+        nxt = logits.argmax(-1)
+        self.tok[at] = nxt
+        self.pos[at] = batch.lengths
+        self.lens[at] = batch.lengths + 1
+        self.filled = max(max(lens), self.filled) if len(rows) < self.B else max(lens)
+        return nxt
+
+    @torch.no_grad()
     def prefill(self, tokens: torch.Tensor, rows: tuple[int, int] | None = None) -> torch.Tensor:
         """tokens [B, P] -> next token [B]; fills cache positions [0, P).
         With rows=(r0, r1) only batch rows [r0, r1) are prefilled (tokens
@@ -75,6 +152,8 @@ class Generator:
         if not (0 <= r0 < r1 <= self.B) or B != r1 - r0 or P >= self.smax:
             raise ValueError(f"prefill: expected [B={r1 - r0}, P<{self.smax}] for rows {r0}:{r1} of {self.B}, "
                              f"got {tuple(tokens.shape)}")
+        if self.prefix_len:
+            return self.prefill_packed(list(tokens), list(range(r0, r1)))
         hq, hkv, d = c.n_heads, c.n_kv_heads, c.head_dim
         cos, sin = self.cos[:P], self.sin[:P]
         h = m.tok_embeddings(tokens)
@@ -85,7 +164,11 @@ class Generator:
             else:
                 xn, residual = K.rmsnorm(h, layer.attention_norm, c.norm_eps, residual=residual)
             qkv = K.linear(xn, layer.attention.wqkv).view(B * P, -1)
-            q, k, v = K.rope_qkv(qkv, cos, sin, P, hq, hkv, d)
+            if c.qk_norm:
+                q, k, v = K.norm_rope_qkv(qkv, cos, sin, P, hq, hkv, d, layer.attention.q_norm, layer.attention.k_norm,
+                                          c.norm_eps)
+            else:
+                q, k, v = K.rope_qkv(qkv, cos, sin, P, hq, hkv, d)
             k4, v4 = k.view(B, P, hkv, d), v.view(B, P, hkv, d)
             self.kv[0, i, r0:r1, :, :P].copy_(k4.transpose(1, 2))
             self.kv[1, i, r0:r1, :, :P].copy_(v4.transpose(1, 2))
@@ -105,6 +188,20 @@ class Generator:
         return nxt
 
     # ------------------------------------------------------------ decode
+    def _attend(self, i: int, qkv: torch.Tensor) -> torch.Tensor:
+        """Layer i's new token: rotation (and q / k norms), append to the cache,
+        attention.  qkv [B, (hq+2hkv)d] -> [B, hq, d]."""
+        c, at = self.cfg, self.m.layers[i].attention
+        hq, hkv, d = c.n_heads, c.n_kv_heads, c.head_dim
+        kc, vc = self.kv[0, i], self.kv[1, i]
+        if not (c.qk_norm or self.prefix_len):
+            return self.attn.rope_attend(qkv, self.cos, self.sin, kc, vc, self.lens)
+        q = dec.norm_rope_append(qkv, self.pos, self.cos, self.sin, kc, vc, hq, hkv, d, at.q_norm, at.k_norm, c.norm_eps,
+                                 offset=self.prefix_len)
+        if self.prefix_len:
+            return self.attn(q, self.prefix_kv[0, i], self.prefix_kv[1, i], kc, vc, self.lens)
+        return self.attn(q, kc, vc, self.lens)
+
     @torch.no_grad()
     def _step_fused(self) -> None:
         """One decode step in 5 kernels per layer (7 for a serving batch, whose
@@ -113,7 +210,6 @@ class Generator:
         [RMSNorm(+res) -> w13 -> SwiGLU], w2; and [RMSNorm(+res) -> LM head ->
         argmax] at the end."""
         c, m = self.cfg, self.m
-        hq, hkv, d = c.n_heads, c.n_kv_heads, c.head_dim
         B, eps = self.B, c.norm_eps
         x = m.tok_embeddings(self.tok)  # [B, dim]
         res = None
@@ -126,7 +222,7 @@ class Generator:
                 at, ff = layer.attention, layer.feed_forward
                 xn, h = K.rmsnorm(x, layer.attention_norm, eps, residual=res)
                 qkv = dec.gemv(xn, at.wqkv)
-                o = self.attn.rope_attend(qkv, self.cos, self.sin, self.kv[0, i], self.kv[1, i], self.lens)
+                o = self._attend(i, qkv)
                 a = dec.gemv(o.view(B, -1), at.wo)
                 xn, res = K.rmsnorm(a, layer.ffn_norm, eps, residual=h)
                 f = dec.gemv(xn, ff.w13, dec.GEMV_SWIGLU)
@@ -148,7 +244,7 @@ class Generator:
             else:
                 qkv = dec.gemv(x, at.wqkv, dec.GEMV_NORM, res=res, g=layer.attention_norm, eps=eps, h_out=hA)
                 h = hA
-            o = self.attn.rope_attend(qkv, self.cos, self.sin, self.kv[0, i], self.kv[1, i], self.lens)
+            o = self._attend(i, qkv)
             a = dec.gemv(o.view(B, -1), at.wo)
             f = dec.gemv(a, ff.w13, dec.GEMV_NORM_SWIGLU, res=h, g=layer.ffn_norm, eps=eps, h_out=hB)
             x = dec.gemv(f, ff.w2) if self.w2_fused else K.linear(f, ff.w2)
@@ -175,8 +271,8 @@ class Generator:
             else:
                 xn, residual = K.rmsnorm(h, layer.attention_norm, c.norm_eps, residual=residual)
             qkv = K.linear(xn, layer.attention.wqkv)
-            if self.dev.type == "cuda":  # RoPE + cache append inside the attention launch
-                o = self.attn.rope_attend(qkv, self.cos, self.sin, self.kv[0, i], self.kv[1, i], self.lens)
+            if self.dev.type == "cuda" or c.qk_norm or self.prefix_len:
+                o = self._attend(i, qkv)  # on a GPU RoPE + cache append inside the attention launch
             else:
                 q = dec.rope_append(qkv, self.pos, self.cos, self.sin, self.kv[0, i], self.kv[1, i], hq, hkv, d)
                 o = self.attn(q, self.kv[0, i], self.kv[1, i], self.lens)

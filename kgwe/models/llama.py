@@ -11,6 +11,9 @@ parameter count) — so this module is new, written MI355X-first:
 * fused gate|up (w13) projection -> one HIP SwiGLU kernel reading it in place;
 * residual add fused into RMSNorm (one HBM pass instead of two);
 * fused vocabulary cross-entropy (no fp32 logits copy);
+* documents of different lengths train packed on one token axis
+  (``Llama.forward(..., batch=PackedBatch)``): attention stays inside a
+  document, positions start at 0 in each, nothing is padded to a common length;
 * GEMMs are hipBLASLt GEMMs; the weight-gradient GEMMs get their operands
   transposed into the library's fast layouts (``K.linear``).
 """
@@ -24,6 +27,7 @@ import torch.nn as nn
 from ..ops import attn as attn_ops
 from ..ops import functional as K
 from ..ops import reference as ref
+from ..ops.packed import PackedBatch
 
 
 @dataclass(frozen=True)
@@ -38,6 +42,7 @@ class LlamaConfig:
     norm_eps: float = 1e-5
     rope_theta: float = 500000.0
     max_seq_len: int = 8192
+    qk_norm: bool = False  # RMS norm of every query and key head, fused with the rotation
 
     @property
     def head_dim(self) -> int:
@@ -48,7 +53,7 @@ class LlamaConfig:
         hd = self.head_dim
         attn = d * (self.n_heads + 2 * self.n_kv_heads) * hd + self.n_heads * hd * d
         mlp = 3 * d * f
-        per_layer = attn + mlp + 2 * d
+        per_layer = attn + mlp + 2 * d + (2 * hd if self.qk_norm else 0)
         return self.n_layers * per_layer + 2 * v * d + d
 
     def flops_per_token(self, seq_len: int) -> float:
@@ -92,6 +97,11 @@ class RopeCache:
             RopeCache._tables[key] = t
         return t
 
+    def for_batch(self, batch: PackedBatch) -> tuple[torch.Tensor, torch.Tensor]:
+        """Tables long enough for any sequence of a packed batch; their length
+        is rounded up to a power of two, so batches of all sizes share few."""
+        return self(1 << max(batch.total - 1, 1).bit_length(), batch.device)
+
 
 class Attention(nn.Module):
     def __init__(self, cfg: LlamaConfig):
@@ -100,12 +110,24 @@ class Attention(nn.Module):
         hd = cfg.head_dim
         self.wqkv = nn.Parameter(torch.empty((cfg.n_heads + 2 * cfg.n_kv_heads) * hd, cfg.dim))
         self.wo = nn.Parameter(torch.empty(cfg.dim, cfg.n_heads * hd))
+        self.q_norm = nn.Parameter(torch.ones(hd)) if cfg.qk_norm else None
+        self.k_norm = nn.Parameter(torch.ones(hd)) if cfg.qk_norm else None
 
-    def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                batch: PackedBatch | None = None) -> torch.Tensor:
         B, S, _ = x.shape
         c = self.cfg
         qkv = K.linear(x, self.wqkv).view(B * S, -1)
-        q, k, v = K.rope_qkv(qkv, cos, sin, S, c.n_heads, c.n_kv_heads, c.head_dim)
+        if batch is not None:
+            q, k, v = K.norm_rope_qkv(qkv, cos, sin, batch.positions, c.n_heads, c.n_kv_heads, c.head_dim,
+                                      self.q_norm, self.k_norm, c.norm_eps)
+            o = attn_ops.attention_packed(q, k, v, batch)
+            return K.linear(o.view(B, S, -1), self.wo)
+        if c.qk_norm:
+            q, k, v = K.norm_rope_qkv(qkv, cos, sin, S, c.n_heads, c.n_kv_heads, c.head_dim, self.q_norm, self.k_norm,
+                                      c.norm_eps)
+        else:
+            q, k, v = K.rope_qkv(qkv, cos, sin, S, c.n_heads, c.n_kv_heads, c.head_dim)
         o = attn_ops.attention(q.view(B, S, c.n_heads, c.head_dim),
                                k.view(B, S, c.n_kv_heads, c.head_dim),
                                v.view(B, S, c.n_kv_heads, c.head_dim), causal=True)
@@ -132,18 +154,18 @@ class TransformerBlock(nn.Module):
         self.ffn_norm = nn.Parameter(torch.ones(cfg.dim))
         self.rope_tables = RopeCache(cfg)
 
-    def forward(self, x, residual):
+    def forward(self, x, residual, batch: PackedBatch | None = None):
         """(x, residual) -> (mlp_out, residual'); the residual add happens inside
         the next RMSNorm kernel.  RoPE tables come from the shared cache, NOT
         from forward args: FSDP2's MixedPrecisionPolicy casts floating-point
         forward inputs to bf16, which would corrupt the fp32 cos/sin tables."""
         eps = self.cfg.norm_eps
-        cos, sin = self.rope_tables(x.shape[1], x.device)
+        cos, sin = self.rope_tables(x.shape[1], x.device) if batch is None else self.rope_tables.for_batch(batch)
         if residual is None:
             xn, residual = K.rmsnorm(x, self.attention_norm, eps)
         else:
             xn, residual = K.rmsnorm(x, self.attention_norm, eps, residual=residual)
-        a = self.attention(xn, cos, sin)
+        a = self.attention(xn, cos, sin, batch)
         xn, residual = K.rmsnorm(a, self.ffn_norm, eps, residual=residual)
         return self.feed_forward(xn), residual
 
@@ -167,20 +189,26 @@ class Llama(nn.Module):
             else:
                 p.normal_(0.0, std, generator=g)
 
-    def forward_hidden(self, tokens: torch.Tensor) -> torch.Tensor:
-        h = self.tok_embeddings(tokens)
+    def forward_hidden(self, tokens: torch.Tensor, batch: PackedBatch | None = None) -> torch.Tensor:
+        if batch is not None and tokens.numel() != batch.total:
+            raise ValueError(f"packed batch of {batch.total} rows, tokens {tuple(tokens.shape)}")
+        h = self.tok_embeddings(tokens if batch is None else tokens.reshape(1, -1))
         residual = None
         for layer in self.layers:
             if self.activation_checkpointing and torch.is_grad_enabled():
                 h, residual = torch.utils.checkpoint.checkpoint(
-                    layer, h, residual, use_reentrant=False)
+                    layer, h, residual, batch, use_reentrant=False)
             else:
-                h, residual = layer(h, residual)
+                h, residual = layer(h, residual, batch)
         h, _ = K.rmsnorm(h, self.norm, self.cfg.norm_eps, residual=residual)
         return h
 
-    def forward(self, tokens: torch.Tensor, labels: torch.Tensor | None = None):
-        h = self.forward_hidden(tokens)
+    def forward(self, tokens: torch.Tensor, labels: torch.Tensor | None = None, batch: PackedBatch | None = None):
+        """tokens [B, S] -> logits [B, S, V], or the mean loss over labels
+        [B, S].  With ``batch``: tokens [T] are the batch's documents one after
+        the other (logits [1, T, V]); label what has no next token in its
+        document, padding included, -100."""
+        h = self.forward_hidden(tokens, batch)
         logits = K.linear(h, self.output)
         if labels is None:
             return logits

@@ -73,9 +73,9 @@ _SIGS = {
                                 c_int, c_int, c_int, c_int, c_void_p]),
     "kgwe_wgrad_splits": (c_int, [c_int, c_int, c_int]),
     "kgwe_wgrad_workspace": (c_int64, [c_int, c_int, c_int]),
-    "kgwe_norm_rope_fwd": (c_int, [c_void_p, c_int64, *[c_void_p] * 11, *[c_int] * 8, c_float, c_int, c_void_p]),
+    "kgwe_norm_rope_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_int, *[c_void_p] * 10, *[c_int] * 8, c_float, c_int, c_void_p]),
     "kgwe_norm_rope_bwd_blocks": (c_int, [c_int, c_int, c_int, c_int]),
-    "kgwe_norm_rope_bwd": (c_int, [c_void_p, c_int64, *[c_void_p] * 12, *[c_int] * 6, c_float, c_int, c_void_p]),
+    "kgwe_norm_rope_bwd": (c_int, [c_void_p, c_int64, c_void_p, c_int, *[c_void_p] * 11, *[c_int] * 6, c_float, c_int, c_void_p]),
     "kgwe_packed_plan_jobs": (c_int, [c_int, c_int]),
     "kgwe_packed_plan": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
                                  c_void_p]),

@@ -126,6 +126,7 @@ def norm_rope_append(qkv: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, si
              and kc.dtype == vc.dtype == qkv.dtype and kc.is_contiguous() and vc.is_contiguous()
              and kc.device == vc.device == qkv.device and kc.data_ptr() != vc.data_ptr(),
              "norm_rope_append: caches must be contiguous [R, hkv, Smax, d] of qkv's type")
+    _require(isinstance(pos, torch.Tensor), "norm_rope_append: pos int32 [T]")
     check_norm_rope("norm_rope_append", qkv, pos, cos, sin, hq, hkv, d, q_weight, k_weight, offset,
                     kc.shape[2] + offset)
     _require(rows is not None or T <= kc.shape[0], "norm_rope_append: more rows than the cache has")
@@ -148,8 +149,8 @@ def norm_rope_append(qkv: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, si
         cos, sin, pos = rows16(cos.contiguous()), rows16(sin.contiguous()), pos.contiguous()
         rows = None if rows is None else rows.contiguous()
         with torch.cuda.device(qkv.device):
-            check(lib().kgwe_norm_rope_fwd(ptr(qkv), qkv.stride(0), ptr(pos), ptr(cos), ptr(sin), ptr(qw), ptr(kw),
-                                           ptr(q), ptr(k), ptr(v), ptr(kc), ptr(vc), ptr(rows), T, offset,
+            check(lib().kgwe_norm_rope_fwd(ptr(qkv), qkv.stride(0), ptr(pos), 0, ptr(cos), ptr(sin), ptr(qw),
+                                           ptr(kw), ptr(q), ptr(k), ptr(v), ptr(kc), ptr(vc), ptr(rows), T, offset,
                                            cos.shape[0], hq, hkv, d, kc.shape[2], kc.shape[0], eps,
                                            HALF_TYPES[qkv.dtype], stream(qkv)), "norm_rope_append")
     return (q, k, v) if keep_kv else q

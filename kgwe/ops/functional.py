@@ -220,7 +220,10 @@ def check_norm_rope(what, qkv, positions, cos, sin, hq, hkv, d, q_weight, k_weig
     ``reach``: table rows that have to be there."""
     _require(qkv.dim() == 2 and qkv.shape[1] == (hq + 2 * hkv) * d and hq > 0 and hkv > 0,
              f"{what}: qkv must be [T, (hq+2hkv)*d]")
-    _require(positions.dtype == torch.int32 and positions.shape == (qkv.shape[0],), f"{what}: positions int32 [T]")
+    if isinstance(positions, int):
+        _require(positions > 0, f"{what}: a sequence length must be positive")
+    else:
+        _require(positions.dtype == torch.int32 and positions.shape == (qkv.shape[0],), f"{what}: positions int32 [T]")
     _require((q_weight is None) == (k_weight is None), f"{what}: give both norm weights or neither")
     _require(q_weight is None or (q_weight.shape == k_weight.shape == (d,)
                                   and q_weight.dtype == k_weight.dtype == qkv.dtype),
@@ -228,11 +231,17 @@ def check_norm_rope(what, qkv, positions, cos, sin, hq, hkv, d, q_weight, k_weig
     _require(cos.dtype == sin.dtype == torch.float32 and cos.shape == sin.shape and cos.dim() == 2
              and cos.shape[0] >= max(reach, 1) and cos.shape[1] == d // 2, f"{what}: cos/sin fp32 [>= positions, d/2]")
     _require(0 <= offset < 2**30, f"{what}: offset must not be negative")
-    _require(all(t is None or t.device == qkv.device for t in (positions, cos, sin, q_weight, k_weight)),
+    _require(all(t is None or t.device == qkv.device
+                 for t in (None if isinstance(positions, int) else positions, cos, sin, q_weight, k_weight)),
              f"{what}: every tensor must be on qkv's device")
     if use_hip(qkv):
         _require(qkv.dtype in HALF_TYPES and d in (32, 64, 128, 256) and hq <= 4096 and hkv <= 4096
                  and qkv.shape[0] < 2**31, f"{what}: bf16 or fp16 with head_dim 32, 64, 128 or 256")
+
+
+def _places(positions) -> tuple:
+    """(pointer, period) of the kernels: a table of positions, or row % period."""
+    return (None, positions) if isinstance(positions, int) else (ptr(positions), 0)
 
 
 class _NormRopeQKV(torch.autograd.Function):
@@ -243,20 +252,21 @@ class _NormRopeQKV(torch.autograd.Function):
         k = torch.empty(T, hkv, d, device=qkv.device, dtype=qkv.dtype)
         v = torch.empty_like(k)
         with torch.cuda.device(qkv.device):
-            check(lib().kgwe_norm_rope_fwd(ptr(qkv), qkv.stride(0), ptr(positions), ptr(cos), ptr(sin), ptr(qw),
-                                           ptr(kw), ptr(q), ptr(k), ptr(v), None, None, None, T, offset,
+            check(lib().kgwe_norm_rope_fwd(ptr(qkv), qkv.stride(0), *_places(positions), ptr(cos), ptr(sin),
+                                           ptr(qw), ptr(kw), ptr(q), ptr(k), ptr(v), None, None, None, T, offset,
                                            cos.shape[0], hq, hkv, d, 0, 0, eps, HALF_TYPES[qkv.dtype], stream(qkv)),
                   "norm_rope_fwd")
         # without norms the gradient needs no activation
-        ctx.save_for_backward(qkv if qw is not None else None, qw, kw, cos, sin, positions)
-        ctx.meta = (T, hq, hkv, d, eps, offset)
+        at = None if isinstance(positions, int) else positions
+        ctx.save_for_backward(qkv if qw is not None else None, qw, kw, cos, sin, at)
+        ctx.meta = (T, hq, hkv, d, eps, offset, positions if at is None else 0)
         return q, k, v
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk, dv):
-        qkv, qw, kw, cos, sin, positions = ctx.saved_tensors
-        T, hq, hkv, d, eps, offset = ctx.meta
+        qkv, qw, kw, cos, sin, at = ctx.saved_tensors
+        T, hq, hkv, d, eps, offset, period = ctx.meta
         dq, dk, dv = rows16(dq.contiguous()), rows16(dk.contiguous()), rows16(dv.contiguous())
         dqkv = torch.empty(T, (hq + 2 * hkv) * d, device=dq.device, dtype=dq.dtype)
         part = dqw = dkw = None
@@ -265,20 +275,21 @@ class _NormRopeQKV(torch.autograd.Function):
                 blocks = int(lib().kgwe_norm_rope_bwd_blocks(T, hq, hkv, d))
                 part = torch.empty(blocks, 2, d, device=dq.device, dtype=torch.float32)
                 dqw, dkw = torch.empty_like(qw), torch.empty_like(kw)
-            check(lib().kgwe_norm_rope_bwd(ptr(qkv), 0 if qkv is None else qkv.stride(0), ptr(positions), ptr(cos),
+            check(lib().kgwe_norm_rope_bwd(ptr(qkv), 0 if qkv is None else qkv.stride(0), ptr(at), period, ptr(cos),
                                            ptr(sin), ptr(qw), ptr(kw), ptr(dq), ptr(dk), ptr(dv), ptr(dqkv),
                                            ptr(part), ptr(dqw), ptr(dkw), T, offset, cos.shape[0], hq, hkv, d, eps,
                                            HALF_TYPES[dq.dtype], stream(dq)), "norm_rope_bwd")
         return dqkv, dqw, dkw, None, None, None, None, None, None, None, None
 
 
-def norm_rope_qkv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, hq: int, hkv: int,
-                  d: int, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
+def norm_rope_qkv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | int, hq: int,
+                  hkv: int, d: int, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
                   eps: float = 1e-5, offset: int = 0):
     """qkv [T, (hq+2hkv)d] -> q [T,hq,d], k [T,hkv,d], v [T,hkv,d]: every q and k
     head RMS-normed with its weight [d] (no weights: no norm), then rotated at
-    ``positions[t] + offset`` (int32 [T], as a PackedBatch has them), in one
-    pass and with one rounding; v is copied.  A row whose position is negative
+    ``positions[t] + offset`` (int32 [T], as a PackedBatch has them; or the
+    sequence length S of a rectangular batch: row t is at t % S), in one pass
+    and with one rounding; v is copied.  A row whose position is negative
     or outside the tables gives zeros and takes no gradient.  Differentiable
     with regard to qkv and the weights."""
     check_norm_rope("norm_rope_qkv", qkv, positions, cos, sin, hq, hkv, d, q_weight, k_weight, offset, 1)
@@ -290,7 +301,8 @@ def norm_rope_qkv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, posit
     if q_weight is not None:
         q_weight, k_weight = rows16(q_weight), rows16(k_weight)
     return _NormRopeQKV.apply(rows16(qkv), q_weight, k_weight, rows16(cos.contiguous()), rows16(sin.contiguous()),
-                              positions.contiguous(), hq, hkv, d, eps, offset)
+                              positions if isinstance(positions, int) else positions.contiguous(), hq, hkv, d, eps,
+                              offset)
 
 
 # --------------------------------------------------------------------------

@@ -87,12 +87,14 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, lengths:
     return torch.cat(out)
 
 
-def norm_rope_qkv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, hq: int,
+def norm_rope_qkv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | int, hq: int,
                   hkv: int, d: int, q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
                   eps: float = 1e-5, offset: int = 0):
     """RMS norm of every q and k head (weights [d]; None: no norm), rotation at
-    positions + offset; rows whose position is outside the tables give zeros."""
+    positions + offset (an int S: row t is at t % S); rows whose position is outside the tables give zeros."""
     T = qkv.shape[0]
+    if isinstance(positions, int):
+        positions = torch.arange(T, device=qkv.device) % positions
     at = positions.long() + offset
     live = (positions >= 0) & (at < cos.shape[0])
     x = qkv.view(T, hq + 2 * hkv, d).float().masked_fill(~live[:, None, None], 0.0)

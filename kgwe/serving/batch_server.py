@@ -13,10 +13,15 @@ src/sharing/mig_controller.go:636-678).
 Continuous batching over a fixed-shape hipGraph: the decode step is captured
 once for ``slots x rows`` batch rows.  A request takes a free slot (a
 contiguous group of rows), is prefilled between two graph replays (requests
-that wait together and have one prompt length share a prefill pass), decodes
-with everyone else, and frees its slot when it has its tokens; unused rows are
+that wait together and have one prompt length share a prefill pass; with
+``packed``, all that wait together share one, whatever their lengths, and the
+rows of a request may differ in length), decodes with everyone else, and frees its slot when it has its tokens; unused rows are
 parked at position 0.  Tokens are collected on the device and copied out every
 ``flush`` steps (one sync per flush, not per step).
+
+``prefix`` names the tokens that every request starts with (the group's system
+prompt): they are prefilled once, kept once, and read once per step for the
+whole batch; requests hold only what follows.
 
 Wire protocol (Unix socket or TCP, newline-delimited JSON):
   -> {"op": "generate", "prompt": [[int, ...] x rows], "new": n}
@@ -74,16 +79,21 @@ class _Slot:
 class BatchServer:
     """slots x rows decode batch over one model (see the module docstring)."""
 
-    def __init__(self, model, slots: int, rows: int, max_seq: int, flush: int = 16, graph: bool = True):
+    def __init__(self, model, slots: int, rows: int, max_seq: int, flush: int = 16, graph: bool = True,
+                 packed: bool = False, prefix=None):
         import torch
 
         from ..models.infer import Generator
 
         self.torch = torch
         self.slots_n, self.rows, self.max_seq, self.flush = slots, rows, max_seq, max(1, flush)
-        self.gen = Generator(model, slots * rows, max_seq)
-        self.dev = self.gen.dev
         self.vocab = model.cfg.vocab_size
+        prefix = list(prefix) if prefix is not None else []
+        if any((not isinstance(t, int)) or t < 0 or t >= self.vocab for t in prefix):
+            raise ValueError("prefix: token id out of range")
+        self.packed = packed or bool(prefix)
+        self.gen = Generator(model, slots * rows, max_seq, prefix=prefix or None)
+        self.dev = self.gen.dev
         self.gen.idle_rows(0, slots * rows)
         if self.dev.type == "cuda":
             # Warm the prefill path before the server reports ready: the GEMM library creates
@@ -91,7 +101,10 @@ class BatchServer:
             # step of a serving batch runs on kgwe's own kernels, so the first admission would
             # pay for it (time to first token 190-230 ms instead of 13-57 ms).
             warm = torch.zeros(rows, min(32, max_seq - 2), dtype=torch.long, device=self.dev)
-            self.gen.prefill(warm, rows=(0, rows))
+            if self.packed:
+                self.gen.prefill_packed(list(warm), list(range(rows)))
+            else:
+                self.gen.prefill(warm, rows=(0, rows))
             self.gen.idle_rows(0, rows)
             torch.cuda.synchronize(self.dev)
         if graph and self.dev.type == "cuda":
@@ -174,8 +187,8 @@ class BatchServer:
         p = req.get("prompt")
         if not isinstance(p, list) or len(p) != self.rows or not all(isinstance(r, list) and r for r in p):
             return f"prompt must be {self.rows} rows of token ids"
-        n = len(p[0])
-        if any(len(r) != n for r in p):
+        n = max(len(r) for r in p)
+        if not self.packed and any(len(r) != n for r in p):
             return "prompt rows must have one length"
         new = int(req.get("new", 0))
         if new < 1 or n + new + 1 > self.max_seq:
@@ -187,7 +200,7 @@ class BatchServer:
     def stats(self) -> dict:
         return {"slots": self.slots_n, "rows_per_slot": self.rows, "active": sum(s.conn is not None for s in self.slots),
                 "steps": self.steps, "served": self.served, "tokens_out": self.tokens_out,
-                "prefill_passes": self.prefill_passes,
+                "prefill_passes": self.prefill_passes, "prefix_tokens": self.gen.prefix_len,
                 "busy_s": round(self.busy_s, 4), "address": self.address,
                 "peak_mem_gb": (self.torch.cuda.max_memory_allocated(self.dev) / 2**30
                                 if self.dev.type == "cuda" else 0.0)}
@@ -200,6 +213,9 @@ class BatchServer:
         requests costs about one prefill of N x rows sequences instead of N
         prefills in a row — the last of 32 waits ~40 ms for its first token
         instead of ~200 ms."""
+        if self.packed:
+            self._admit_packed(free, items)
+            return
         torch = self.torch
         by_len: dict[int, list] = {}
         for it in items:
@@ -216,16 +232,29 @@ class BatchServer:
                                       device=self.dev)
                 self.gen.idle_rows(r0, r1, idle=False)
                 first = self.gen.prefill(prompt, rows=(r0, r1)).tolist()
-                self.prefill_passes += 1
-                now = time.time()
-                for j, (idx, (conn, req)) in enumerate(zip(run, batch)):
-                    sl = self.slots[idx]
-                    sl.conn, sl.new, sl.got = conn, int(req["new"]), 1
-                    sl.t_first = now
-                    conn.send({"tokens": [[int(t)] for t in first[j * self.rows:(j + 1) * self.rows]]})
-                    self.tokens_out += self.rows
-                    if sl.got >= sl.new:
-                        self._finish(idx)
+                self._started(run, batch, first)
+
+    def _admit_packed(self, free: list[int], items: list) -> None:
+        """All waiting requests in one packed pass, on any free slots."""
+        slots = sorted(free)[:len(items)]
+        for idx in slots:
+            self.gen.idle_rows(idx * self.rows, (idx + 1) * self.rows, idle=False)
+        first = self.gen.prefill_packed([row for _, req in items for row in req["prompt"]],
+                                        [idx * self.rows + r for idx in slots for r in range(self.rows)]).tolist()
+        self._started(slots, items, first)
+
+    def _started(self, slots: list[int], items: list, first: list[int]) -> None:
+        """One prefill pass is done: its requests hold their slots and get their first tokens."""
+        self.prefill_passes += 1
+        now = time.time()
+        for j, (idx, (conn, req)) in enumerate(zip(slots, items)):
+            sl = self.slots[idx]
+            sl.conn, sl.new, sl.got = conn, int(req["new"]), 1
+            sl.t_first = now
+            conn.send({"tokens": [[int(t)] for t in first[j * self.rows:(j + 1) * self.rows]]})
+            self.tokens_out += self.rows
+            if sl.got >= sl.new:
+                self._finish(idx)
 
     def _finish(self, idx: int) -> None:
         sl = self.slots[idx]
@@ -317,7 +346,15 @@ def main(argv=None) -> int:
     ap.add_argument("--ready-file", default="")
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--no-graph", action="store_true")
+    ap.add_argument("--packed", action="store_true",
+                    help="admit waiting requests of all lengths in one packed prefill pass")
+    ap.add_argument("--prefix-file", default="",
+                    help="token ids (whitespace between them) that every request starts with; implies --packed")
     a = ap.parse_args(argv)
+    prefix = None
+    if a.prefix_file:
+        with open(a.prefix_file) as f:
+            prefix = [int(t) for t in f.read().split()]
     import torch
 
     from ..models import llama
@@ -331,7 +368,8 @@ def main(argv=None) -> int:
     torch.manual_seed(a.seed)
     model = llama.build(a.model, device=dev, dtype=torch.bfloat16 if dev.type == "cuda" else torch.float32)
     model.eval()
-    srv = BatchServer(model, a.slots, a.rows, a.max_seq, flush=a.flush, graph=not a.no_graph)
+    srv = BatchServer(model, a.slots, a.rows, a.max_seq, flush=a.flush, graph=not a.no_graph,
+                      packed=a.packed, prefix=prefix)
     addr = srv.listen(a.listen)
     print(json.dumps({"listening": addr, "slots": a.slots, "rows": a.rows, "share": share}), flush=True)
     if a.ready_file:

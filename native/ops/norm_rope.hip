@@ -5,7 +5,8 @@
 //   n = x * rsqrt(mean(x^2) + eps) * w        per head, w [D] (absent: n = x)
 //   y[i]       = n[i] cos[p, i] - n[i + D/2] sin[p, i]         i < D/2
 //   y[i + D/2] = n[i + D/2] cos[p, i] + n[i] sin[p, i]
-// with p = pos[t] + offset and fp32 tables.  v is copied.  A row whose p is
+// with p = pos[t] + offset and fp32 tables (no pos: row t is at t % period, a
+// rectangular batch).  v is copied.  A row whose p is
 // outside the tables (a packed batch marks its padding rows with position -1)
 // gives zeros and takes no gradient.  Everything between the load and the
 // store is fp32: ONE rounding per output, where norm and rotation as two
@@ -80,7 +81,7 @@ struct FwdArgs {
   unsigned short* kc;        // null: no cache
   unsigned short* vc;
   const int* cache_row;      // null: row t
-  int T, offset, table_rows, Hq, Hkv, Smax, cache_rows;
+  int T, period, offset, table_rows, Hq, Hkv, Smax, cache_rows;
   float eps;
 };
 
@@ -98,7 +99,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_fwd_kernel(FwdArgs a) {
     const int c = static_cast<int>(i % L) * 8;
     const int64_t t = th / Ht;
     const int head = static_cast<int>(th - t * Ht);
-    const int cp = a.pos[t];
+    const int cp = a.pos != nullptr ? a.pos[t] : static_cast<int>(t % a.period);
     const int64_t p = static_cast<int64_t>(cp) + a.offset;
     const bool live = cp >= 0 && p < a.table_rows;
     const unsigned short* in = a.qkv + t * a.row_stride + static_cast<int64_t>(head) * D + c;
@@ -168,7 +169,7 @@ struct BwdArgs {
   const unsigned short* dv;
   unsigned short* dqkv;
   float* part;                // [grid, 2, D] sums of dw (norm only)
-  int T, offset, table_rows, Hq, Hkv;
+  int T, period, offset, table_rows, Hq, Hkv;
   float eps;
 };
 
@@ -194,7 +195,7 @@ __global__ __launch_bounds__(kThreads) void norm_rope_bwd_kernel(BwdArgs a) {
     const int64_t th = i / L;
     const int64_t t = th / Ht;
     const int head = static_cast<int>(th - t * Ht);
-    const int cp = a.pos[t];
+    const int cp = a.pos != nullptr ? a.pos[t] : static_cast<int>(t % a.period);
     const int64_t p = static_cast<int64_t>(cp) + a.offset;
     const bool live = cp >= 0 && p < a.table_rows;
     const bool is_q = head < a.Hq, is_v = head >= a.Hq + a.Hkv;
@@ -351,14 +352,14 @@ int bwd(const BwdArgs& a, int D, int grid, unsigned short* dwq, unsigned short* 
 
 }  // namespace
 
-// wq / wk null: rotation alone.  k / v null: the rotated keys and the values go
+// pos null: row t is at t % period.  wq / wk null: rotation alone.  k / v null: the rotated keys and the values go
 // to the cache only (kc, vc then required).  cache_row null: row t of the cache.
-KGWE_API int kgwe_norm_rope_fwd(const void* qkv, int64_t row_stride, const int* pos, const float* cos_t,
+KGWE_API int kgwe_norm_rope_fwd(const void* qkv, int64_t row_stride, const int* pos, int period, const float* cos_t,
                                 const float* sin_t, const void* wq, const void* wk, void* q, void* k, void* v,
                                 void* kc, void* vc, const int* cache_row, int T, int offset, int table_rows,
                                 int Hq, int Hkv, int D, int Smax, int cache_rows, float eps, int dtype,
                                 hipStream_t s) {
-  if (!shape_ok(T, Hq, Hkv, D, dtype, row_stride) || offset < 0 || table_rows <= 0) return -1;
+  if (!shape_ok(T, Hq, Hkv, D, dtype, row_stride) || offset < 0 || table_rows <= 0 || (!pos && period <= 0)) return -1;
   if ((wq == nullptr) != (wk == nullptr) || (k == nullptr) != (v == nullptr) || (kc == nullptr) != (vc == nullptr) ||
       (k == nullptr && kc == nullptr) || q == nullptr || (kc != nullptr && (Smax <= 0 || cache_rows <= 0)))
     return -1;
@@ -368,7 +369,7 @@ KGWE_API int kgwe_norm_rope_fwd(const void* qkv, int64_t row_stride, const int* 
   using u16 = unsigned short;
   const FwdArgs a{static_cast<const u16*>(qkv), row_stride, pos, cos_t, sin_t, static_cast<const u16*>(wq),
                   static_cast<const u16*>(wk), static_cast<u16*>(q), static_cast<u16*>(k), static_cast<u16*>(v),
-                  static_cast<u16*>(kc), static_cast<u16*>(vc), cache_row, T, offset, table_rows, Hq, Hkv, Smax,
+                  static_cast<u16*>(kc), static_cast<u16*>(vc), cache_row, T, period, offset, table_rows, Hq, Hkv, Smax,
                   cache_rows, eps};
   return dtype == kTypeBf16 ? fwd<Bf16>(a, D, s) : fwd<Fp16>(a, D, s);
 }
@@ -381,11 +382,11 @@ KGWE_API int kgwe_norm_rope_bwd_blocks(int T, int Hq, int Hkv, int D) {
 
 // dq, dk, dv contiguous; dqkv contiguous [T, (Hq + 2 Hkv) D].  With norms also
 // part [blocks, 2, D] fp32 and dwq, dwk [D] (always both).
-KGWE_API int kgwe_norm_rope_bwd(const void* qkv, int64_t row_stride, const int* pos, const float* cos_t,
+KGWE_API int kgwe_norm_rope_bwd(const void* qkv, int64_t row_stride, const int* pos, int period, const float* cos_t,
                                 const float* sin_t, const void* wq, const void* wk, const void* dq, const void* dk,
                                 const void* dv, void* dqkv, float* part, void* dwq, void* dwk, int T, int offset,
                                 int table_rows, int Hq, int Hkv, int D, float eps, int dtype, hipStream_t s) {
-  if (!shape_ok(T, Hq, Hkv, D, dtype, row_stride) || offset < 0 || table_rows <= 0) return -1;
+  if (!shape_ok(T, Hq, Hkv, D, dtype, row_stride) || offset < 0 || table_rows <= 0 || (!pos && period <= 0)) return -1;
   if ((wq == nullptr) != (wk == nullptr) || (wq != nullptr && (!part || !dwq || !dwk || !qkv))) return -1;
   if (!aligned16(qkv) || !aligned16(wq) || !aligned16(wk) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) ||
       !aligned16(dqkv) || !aligned16(cos_t) || !aligned16(sin_t))
@@ -393,7 +394,7 @@ KGWE_API int kgwe_norm_rope_bwd(const void* qkv, int64_t row_stride, const int* 
   using u16 = unsigned short;
   const BwdArgs a{static_cast<const u16*>(qkv), row_stride, pos, cos_t, sin_t, static_cast<const u16*>(wq),
                   static_cast<const u16*>(wk), static_cast<const u16*>(dq), static_cast<const u16*>(dk),
-                  static_cast<const u16*>(dv), static_cast<u16*>(dqkv), part, T, offset, table_rows, Hq, Hkv, eps};
+                  static_cast<const u16*>(dv), static_cast<u16*>(dqkv), part, T, period, offset, table_rows, Hq, Hkv, eps};
   const int grid = kgwe_norm_rope_bwd_blocks(T, Hq, Hkv, D);
   return dtype == kTypeBf16 ? bwd<Bf16>(a, D, grid, static_cast<u16*>(dwq), static_cast<u16*>(dwk), s)
                             : bwd<Fp16>(a, D, grid, static_cast<u16*>(dwq), static_cast<u16*>(dwk), s);

@@ -383,6 +383,22 @@ def test_norm_rope_append(norm, d, dtype):
     assert torch.equal(step, q[:R])
 
 
+@pytest.mark.parametrize("norm", [True, False])
+def test_norm_rope_of_a_rectangular_batch(norm):
+    """A sequence length in the place of positions: the same bits as its table of positions."""
+    g = torch.Generator(device="cuda").manual_seed(12)
+    S, hq, hkv, d = 50, 4, 2, 64
+    qkv = _rnd(g, 3 * S, (hq + 2 * hkv) * d).requires_grad_(True)
+    cos, sin = ref.rope_tables(S, d, device="cuda")
+    w = [(1 + 0.3 * torch.randn(d, device="cuda", generator=g)).bfloat16().requires_grad_(True) for _ in "qk"]
+    dy = [_rnd(g, 3 * S, h, d) for h in (hq, hkv, hkv)]
+    res = []
+    for at in (S, PackedBatch([S] * 3).positions):
+        out = norm_rope_qkv(qkv, cos, sin, at, hq, hkv, d, *(w if norm else ()))
+        res.append([*out, *torch.autograd.grad(out, (qkv, *(w if norm else ())), dy)])
+    assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
 def test_norm_rope_gpu_refusals():
     pos = torch.zeros(2, dtype=torch.int32, device="cuda")
     cos, sin = ref.rope_tables(4, 48, device="cuda")

@@ -73,8 +73,9 @@ def test_rotation_alone_is_rope_qkv():
     qkv = torch.randn(2 * S, (hq + 2 * hkv) * d)
     cos, sin = ref.rope_tables(S, d)
     got = norm_rope_qkv(qkv, cos, sin, PackedBatch([S, S], device="cpu").positions, hq, hkv, d)
-    for a, b in zip(got, rope_qkv(qkv, cos, sin, S, hq, hkv, d)):
-        assert torch.equal(a, b)
+    for other in (rope_qkv(qkv, cos, sin, S, hq, hkv, d), norm_rope_qkv(qkv, cos, sin, S, hq, hkv, d)):
+        for a, b in zip(got, other):
+            assert torch.equal(a, b)
 
 
 def test_norm_rope_reference_padding_and_offset():
@@ -114,6 +115,8 @@ def test_norm_rope_refusals():
     for bad in (lambda: norm_rope_qkv(qkv[:, 1:], cos, sin, pos, hq, hkv, d),
                 lambda: norm_rope_qkv(qkv, cos, sin, pos.long(), hq, hkv, d),
                 lambda: norm_rope_qkv(qkv, cos, sin, pos[:2], hq, hkv, d),
+                lambda: norm_rope_qkv(qkv, cos, sin, 0, hq, hkv, d),
+                lambda: dec.norm_rope_append(qkv, 3, cos, sin, kc, kc.clone(), hq, hkv, d),
                 lambda: norm_rope_qkv(qkv, cos, sin, pos, hq, hkv, d, q_weight=w),
                 lambda: norm_rope_qkv(qkv, cos, sin, pos, hq, hkv, d, w[:4], w[:4]),
                 lambda: norm_rope_qkv(qkv, cos, sin, pos, hq, hkv, d, w.double(), w.double()),
