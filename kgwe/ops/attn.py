@@ -18,7 +18,7 @@ import torch
 import torch.nn.functional as F
 
 from . import reference as ref
-from ._lib import HALF_TYPES, check, has_symbol, lib, ptr, rows16, stream, use_hip
+from ._lib import HALF_TYPES, check, dense16, has_symbol, launch, lib, ptr, rows16, stream, use_hip
 from .packed import PackedBatch
 
 
@@ -100,18 +100,16 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
 # --------------------------------------------------------------------------
 def _packed_fwd(q, k, v, batch, causal, prefix, want_lse):
     T, Hq, D = q.shape
-    Hkv = k.shape[1]
-    o = torch.empty(T, Hq, D, device=q.device, dtype=q.dtype)
-    lse = torch.empty(Hq, T, device=q.device, dtype=torch.float32) if want_lse else None
-    pk, pv = prefix if prefix is not None else (None, None)
-    P = pk.shape[1] if pk is not None else 0
-    views = [x for t in (q, k, v) for x in (ptr(t), t.stride(0), t.stride(1))]
-    for t in (pk, pv):  # [Hkv, P, D]: row stride, head stride
-        views += [ptr(t), t.stride(1), t.stride(0)] if P else [None, 0, 0]
-    with torch.cuda.device(q.device):
-        check(lib().kgwe_packed_attn_fwd(*views, P, ptr(o), ptr(lse), ptr(batch.cu), ptr(batch.jobs),
-                                         batch.jobs.shape[0], batch.n, T, Hq, Hkv, D, 1.0 / math.sqrt(D),
-                                         int(causal), HALF_TYPES[q.dtype], stream(q)), "packed_attn_fwd")
+    o = torch.empty((T, Hq, D), device=q.device, dtype=q.dtype)
+    lse = torch.empty((Hq, T), device=q.device, dtype=torch.float32) if want_lse else None
+    (qr, qh, _), (kr, kh, _), (vr, vh, _) = q.stride(), k.stride(), v.stride()
+    pre = (None, 0, 0, None, 0, 0, 0)
+    if prefix is not None:  # [Hkv, P, D]: row stride, head stride
+        pk, pv = prefix
+        pre = (pk.data_ptr(), pk.stride(1), pk.stride(0), pv.data_ptr(), pv.stride(1), pv.stride(0), pk.shape[1])
+    launch(lib().kgwe_packed_attn_fwd, "packed_attn_fwd", q.device, q.data_ptr(), qr, qh, k.data_ptr(), kr, kh,
+           v.data_ptr(), vr, vh, *pre, o.data_ptr(), ptr(lse), *batch.tables, T, Hq, k.shape[1], D, D ** -0.5, causal,
+           HALF_TYPES[q.dtype])
     return o, lse
 
 
@@ -130,19 +128,15 @@ class _PackedAttn(torch.autograd.Function):
         batch = ctx.batch
         T, Hq, D = q.shape
         Hkv = k.shape[1]
-        do = do.contiguous()
-        if do.data_ptr() % 16:
-            do = do.clone()
-        dq = torch.empty(T, Hq, D, device=q.device, dtype=q.dtype)
-        dk = torch.empty(T, Hkv, D, device=q.device, dtype=q.dtype)
+        do = dense16(do)
+        dq = torch.empty((T, Hq, D), device=q.device, dtype=q.dtype)
+        dk = torch.empty((T, Hkv, D), device=q.device, dtype=q.dtype)
         dv = torch.empty_like(dk)
         delta = torch.empty_like(lse)
-        views = [x for t in (q, k, v) for x in (ptr(t), t.stride(0), t.stride(1))]
-        with torch.cuda.device(q.device):
-            check(lib().kgwe_packed_attn_bwd(*views, ptr(o), ptr(lse), ptr(do), ptr(delta), ptr(dq), ptr(dk), ptr(dv),
-                                             ptr(batch.cu), ptr(batch.jobs), batch.jobs.shape[0], batch.n, T, Hq, Hkv,
-                                             D, 1.0 / math.sqrt(D), int(ctx.causal), HALF_TYPES[q.dtype], stream(q)),
-                  "packed_attn_bwd")
+        (qr, qh, _), (kr, kh, _), (vr, vh, _) = q.stride(), k.stride(), v.stride()
+        launch(lib().kgwe_packed_attn_bwd, "packed_attn_bwd", q.device, q.data_ptr(), qr, qh, k.data_ptr(), kr, kh,
+               v.data_ptr(), vr, vh, o.data_ptr(), lse.data_ptr(), do.data_ptr(), delta.data_ptr(), dq.data_ptr(),
+               dk.data_ptr(), dv.data_ptr(), *batch.tables, T, Hq, Hkv, D, D ** -0.5, ctx.causal, HALF_TYPES[q.dtype])
         return dq, dk, dv, None, None
 
 
@@ -158,29 +152,31 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: P
     dense 16-byte aligned rows (slices of a fused projection), others are
     copied.  A NaN or infinity in v reaches the rows that see it and may reach
     up to 63 rows before it in its own sequence, never another sequence."""
-    if not (q.dim() == k.dim() == v.dim() == 3 and q.shape[0] == k.shape[0] == batch.total and k.shape == v.shape
-            and q.shape[2] == k.shape[2] and k.shape[1] > 0 and q.shape[1] > 0 and q.shape[1] % k.shape[1] == 0):
+    qs, ks = q.shape, k.shape
+    if not (len(qs) == len(ks) == 3 and v.shape == ks and qs[0] == ks[0] == batch.total and qs[2] == ks[2]
+            and qs[1] > 0 and ks[1] > 0 and qs[1] % ks[1] == 0):
         raise ValueError(f"attention_packed: q [T, Hq, D], k / v [T, Hkv, D] with T = {batch.total} and Hq % Hkv == 0, "
-                         f"got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    tensors = [q, k, v]
+                         f"got {tuple(qs)}, {tuple(ks)}, {tuple(v.shape)}")
+    dtype, device = q.dtype, q.device
+    if not (k.dtype == v.dtype == dtype and k.device == v.device == device == batch.device):
+        raise ValueError("attention_packed: tensors and batch must share one type and device")
+    grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if prefix is not None:
         pk, pv = prefix
-        if not (pk.dim() == 3 and pk.shape == pv.shape and pk.shape[0] == k.shape[1] and pk.shape[2] == k.shape[2]):
-            raise ValueError("attention_packed: prefix keys and values must be [Hkv, P, D]")
-        tensors += [pk, pv]
-        if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        if not (pk.dim() == 3 and pk.shape == pv.shape and pk.shape[0] == ks[1] and pk.shape[2] == ks[2]
+                and pk.dtype == pv.dtype == dtype and pk.device == pv.device == device):
+            raise ValueError("attention_packed: prefix keys and values must be [Hkv, P, D] of k's type and device")
+        if grad or (torch.is_grad_enabled() and (pk.requires_grad or pv.requires_grad)):
             raise ValueError("attention_packed: a shared prefix has no gradient; call it under torch.no_grad()")
-    if any(t.dtype != q.dtype or t.device != q.device for t in tensors) or batch.device != q.device:
-        raise ValueError("attention_packed: tensors and batch must share one type and device")
     if not use_hip(q):
         return ref.attention_packed(q, k, v, batch.lengths.tolist(), causal, prefix)
-    if q.dtype not in HALF_TYPES or q.shape[2] not in (64, 128):
+    if dtype not in HALF_TYPES or qs[2] not in (64, 128):
         raise ValueError("attention_packed: bf16 or fp16 with head_dim 64 or 128")
     if batch.total == 0:
         return q.clone()
     q, k, v = rows16(q), rows16(k), rows16(v)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
-        return _PackedAttn.apply(q, k, v, batch, causal)
+    if grad:
+        return _PackedAttn.apply(q, k, v, batch, bool(causal))
     if prefix is not None:
-        prefix = (rows16(prefix[0]), rows16(prefix[1])) if prefix[0].shape[1] else None
-    return _packed_fwd(q, k, v, batch, causal, prefix, False)[0]
+        prefix = (rows16(pk), rows16(pv)) if pk.shape[1] else None
+    return _packed_fwd(q, k, v, batch, bool(causal), prefix, False)[0]

@@ -25,7 +25,8 @@ import math
 import torch
 
 from . import reference as ref
-from ._lib import HALF_TYPES, check, lib, ptr, rows16, stream, use_hip
+from ._lib import HALF_TYPES, check, dense16, launch, lib, ptr, rows16, stream, use_hip
+from .functional import check_norm_rope
 
 
 def _require(cond: bool, msg: str) -> None:
@@ -119,19 +120,18 @@ def norm_rope_append(qkv: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, si
     decode step, or all rows of a packed prompt.  A row of qkv whose place is
     outside the cache (position -1: padding) writes nothing; two rows must not
     name one place.  Forward only."""
-    from .functional import check_norm_rope  # noqa: PLC0415
-
-    T = qkv.shape[0]
-    _require(kc.shape == vc.shape and kc.dim() == 4 and kc.shape[1] == hkv and kc.shape[3] == d
-             and kc.dtype == vc.dtype == qkv.dtype and kc.is_contiguous() and vc.is_contiguous()
-             and kc.device == vc.device == qkv.device and kc.data_ptr() != vc.data_ptr(),
-             "norm_rope_append: caches must be contiguous [R, hkv, Smax, d] of qkv's type")
+    T, dtype, device, cache = qkv.shape[0], qkv.dtype, qkv.device, kc.shape
+    if not (len(cache) == 4 and vc.shape == cache and cache[1] == hkv and cache[3] == d and kc.dtype == vc.dtype == dtype
+            and kc.is_contiguous() and vc.is_contiguous() and kc.device == vc.device == device
+            and kc.data_ptr() != vc.data_ptr()):
+        raise ValueError("norm_rope_append: caches must be two contiguous [R, hkv, Smax, d] of qkv's type and device")
     _require(isinstance(pos, torch.Tensor), "norm_rope_append: pos int32 [T]")
-    check_norm_rope("norm_rope_append", qkv, pos, cos, sin, hq, hkv, d, q_weight, k_weight, offset,
-                    kc.shape[2] + offset)
-    _require(rows is not None or T <= kc.shape[0], "norm_rope_append: more rows than the cache has")
-    _require(rows is None or (rows.dtype == torch.int32 and rows.shape == (T,) and rows.device == qkv.device),
-             "norm_rope_append: rows int32 [T]")
+    check_norm_rope("norm_rope_append", qkv, pos, cos, sin, hq, hkv, d, q_weight, k_weight, offset, cache[2] + offset)
+    if rows is None:
+        _require(T <= cache[0], "norm_rope_append: more rows than the cache has")
+    else:
+        _require(rows.dtype == torch.int32 and rows.shape == (T,) and rows.device == device,
+                 "norm_rope_append: rows int32 [T]")
     if not use_hip(qkv):
         q, k, v = ref.norm_rope_qkv(qkv, cos, sin, pos, hq, hkv, d, q_weight, k_weight, eps, offset)
         at = torch.arange(T, device=qkv.device) if rows is None else rows.long()
@@ -139,20 +139,21 @@ def norm_rope_append(qkv: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, si
         kc[at[ok], :, pos[ok].long()] = k[ok]
         vc[at[ok], :, pos[ok].long()] = v[ok]
         return (q, k, v) if keep_kv else q
-    q = torch.empty(T, hq, d, device=qkv.device, dtype=qkv.dtype)
-    k = torch.empty(T, hkv, d, device=qkv.device, dtype=qkv.dtype) if keep_kv else None
-    v = torch.empty_like(k) if keep_kv else None
+    q = torch.empty((T, hq, d), device=device, dtype=dtype)
+    k = v = None
+    if keep_kv:
+        k = torch.empty((T, hkv, d), device=device, dtype=dtype)
+        v = torch.empty((T, hkv, d), device=device, dtype=dtype)
     if T > 0 and kc.numel() > 0:
-        _require(kc.data_ptr() % 16 == 0 and vc.data_ptr() % 16 == 0, "norm_rope_append: caches must be 16-byte aligned")
-        qkv = rows16(qkv)
-        qw, kw = (None, None) if q_weight is None else (rows16(q_weight), rows16(k_weight))
-        cos, sin, pos = rows16(cos.contiguous()), rows16(sin.contiguous()), pos.contiguous()
+        if (kc.data_ptr() | vc.data_ptr()) & 15:
+            raise ValueError("norm_rope_append: caches must be 16-byte aligned")
+        qkv, cos, sin, pos = rows16(qkv), dense16(cos), dense16(sin), pos.contiguous()
+        if q_weight is not None:
+            q_weight, k_weight = dense16(q_weight), dense16(k_weight)
         rows = None if rows is None else rows.contiguous()
-        with torch.cuda.device(qkv.device):
-            check(lib().kgwe_norm_rope_fwd(ptr(qkv), qkv.stride(0), ptr(pos), 0, ptr(cos), ptr(sin), ptr(qw),
-                                           ptr(kw), ptr(q), ptr(k), ptr(v), ptr(kc), ptr(vc), ptr(rows), T, offset,
-                                           cos.shape[0], hq, hkv, d, kc.shape[2], kc.shape[0], eps,
-                                           HALF_TYPES[qkv.dtype], stream(qkv)), "norm_rope_append")
+        launch(lib().kgwe_norm_rope_fwd, "norm_rope_append", device, qkv.data_ptr(), qkv.stride(0), pos.data_ptr(), 0,
+               cos.data_ptr(), sin.data_ptr(), ptr(q_weight), ptr(k_weight), q.data_ptr(), ptr(k), ptr(v), kc.data_ptr(),
+               vc.data_ptr(), ptr(rows), T, offset, cos.shape[0], hq, hkv, d, cache[2], cache[0], eps, HALF_TYPES[dtype])
     return (q, k, v) if keep_kv else q
 
 
@@ -242,26 +243,27 @@ class PrefixDecodeAttention:
     def __call__(self, q: torch.Tensor, pk: torch.Tensor, pv: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor,
                  lens: torch.Tensor) -> torch.Tensor:
         B, hq, hkv, d, smax, P = self.B, self.hq, self.hkv, self.d, self.smax, self.prefix_len
-        _require(q.shape == (B, hq, d), "prefix attention: q must be [B, Hq, D]")
-        _require(pk.shape == pv.shape == (hkv, P, d), "prefix attention: prefix must be [Hkv, P, D]")
-        _require(kc.shape == vc.shape == (B, hkv, smax, d), "prefix attention: cache shape")
-        _require(lens.dtype == torch.int32 and lens.shape == (B,), "prefix attention: lens int32 [B]")
-        _require(all(t.dtype == self.dtype for t in (q, pk, pv, kc, vc))
-                 and all(t.device == q.device for t in (pk, pv, kc, vc, lens)) and q.is_cuda == self.hip,
-                 "prefix attention: one type and one device")
+        if not (q.shape == (B, hq, d) and pk.shape == pv.shape == (hkv, P, d) and kc.shape == vc.shape == (B, hkv, smax, d)):
+            raise ValueError(f"prefix attention: q {(B, hq, d)}, prefix {(hkv, P, d)}, caches {(B, hkv, smax, d)}, got "
+                             f"{[tuple(t.shape) for t in (q, pk, pv, kc, vc)]}")
+        dtype, device = self.dtype, q.device
+        if not (q.dtype == pk.dtype == pv.dtype == kc.dtype == vc.dtype == dtype and q.is_cuda == self.hip
+                and pk.device == pv.device == kc.device == vc.device == lens.device == device):
+            raise ValueError("prefix attention: one type and one device")
+        if not (lens.dtype == torch.int32 and lens.shape == (B,)):
+            raise ValueError("prefix attention: lens int32 [B]")
         if not self.hip:
             return prefix_attention_reference(q, pk, pv, kc, vc, lens)
-        _require(kc.is_contiguous() and vc.is_contiguous() and kc.data_ptr() % 16 == 0 and vc.data_ptr() % 16 == 0,
-                 "prefix attention: caches must be contiguous and 16-byte aligned")
-        q, pk, pv, lens = rows16(q.contiguous()), rows16(pk), rows16(pv), lens.contiguous()
+        if not (kc.is_contiguous() and vc.is_contiguous()) or (kc.data_ptr() | vc.data_ptr()) & 15:
+            raise ValueError("prefix attention: caches must be contiguous and 16-byte aligned")
+        q, pk, pv, lens = dense16(q), rows16(pk), rows16(pv), lens.contiguous()
         if P > 0 and pk.stride() != pv.stride():  # one pair of strides for both
-            pk, pv = rows16(pk.contiguous()), rows16(pv.contiguous())
+            pk, pv = dense16(pk), dense16(pv)
         out = torch.empty_like(q)
-        with torch.cuda.device(q.device):
-            work = torch.empty(self.words, device=q.device, dtype=torch.float32)
-            check(lib().kgwe_prefix_attn(ptr(q), ptr(pk), ptr(pv), max(pk.stride(1), d), pk.stride(0), ptr(kc),
-                                         ptr(vc), ptr(lens), ptr(work), ptr(out), B, hq, hkv, d, P, smax,
-                                         1.0 / math.sqrt(d), HALF_TYPES[q.dtype], stream(q)), "prefix_attn")
+        work = torch.empty(self.words, device=device, dtype=torch.float32) if self.words else None
+        launch(lib().kgwe_prefix_attn, "prefix_attn", device, q.data_ptr(), pk.data_ptr(), pv.data_ptr(),
+               max(pk.stride(1), d), pk.stride(0), kc.data_ptr(), vc.data_ptr(), lens.data_ptr(), ptr(work),
+               out.data_ptr(), B, hq, hkv, d, P, smax, d ** -0.5, HALF_TYPES[dtype])
         return out
 
 

@@ -11,7 +11,7 @@ import os
 import torch
 
 from . import reference as ref
-from ._lib import HALF_TYPES, check, lib, ptr, rows16, stream, use_hip
+from ._lib import HALF_TYPES, check, dense16, launch, lib, ptr, rows16, stream, use_hip
 from .gemm import wgrad, wgrad_supported
 
 
@@ -218,67 +218,67 @@ def rope_qkv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, seq_len: i
 def check_norm_rope(what, qkv, positions, cos, sin, hq, hkv, d, q_weight, k_weight, offset, reach):
     """Host-side contract shared by norm_rope_qkv and decode.norm_rope_append;
     ``reach``: table rows that have to be there."""
-    _require(qkv.dim() == 2 and qkv.shape[1] == (hq + 2 * hkv) * d and hq > 0 and hkv > 0,
-             f"{what}: qkv must be [T, (hq+2hkv)*d]")
+    shape, dtype, device = qkv.shape, qkv.dtype, qkv.device
+    if not (len(shape) == 2 and hq > 0 and hkv > 0 and shape[1] == (hq + 2 * hkv) * d):
+        raise ValueError(f"{what}: qkv must be [T, (hq+2hkv)*d]")
     if isinstance(positions, int):
         _require(positions > 0, f"{what}: a sequence length must be positive")
-    else:
-        _require(positions.dtype == torch.int32 and positions.shape == (qkv.shape[0],), f"{what}: positions int32 [T]")
-    _require((q_weight is None) == (k_weight is None), f"{what}: give both norm weights or neither")
-    _require(q_weight is None or (q_weight.shape == k_weight.shape == (d,)
-                                  and q_weight.dtype == k_weight.dtype == qkv.dtype),
-             f"{what}: norm weights must be [d] of qkv's type")
-    _require(cos.dtype == sin.dtype == torch.float32 and cos.shape == sin.shape and cos.dim() == 2
-             and cos.shape[0] >= max(reach, 1) and cos.shape[1] == d // 2, f"{what}: cos/sin fp32 [>= positions, d/2]")
-    _require(0 <= offset < 2**30, f"{what}: offset must not be negative")
-    _require(all(t is None or t.device == qkv.device
-                 for t in (None if isinstance(positions, int) else positions, cos, sin, q_weight, k_weight)),
-             f"{what}: every tensor must be on qkv's device")
-    if use_hip(qkv):
-        _require(qkv.dtype in HALF_TYPES and d in (32, 64, 128, 256) and hq <= 4096 and hkv <= 4096
-                 and qkv.shape[0] < 2**31, f"{what}: bf16 or fp16 with head_dim 32, 64, 128 or 256")
+    elif not (positions.dtype == torch.int32 and positions.shape == shape[:1] and positions.device == device):
+        raise ValueError(f"{what}: positions int32 [T] on qkv's device")
+    if (q_weight is None) != (k_weight is None):
+        raise ValueError(f"{what}: give both norm weights or neither")
+    if q_weight is not None and not (
+            q_weight.shape == k_weight.shape == (d,) and q_weight.dtype == k_weight.dtype == dtype
+            and q_weight.device == k_weight.device == device):
+        raise ValueError(f"{what}: norm weights must be [d] of qkv's type and device")
+    table = cos.shape
+    if not (len(table) == 2 and sin.shape == table and cos.dtype == sin.dtype == torch.float32
+            and table[0] >= max(reach, 1) and table[1] == d // 2 and cos.device == sin.device == device):
+        raise ValueError(f"{what}: cos/sin fp32 [>= positions, d/2] on qkv's device")
+    if not 0 <= offset < 2**30:
+        raise ValueError(f"{what}: offset must not be negative")
+    if device.type == "cuda" and not (dtype in HALF_TYPES and d in (32, 64, 128, 256) and hq <= 4096 and hkv <= 4096
+                                      and shape[0] < 2**31):
+        raise ValueError(f"{what}: bf16 or fp16 with head_dim 32, 64, 128 or 256")
 
 
-def _places(positions) -> tuple:
-    """(pointer, period) of the kernels: a table of positions, or row % period."""
-    return (None, positions) if isinstance(positions, int) else (ptr(positions), 0)
+def _norm_rope_fwd(qkv, qw, kw, cos, sin, positions, hq, hkv, d, eps, offset):
+    T, dtype, device = qkv.shape[0], qkv.dtype, qkv.device
+    q = torch.empty((T, hq, d), device=device, dtype=dtype)
+    k = torch.empty((T, hkv, d), device=device, dtype=dtype)
+    v = torch.empty((T, hkv, d), device=device, dtype=dtype)
+    pos, period = (None, positions) if isinstance(positions, int) else (positions.data_ptr(), 0)
+    launch(lib().kgwe_norm_rope_fwd, "norm_rope_fwd", device, qkv.data_ptr(), qkv.stride(0), pos, period,
+           cos.data_ptr(), sin.data_ptr(), ptr(qw), ptr(kw), q.data_ptr(), k.data_ptr(), v.data_ptr(), None, None, None,
+           T, offset, cos.shape[0], hq, hkv, d, 0, 0, eps, HALF_TYPES[dtype])
+    return q, k, v
 
 
 class _NormRopeQKV(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, qw, kw, cos, sin, positions, hq, hkv, d, eps, offset):
-        T = qkv.shape[0]
-        q = torch.empty(T, hq, d, device=qkv.device, dtype=qkv.dtype)
-        k = torch.empty(T, hkv, d, device=qkv.device, dtype=qkv.dtype)
-        v = torch.empty_like(k)
-        with torch.cuda.device(qkv.device):
-            check(lib().kgwe_norm_rope_fwd(ptr(qkv), qkv.stride(0), *_places(positions), ptr(cos), ptr(sin),
-                                           ptr(qw), ptr(kw), ptr(q), ptr(k), ptr(v), None, None, None, T, offset,
-                                           cos.shape[0], hq, hkv, d, 0, 0, eps, HALF_TYPES[qkv.dtype], stream(qkv)),
-                  "norm_rope_fwd")
-        # without norms the gradient needs no activation
         at = None if isinstance(positions, int) else positions
+        # without norms the gradient needs no activation
         ctx.save_for_backward(qkv if qw is not None else None, qw, kw, cos, sin, at)
-        ctx.meta = (T, hq, hkv, d, eps, offset, positions if at is None else 0)
-        return q, k, v
+        ctx.meta = (qkv.shape[0], hq, hkv, d, eps, offset, positions if at is None else 0)
+        return _norm_rope_fwd(qkv, qw, kw, cos, sin, positions, hq, hkv, d, eps, offset)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk, dv):
         qkv, qw, kw, cos, sin, at = ctx.saved_tensors
         T, hq, hkv, d, eps, offset, period = ctx.meta
-        dq, dk, dv = rows16(dq.contiguous()), rows16(dk.contiguous()), rows16(dv.contiguous())
-        dqkv = torch.empty(T, (hq + 2 * hkv) * d, device=dq.device, dtype=dq.dtype)
+        dq, dk, dv = dense16(dq), dense16(dk), dense16(dv)
+        dqkv = torch.empty((T, (hq + 2 * hkv) * d), device=dq.device, dtype=dq.dtype)
         part = dqw = dkw = None
-        with torch.cuda.device(dq.device):
-            if qw is not None:
-                blocks = int(lib().kgwe_norm_rope_bwd_blocks(T, hq, hkv, d))
-                part = torch.empty(blocks, 2, d, device=dq.device, dtype=torch.float32)
-                dqw, dkw = torch.empty_like(qw), torch.empty_like(kw)
-            check(lib().kgwe_norm_rope_bwd(ptr(qkv), 0 if qkv is None else qkv.stride(0), ptr(at), period, ptr(cos),
-                                           ptr(sin), ptr(qw), ptr(kw), ptr(dq), ptr(dk), ptr(dv), ptr(dqkv),
-                                           ptr(part), ptr(dqw), ptr(dkw), T, offset, cos.shape[0], hq, hkv, d, eps,
-                                           HALF_TYPES[dq.dtype], stream(dq)), "norm_rope_bwd")
+        if qw is not None:
+            blocks = int(lib().kgwe_norm_rope_bwd_blocks(T, hq, hkv, d))
+            part = torch.empty((blocks, 2, d), device=dq.device, dtype=torch.float32)
+            dqw, dkw = torch.empty_like(qw), torch.empty_like(kw)
+        launch(lib().kgwe_norm_rope_bwd, "norm_rope_bwd", dq.device, ptr(qkv), 0 if qkv is None else qkv.stride(0),
+               ptr(at), period, cos.data_ptr(), sin.data_ptr(), ptr(qw), ptr(kw), dq.data_ptr(), dk.data_ptr(),
+               dv.data_ptr(), dqkv.data_ptr(), ptr(part), ptr(dqw), ptr(dkw), T, offset, cos.shape[0], hq, hkv, d, eps,
+               HALF_TYPES[dq.dtype])
         return dqkv, dqw, dkw, None, None, None, None, None, None, None, None
 
 
@@ -298,11 +298,16 @@ def norm_rope_qkv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, posit
     if qkv.shape[0] == 0:
         q, k, v = qkv.reshape(0, hq + 2 * hkv, d).split((hq, hkv, hkv), dim=1)
         return q, k, v
+    qkv, cos, sin = rows16(qkv), dense16(cos), dense16(sin)
     if q_weight is not None:
-        q_weight, k_weight = rows16(q_weight), rows16(k_weight)
-    return _NormRopeQKV.apply(rows16(qkv), q_weight, k_weight, rows16(cos.contiguous()), rows16(sin.contiguous()),
-                              positions if isinstance(positions, int) else positions.contiguous(), hq, hkv, d, eps,
-                              offset)
+        q_weight, k_weight = dense16(q_weight), dense16(k_weight)
+    if not isinstance(positions, int):
+        positions = positions.contiguous()
+    args = (qkv, q_weight, k_weight, cos, sin, positions, hq, hkv, d, eps, offset)
+    if torch.is_grad_enabled() and (qkv.requires_grad or (q_weight is not None and (
+            q_weight.requires_grad or k_weight.requires_grad))):
+        return _NormRopeQKV.apply(*args)
+    return _norm_rope_fwd(*args)
 
 
 # --------------------------------------------------------------------------
