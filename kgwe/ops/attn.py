@@ -98,33 +98,34 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
 # --------------------------------------------------------------------------
 # Packed sequences
 # --------------------------------------------------------------------------
-def _packed_fwd(q, k, v, batch, causal, prefix, want_lse):
+def _packed_fwd(q, k, v, batch, causal, prefix, train):
     T, Hq, D = q.shape
     o = torch.empty((T, Hq, D), device=q.device, dtype=q.dtype)
-    lse = torch.empty((Hq, T), device=q.device, dtype=torch.float32) if want_lse else None
+    lse = torch.empty((Hq, T), device=q.device, dtype=torch.float32) if train else None
+    low = torch.empty_like(o) if train else None  # what the rounding of o drops
     (qr, qh, _), (kr, kh, _), (vr, vh, _) = q.stride(), k.stride(), v.stride()
     pre = (None, 0, 0, None, 0, 0, 0)
     if prefix is not None:  # [Hkv, P, D]: row stride, head stride
         pk, pv = prefix
         pre = (pk.data_ptr(), pk.stride(1), pk.stride(0), pv.data_ptr(), pv.stride(1), pv.stride(0), pk.shape[1])
     launch(lib().kgwe_packed_attn_fwd, "packed_attn_fwd", q.device, q.data_ptr(), qr, qh, k.data_ptr(), kr, kh,
-           v.data_ptr(), vr, vh, *pre, o.data_ptr(), ptr(lse), *batch.tables, T, Hq, k.shape[1], D, D ** -0.5, causal,
+           v.data_ptr(), vr, vh, *pre, o.data_ptr(), ptr(low), ptr(lse), *batch.tables, T, Hq, k.shape[1], D, D ** -0.5, causal,
            HALF_TYPES[q.dtype])
-    return o, lse
+    return o, low, lse
 
 
 class _PackedAttn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, batch, causal):
-        o, lse = _packed_fwd(q, k, v, batch, causal, None, True)
-        ctx.save_for_backward(q, k, v, o, lse)
+        o, low, lse = _packed_fwd(q, k, v, batch, causal, None, True)
+        ctx.save_for_backward(q, k, v, o, low, lse)
         ctx.batch, ctx.causal = batch, causal
         return o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
-        q, k, v, o, lse = ctx.saved_tensors
+        q, k, v, o, low, lse = ctx.saved_tensors
         batch = ctx.batch
         T, Hq, D = q.shape
         Hkv = k.shape[1]
@@ -135,7 +136,7 @@ class _PackedAttn(torch.autograd.Function):
         delta = torch.empty_like(lse)
         (qr, qh, _), (kr, kh, _), (vr, vh, _) = q.stride(), k.stride(), v.stride()
         launch(lib().kgwe_packed_attn_bwd, "packed_attn_bwd", q.device, q.data_ptr(), qr, qh, k.data_ptr(), kr, kh,
-               v.data_ptr(), vr, vh, o.data_ptr(), lse.data_ptr(), do.data_ptr(), delta.data_ptr(), dq.data_ptr(),
+               v.data_ptr(), vr, vh, o.data_ptr(), low.data_ptr(), lse.data_ptr(), do.data_ptr(), delta.data_ptr(), dq.data_ptr(),
                dk.data_ptr(), dv.data_ptr(), *batch.tables, T, Hq, Hkv, D, D ** -0.5, ctx.causal, HALF_TYPES[q.dtype])
         return dq, dk, dv, None, None
 

@@ -173,132 +173,146 @@ struct BwdArgs {
   float eps;
 };
 
+// Sums of a thread's share of dw over the lanes that hold the same chunk, then
+// over the four waves, in a fixed order; out [D].
+template <int L>
+__device__ __forceinline__ void reduce_dw(float (&acc)[16], int c, float (&red)[kThreads / kWave][16 * L], float* out) {
+  constexpr int D = 16 * L, half = D / 2;
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+#pragma unroll
+    for (int off = kWave / 2; off >= L; off >>= 1) acc[j] += __shfl_xor(acc[j], off, kWave);
+  if (lane < L) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      red[wave][c + j] = acc[j];
+      red[wave][half + c + j] = acc[8 + j];
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < D; i += kThreads) {
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kThreads / kWave; ++w) s += red[w][i];
+    out[i] = s;
+  }
+  __syncthreads();
+}
+
+// The query heads of all rows, then the key heads, then the value heads: one
+// weight and one set of dw sums live at a time (one sweep over all heads held
+// two of each: 136 registers, 3 workgroups per CU, 88 us at 10,339 rows of
+// 32 / 8 heads x 128 against 66 us).
 template <class T, int L, bool NORM>
 __global__ __launch_bounds__(kThreads) void norm_rope_bwd_kernel(BwdArgs a) {
   constexpr int D = 16 * L, half = D / 2;
+  __shared__ float red[kThreads / kWave][D];
   const int Ht = a.Hq + 2 * a.Hkv;
-  const int64_t n = static_cast<int64_t>(a.T) * Ht * L;
-  // The stride is a multiple of L, so a thread always holds the same chunk of
+  // The strides are multiples of L, so a thread always holds the same chunk of
   // a head and sums its share of dw in registers.
   const int c = static_cast<int>(threadIdx.x % L) * 8;
-  float wq0[8], wq1[8], wk0[8], wk1[8], aq[16], ak[16];
-  if (NORM) {
-    up8<T>(ld8(a.wq + c), wq0);
-    up8<T>(ld8(a.wq + half + c), wq1);
-    up8<T>(ld8(a.wk + c), wk0);
-    up8<T>(ld8(a.wk + half + c), wk1);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) aq[j] = ak[j] = 0.f;
-  }
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < n;
-       i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int64_t th = i / L;
-    const int64_t t = th / Ht;
-    const int head = static_cast<int>(th - t * Ht);
-    const int cp = a.pos != nullptr ? a.pos[t] : static_cast<int>(t % a.period);
-    const int64_t p = static_cast<int64_t>(cp) + a.offset;
-    const bool live = cp >= 0 && p < a.table_rows;
-    const bool is_q = head < a.Hq, is_v = head >= a.Hq + a.Hkv;
-    const unsigned short* dy = is_q ? a.dq + (t * a.Hq + head) * D
-        : (is_v ? a.dv : a.dk) + (t * a.Hkv + (head - a.Hq - (is_v ? a.Hkv : 0))) * D;
-    const bf16x8 lo = live ? ld8(dy + c) : bf16x8{}, hi = live ? ld8(dy + half + c) : bf16x8{};
-    unsigned short* out = a.dqkv + (t * Ht + head) * static_cast<int64_t>(D);
-    float g0[8], g1[8];
-    {
-      float y0[8], y1[8], cs[8], sn[8];
-      up8<T>(lo, y0);
-      up8<T>(hi, y1);
-      if (live && !is_v) {
+  const int64_t start = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
+  auto sweep = [&](const unsigned short* dy, const unsigned short* w, int heads, int first, float (&acc)[16]) {
+    float w0[8], w1[8];
+    if (NORM) {
+      up8<T>(ld8(w + c), w0);
+      up8<T>(ld8(w + half + c), w1);
+    }
+    const int64_t n = static_cast<int64_t>(a.T) * heads * L;
+    for (int64_t i = start; i < n; i += step) {
+      const int64_t th = i / L, t = th / heads;
+      const int head = static_cast<int>(th - t * heads);
+      const int cp = a.pos != nullptr ? a.pos[t] : static_cast<int>(t % a.period);
+      const int64_t p = static_cast<int64_t>(cp) + a.offset;
+      const bool live = cp >= 0 && p < a.table_rows;
+      unsigned short* out = a.dqkv + (t * Ht + first + head) * static_cast<int64_t>(D) + c;
+      float g0[8] = {}, g1[8] = {};
+      if (live) {  // the same for all lanes of a head
+        const unsigned short* y = dy + th * D + c;
+        float y0[8], y1[8], cs[8], sn[8];
+        up8<T>(ld8(y), y0);
+        up8<T>(ld8(y + half), y1);
         load_table(a.cosT + p * half + c, cs);
         load_table(a.sinT + p * half + c, sn);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) cs[j] = 1.f, sn[j] = 0.f;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        g0[j] = y0[j] * cs[j] + y1[j] * sn[j];
-        g1[j] = y1[j] * cs[j] - y0[j] * sn[j];
-      }
-    }
-    if (NORM) {  // v heads run along with their own loads idle: the shuffles want whole waves
-      const unsigned short* in = a.qkv + t * a.row_stride + static_cast<int64_t>(head) * D + c;
-      const bool use = live && !is_v;
-      float x0[8], x1[8];
-      up8<T>(use ? ld8(in) : bf16x8{}, x0);
-      up8<T>(use ? ld8(in + half) : bf16x8{}, x1);
-      float ss = 0.f, gx = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        ss += x0[j] * x0[j] + x1[j] * x1[j];
-        gx += g0[j] * (is_q ? wq0[j] : wk0[j]) * x0[j] + g1[j] * (is_q ? wq1[j] : wk1[j]) * x1[j];
-      }
-      ss = head_sum<L>(ss);
-      gx = head_sum<L>(gx);
-      if (use) {
-        const float r = 1.f / sqrtf(ss * (1.f / D) + a.eps);
-        const float m = gx * (1.f / D) * r * r;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float s0 = g0[j] * x0[j] * r, s1 = g1[j] * x1[j] * r;
-          if (is_q) aq[j] += s0, aq[8 + j] += s1;
-          else ak[j] += s0, ak[8 + j] += s1;
-          g0[j] = r * (g0[j] * (is_q ? wq0[j] : wk0[j]) - x0[j] * m);
-          g1[j] = r * (g1[j] * (is_q ? wq1[j] : wk1[j]) - x1[j] * m);
+          g0[j] = y0[j] * cs[j] + y1[j] * sn[j];
+          g1[j] = y1[j] * cs[j] - y0[j] * sn[j];
+        }
+        if (NORM) {
+          const unsigned short* x = a.qkv + t * a.row_stride + static_cast<int64_t>(first + head) * D + c;
+          float x0[8], x1[8];
+          up8<T>(ld8(x), x0);
+          up8<T>(ld8(x + half), x1);
+          float ss = 0.f, gx = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            ss += x0[j] * x0[j] + x1[j] * x1[j];
+            gx += g0[j] * w0[j] * x0[j] + g1[j] * w1[j] * x1[j];
+          }
+          ss = head_sum<L>(ss);
+          gx = head_sum<L>(gx);
+          const float r = 1.f / sqrtf(ss * (1.f / D) + a.eps);
+          const float m = gx * (1.f / D) * r * r;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            acc[j] += g0[j] * x0[j] * r;
+            acc[8 + j] += g1[j] * x1[j] * r;
+            g0[j] = r * (g0[j] * w0[j] - x0[j] * m);
+            g1[j] = r * (g1[j] * w1[j] - x1[j] * m);
+          }
         }
       }
+      st8(out, down8<T>(g0));
+      st8(out + half, down8<T>(g1));
     }
-    st8(out + c, is_v ? lo : down8<T>(g0));
-    st8(out + half + c, is_v ? hi : down8<T>(g1));
+  };
+  float* part = a.part + static_cast<int64_t>(blockIdx.x) * 2 * D;
+  {
+    float acc[16] = {};
+    sweep(a.dq, a.wq, a.Hq, 0, acc);
+    if (NORM) reduce_dw<L>(acc, c, red, part);
   }
-  if (NORM) {
-    // Lanes of one chunk (same lane % L), then the four waves, in a fixed order.
-    __shared__ float red[kThreads / kWave][2][D];
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-#pragma unroll
-      for (int off = kWave / 2; off >= L; off >>= 1) {
-        aq[j] += __shfl_xor(aq[j], off, kWave);
-        ak[j] += __shfl_xor(ak[j], off, kWave);
-      }
-    }
-    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-    if (lane < L) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        red[wave][0][c + j] = aq[j];
-        red[wave][0][half + c + j] = aq[8 + j];
-        red[wave][1][c + j] = ak[j];
-        red[wave][1][half + c + j] = ak[8 + j];
-      }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 2 * D; i += kThreads) {
-      float s = 0.f;
-#pragma unroll
-      for (int w = 0; w < kThreads / kWave; ++w) s += red[w][i / D][i % D];
-      a.part[static_cast<int64_t>(blockIdx.x) * 2 * D + i] = s;
-    }
+  {
+    float acc[16] = {};
+    sweep(a.dk, a.wk, a.Hkv, a.Hq, acc);
+    if (NORM) reduce_dw<L>(acc, c, red, part + D);
+  }
+  const int64_t n = static_cast<int64_t>(a.T) * a.Hkv * L;
+  for (int64_t i = start; i < n; i += step) {  // values: a copy
+    const int64_t th = i / L, t = th / a.Hkv;
+    const int head = static_cast<int>(th - t * a.Hkv);
+    const int cp = a.pos != nullptr ? a.pos[t] : static_cast<int>(t % a.period);
+    const bool live = cp >= 0 && static_cast<int64_t>(cp) + a.offset < a.table_rows;
+    const unsigned short* y = a.dv + th * D + c;
+    unsigned short* out = a.dqkv + (t * Ht + a.Hq + a.Hkv + head) * static_cast<int64_t>(D) + c;
+    st8(out, live ? ld8(y) : bf16x8{});
+    st8(out + half, live ? ld8(y + half) : bf16x8{});
   }
 }
 
-// dw[2, D] = sum of the workgroups' partials: 16 columns x 16 row groups per
-// workgroup, the groups joined through LDS in a fixed order.
+// dw[2, D] = sum of the workgroups' partials: 16 columns x 64 row groups per
+// workgroup (16 rows each at most, four loads in flight), the groups joined
+// through LDS in a fixed order.  With 16 row groups: 20 us.
+constexpr int kDwThreads = 1024, kDwGroups = kDwThreads / 16;
 template <class T>
-__global__ __launch_bounds__(kThreads) void norm_rope_dw_kernel(const float* __restrict__ part, int blocks,
+__global__ __launch_bounds__(kDwThreads) void norm_rope_dw_kernel(const float* __restrict__ part, int blocks,
                                                                 int D, unsigned short* __restrict__ dwq,
                                                                 unsigned short* __restrict__ dwk) {
-  __shared__ float red[16][17];
+  __shared__ float red[kDwGroups][17];
   const int col = threadIdx.x % 16, grp = threadIdx.x / 16;
   const int i = blockIdx.x * 16 + col;  // 2 * D is a multiple of 16
   float s = 0.f;
-  for (int b = grp; b < blocks; b += 16) s += part[static_cast<int64_t>(b) * 2 * D + i];
+#pragma unroll 4
+  for (int b = grp; b < blocks; b += kDwGroups) s += part[static_cast<int64_t>(b) * 2 * D + i];
   red[grp][col] = s;
   __syncthreads();
   if (grp == 0) {
     float t = 0.f;
 #pragma unroll
-    for (int g = 0; g < 16; ++g) t += red[g][col];
+    for (int g = 0; g < kDwGroups; ++g) t += red[g][col];
     (i < D ? dwq[i] : dwk[i - D]) = T::down(t);
   }
 }
@@ -346,7 +360,7 @@ int bwd(const BwdArgs& a, int D, int grid, unsigned short* dwq, unsigned short* 
     case 256: rc = bwd_launch<T, 16>(a, grid, s); break;
   }
   if (rc || a.wq == nullptr) return rc;
-  hipLaunchKernelGGL((norm_rope_dw_kernel<T>), dim3(2 * D / 16), dim3(kThreads), 0, s, a.part, grid, D, dwq, dwk);
+  hipLaunchKernelGGL((norm_rope_dw_kernel<T>), dim3(2 * D / 16), dim3(kDwThreads), 0, s, a.part, grid, D, dwq, dwk);
   return KGWE_CHECK_LAUNCH();
 }
 

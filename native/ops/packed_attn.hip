@@ -8,6 +8,12 @@
 //   dV_j = sum_i p_ij dO_i          dP_ij = dO_i v_j      D_i = dO_i o_i
 //   dS = p (dP - D)   dQ_i = s sum_j dS_ij k_j   dK_j = s sum_i dS_ij q_i
 //
+// D comes from the unrounded o: the forward also stores what its rounding
+// dropped (one more 16-bit value), since D is subtracted from every dP of the
+// row and an error of o's rounding would show in dQ and dK (2.6e-3 of the
+// gradient's norm in bf16, against 2.3e-3 for the roundings of dS and of the
+// result alone).
+//
 // One workgroup = 4 waves = 128 rows of one sequence and head (a job of the
 // batch's plan, longest sweep first); q, k, v are read through their strides,
 // so slices of a fused projection need no copy.  Tiles of 64 keys go HBM ->
@@ -56,6 +62,7 @@ struct FwdArgs {
   Batch b;
   View q, k, v, pk, pv;
   u16* o;      // [T, Hq, D]
+  u16* o_low;  // what the rounding of o dropped, rounded in turn; null: not wanted
   float* lse;  // [Hq, T], log2 units; null: not wanted
   int P, causal;
   float c;     // scale * log2 e
@@ -190,7 +197,16 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(FwdArgs a) {
   const float lt = half_add(l);
   const bool ok = qrow < len;
   const int64_t orow = static_cast<int64_t>(row0) + qrow;
-  store_row<T, NB>(a.o + (orow * a.b.Hq + h) * D, oacc, lt == 0.f ? 0.f : 1.f / lt, hh, ok);
+  const float inv = lt == 0.f ? 0.f : 1.f / lt;
+  const int64_t off = (orow * a.b.Hq + h) * D;
+  store_row<T, NB>(a.o + off, oacc, inv, hh, ok);
+  if (a.o_low != nullptr) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) oacc[i][r] = oacc[i][r] * inv - T::up(T::down(oacc[i][r] * inv));
+    store_row<T, NB>(a.o_low + off, oacc, 1.f, hh, ok);
+  }
   if (a.lse != nullptr && ok && hh == 0)
     a.lse[static_cast<int64_t>(h) * a.b.T + orow] = lt == 0.f ? -INFINITY : m + log2f(lt);
 }
@@ -199,6 +215,7 @@ struct BwdArgs {
   Batch b;
   View q, k, v;
   const u16* o;       // [T, Hq, D]
+  const u16* o_low;
   const u16* dout;    // [T, Hq, D]
   const float* lse;   // [Hq, T]
   float* delta;       // [Hq, T]: written by the dQ kernel, read by the dK / dV kernel
@@ -242,8 +259,9 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(BwdArgs a) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const bf16x8 ov = ok ? *reinterpret_cast<const bf16x8*>(a.o + off + 16 * t + 8 * hh) : bf16x8{};
+      const bf16x8 lv = ok ? *reinterpret_cast<const bf16x8*>(a.o_low + off + 16 * t + 8 * hh) : bf16x8{};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) dsum = fmaf(T::up(df[t][e]), T::up(ov[e]), dsum);
+      for (int e = 0; e < 8; ++e) dsum = fmaf(T::up(df[t][e]), T::up(ov[e]) + T::up(lv[e]), dsum);
     }
   }
   const int64_t li = static_cast<int64_t>(h) * a.b.T + row;
@@ -477,40 +495,41 @@ int bwd(const BwdArgs& a, int J, hipStream_t s) {
 
 // Row / head strides in elements.  cu [N + 2] and jobs [J, 2] from
 // kgwe_packed_plan for the same N and T.  Prefix keys / values [Hkv, P, D] by
-// strides (P = 0: none).  o contiguous [T, Hq, D]; lse [Hq, T] or null.
+// strides (P = 0: none).  o contiguous [T, Hq, D]; o_low (alike) and lse [Hq, T]
+// are what the gradient needs, or null.
 KGWE_API int kgwe_packed_attn_fwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
                                   int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const void* pk,
                                   int64_t pk_row, int64_t pk_head, const void* pv, int64_t pv_row, int64_t pv_head,
-                                  int P, void* o, float* lse, const int* cu, const int* jobs, int J, int N, int T,
+                                  int P, void* o, void* o_low, float* lse, const int* cu, const int* jobs, int J, int N, int T,
                                   int Hq, int Hkv, int D, float scale, int causal, int dtype, hipStream_t s) {
   if (!shape_ok(N, T, J, Hq, Hkv, D, dtype) || P < 0) return -1;
   if (!view_ok(q, q_row, q_head) || !view_ok(k, k_row, k_head) || !view_ok(v, v_row, v_head)) return -1;
   if (P > 0 && (!pk || !pv || !view_ok(pk, pk_row, pk_head) || !view_ok(pv, pv_row, pv_head))) return -1;
-  if (reinterpret_cast<uintptr_t>(o) & 15) return -1;
+  if ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(o_low)) & 15) return -1;
   const FwdArgs a{{cu, reinterpret_cast<const int2*>(jobs), N, T, Hq, Hkv},
                   {static_cast<const u16*>(q), q_row, q_head}, {static_cast<const u16*>(k), k_row, k_head},
                   {static_cast<const u16*>(v), v_row, v_head}, {static_cast<const u16*>(pk), pk_row, pk_head},
-                  {static_cast<const u16*>(pv), pv_row, pv_head}, static_cast<u16*>(o), lse, P, causal,
+                  {static_cast<const u16*>(pv), pv_row, pv_head}, static_cast<u16*>(o), static_cast<u16*>(o_low), lse, P, causal,
                   scale * kLog2e};
   if (dtype == kTypeBf16) return D == 64 ? fwd<Bf16, 64>(a, J, s) : fwd<Bf16, 128>(a, J, s);
   return D == 64 ? fwd<Fp16, 64>(a, J, s) : fwd<Fp16, 128>(a, J, s);
 }
 
-// o, lse: the forward's; dout contiguous [T, Hq, D]; delta fp32 [Hq, T]
+// o, o_low, lse: the forward's; dout contiguous [T, Hq, D]; delta fp32 [Hq, T]
 // workspace; dq [T, Hq, D], dk, dv [T, Hkv, D] contiguous, every row written.
 KGWE_API int kgwe_packed_attn_bwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
                                   int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const void* o,
-                                  const float* lse, const void* dout, float* delta, void* dq, void* dk, void* dv,
+                                  const void* o_low, const float* lse, const void* dout, float* delta, void* dq, void* dk, void* dv,
                                   const int* cu, const int* jobs, int J, int N, int T, int Hq, int Hkv, int D,
                                   float scale, int causal, int dtype, hipStream_t s) {
   if (!shape_ok(N, T, J, Hq, Hkv, D, dtype) || !lse || !delta) return -1;
   if (!view_ok(q, q_row, q_head) || !view_ok(k, k_row, k_head) || !view_ok(v, v_row, v_head)) return -1;
-  for (const void* p : {o, dout, static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv)})
+  for (const void* p : {o, o_low, dout, static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv)})
     if (!p || (reinterpret_cast<uintptr_t>(p) & 15)) return -1;
   const BwdArgs a{{cu, reinterpret_cast<const int2*>(jobs), N, T, Hq, Hkv},
                   {static_cast<const u16*>(q), q_row, q_head}, {static_cast<const u16*>(k), k_row, k_head},
                   {static_cast<const u16*>(v), v_row, v_head}, static_cast<const u16*>(o),
-                  static_cast<const u16*>(dout), lse, delta, static_cast<u16*>(dq), static_cast<u16*>(dk),
+                  static_cast<const u16*>(o_low), static_cast<const u16*>(dout), lse, delta, static_cast<u16*>(dq), static_cast<u16*>(dk),
                   static_cast<u16*>(dv), causal, scale * kLog2e, scale};
   if (dtype == kTypeBf16) return D == 64 ? bwd<Bf16, 64>(a, J, s) : bwd<Bf16, 128>(a, J, s);
   return D == 64 ? bwd<Fp16, 64>(a, J, s) : bwd<Fp16, 128>(a, J, s);
