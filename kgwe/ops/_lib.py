@@ -79,11 +79,11 @@ _SIGS = {
     "kgwe_packed_plan_jobs": (c_int, [c_int, c_int]),
     "kgwe_packed_plan": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
                                  c_void_p]),
-    "kgwe_packed_attn_fwd": (c_int, [*[c_void_p, c_int64, c_int64] * 5, c_int, *[c_void_p] * 5, *[c_int] * 6, c_float, c_int, c_int, c_void_p]),
+    "kgwe_packed_attn_fwd": (c_int, [*[c_void_p, c_int64, c_int64] * 5, c_int, *[c_void_p] * 4, *[c_int] * 5, c_float, c_int, c_int, c_void_p]),
     "kgwe_prefix_attn_workspace": (c_int64, [c_int] * 6),
     "kgwe_prefix_attn": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, *[c_void_p] * 5, *[c_int] * 6,
                                  c_float, c_int, c_void_p]),
-    "kgwe_packed_attn_bwd": (c_int, [*[c_void_p, c_int64, c_int64] * 3, *[c_void_p] * 10, *[c_int] * 6, c_float,
+    "kgwe_packed_attn_bwd": (c_int, [*[c_void_p, c_int64, c_int64] * 3, *[c_void_p] * 9, *[c_int] * 5, c_float,
                                      c_int, c_int, c_void_p]),
 }
 _OPTIONAL_SIGS = {

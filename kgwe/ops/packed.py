@@ -102,10 +102,9 @@ class PackedBatch:
             self.jobs = None
             return
         slots = int(lib().kgwe_packed_plan_jobs(n, T))
-        self.jobs = torch.empty(slots, 2, dtype=torch.int32, device=dev)
+        self.jobs = torch.empty(slots, 4, dtype=torch.int32, device=dev)
         first = torch.empty(n + 2, dtype=torch.int32, device=dev)
-        # what the attention launches pass on: cu, jobs, job slots, sequences
-        self.tables = (self.cu.data_ptr(), self.jobs.data_ptr(), slots, n)
+        self.tables = (self.jobs.data_ptr(), slots)  # what the attention launches pass on
         check(lib().kgwe_packed_plan(ptr(self.lengths), n, T, ptr(self.cu), ptr(first), ptr(self.jobs), slots,
                                      ptr(self.positions), ptr(self.seq_ids), stream(self.cu)), "packed_plan")
 

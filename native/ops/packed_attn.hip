@@ -37,21 +37,28 @@ struct View {
 };
 
 struct Batch {
-  const int* cu;    // [N + 2]
-  const int2* jobs;
-  int N, T, Hq, Hkv;
+  const int4* jobs;
+  int T, Hq, Hkv;
+};
+
+// A workgroup's block of a sequence: `rows` rows from `row0` on, of which it
+// takes 128 from 128 * blk on; `keys` of them are keys too (padding: none).
+struct Job {
+  int row0, rows, blk, keys;
 };
 
 // Job and head of this workgroup: all heads of a job are neighbours, and on
 // Hq % 8 == 0 each of the 8 XCDs (workgroups go round them) takes a contiguous
 // run of heads, so the heads that share keys share an L2.
-__device__ __forceinline__ bool pick(const Batch& b, int heads, int* seq, int* blk, int* head) {
+__device__ __forceinline__ bool pick(const Batch& b, int heads, Job* job, int* head) {
   const int j = blockIdx.x / heads, p = blockIdx.x - j * heads;
   *head = heads % 8 == 0 ? (p % 8) * (heads / 8) + p / 8 : p;
-  const int2 jb = b.jobs[j];
-  *seq = __builtin_amdgcn_readfirstlane(jb.x);
-  *blk = __builtin_amdgcn_readfirstlane(jb.y);
-  return *seq >= 0;
+  const int4 v = b.jobs[j];
+  job->row0 = __builtin_amdgcn_readfirstlane(v.x);
+  job->rows = __builtin_amdgcn_readfirstlane(v.y);
+  job->blk = __builtin_amdgcn_readfirstlane(v.z);
+  job->keys = __builtin_amdgcn_readfirstlane(v.w);
+  return job->rows > 0;
 }
 
 // Running max kept until a tile's max passes it by this much (log2 units), so
@@ -75,13 +82,13 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(FwdArgs a) {
   // One array per stage: the compiler orders an LDS read after every DMA in
   // flight that it cannot prove to go to another object.
   __shared__ __attribute__((aligned(1024))) char K0[kImg], V0[kImg], K1[kImg], V1[kImg];
-  int seq, blk, h;
-  if (!pick(a.b, a.b.Hq, &seq, &blk, &h)) return;
+  Job job;
+  int h;
+  if (!pick(a.b, a.b.Hq, &job, &h)) return;
   const int hkv = h / (a.b.Hq / a.b.Hkv);
-  const int row0 = __builtin_amdgcn_readfirstlane(a.b.cu[seq]);
-  const int len = __builtin_amdgcn_readfirstlane(a.b.cu[seq + 1]) - row0;  // query rows
-  const int klen = seq < a.b.N ? len : 0;                                  // padding rows see nothing
-  const int plen = PREFIX && seq < a.b.N ? a.P : 0;
+  const int row0 = job.row0, len = job.rows, blk = job.blk;
+  const int klen = job.keys;  // padding rows see nothing
+  const int plen = PREFIX && klen > 0 ? a.P : 0;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lq = lane & 31, hh = lane >> 5;
   const int q0 = blk * kRows + w * 32, qrow = q0 + lq;
@@ -233,12 +240,11 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(BwdArgs a) {
   constexpr int NB = D / 32, NT = D / 16;
   constexpr int kImg = kTile * D * 2;
   __shared__ __attribute__((aligned(1024))) char K0[kImg], V0[kImg], K1[kImg], V1[kImg];
-  int seq, blk, h;
-  if (!pick(a.b, a.b.Hq, &seq, &blk, &h)) return;
+  Job job;
+  int h;
+  if (!pick(a.b, a.b.Hq, &job, &h)) return;
   const int hkv = h / (a.b.Hq / a.b.Hkv);
-  const int row0 = __builtin_amdgcn_readfirstlane(a.b.cu[seq]);
-  const int len = __builtin_amdgcn_readfirstlane(a.b.cu[seq + 1]) - row0;
-  const int klen = seq < a.b.N ? len : 0;
+  const int row0 = job.row0, len = job.rows, blk = job.blk, klen = job.keys;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lq = lane & 31, hh = lane >> 5;
   const int q0 = blk * kRows + w * 32, qrow = q0 + lq;
@@ -348,14 +354,14 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(BwdArgs a) {
   __shared__ __attribute__((aligned(1024))) char Q0[kImg], O0[kImg], Q1[kImg], O1[kImg];
   __shared__ __attribute__((aligned(1024))) char Vw[kRows * D * 2];
   __shared__ __attribute__((aligned(256))) float L0[64], L1[64];  // lse and -D of a tile's 32 rows
-  int seq, blk, hkv;
-  if (!pick(a.b, a.b.Hkv, &seq, &blk, &hkv)) return;
+  Job job;
+  int hkv;
+  if (!pick(a.b, a.b.Hkv, &job, &hkv)) return;
   const int G = a.b.Hq / a.b.Hkv;
-  const int row0 = __builtin_amdgcn_readfirstlane(a.b.cu[seq]);
-  const int len = __builtin_amdgcn_readfirstlane(a.b.cu[seq + 1]) - row0;
-  const int qlen = seq < a.b.N ? len : 0;  // nothing looks at padding
+  const int row0 = job.row0, len = job.rows;
+  const int qlen = job.keys;  // nothing looks at padding
   const int nblk = (len + kRows - 1) / kRows;
-  const int kb = nblk - 1 - blk;  // the job table's order, mirrored: the first keys sweep longest
+  const int kb = nblk - 1 - job.blk;  // the job table's order, mirrored: the first keys sweep longest
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lk = lane & 31, hh = lane >> 5;
   const int key0 = kb * kRows + w * 32, key = key0 + lk;
@@ -472,8 +478,8 @@ inline bool view_ok(const void* p, int64_t row, int64_t head) {
          row <= (1 << 22);
 }
 
-inline bool shape_ok(int N, int T, int J, int Hq, int Hkv, int D, int dtype) {
-  return N >= 0 && T > 0 && J > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && (D == 64 || D == 128) &&
+inline bool shape_ok(int T, int J, int Hq, int Hkv, int D, int dtype) {
+  return T > 0 && J > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && (D == 64 || D == 128) &&
          (dtype == kTypeBf16 || dtype == kTypeFp16) && static_cast<int64_t>(J) * Hq < (1LL << 31) &&
          static_cast<int64_t>(Hq) * D < (1 << 22);
 }
@@ -496,20 +502,20 @@ int bwd(const BwdArgs& a, int J, hipStream_t s) {
 
 }  // namespace
 
-// Row / head strides in elements.  cu [N + 2] and jobs [J, 2] from
-// kgwe_packed_plan for the same N and T.  Prefix keys / values [Hkv, P, D] by
+// Row / head strides in elements.  jobs [J, 4] from
+// kgwe_packed_plan for the same T.  Prefix keys / values [Hkv, P, D] by
 // strides (P = 0: none).  o contiguous [T, Hq, D]; o_low (alike) and lse [Hq, T]
 // are what the gradient needs, or null.
 KGWE_API int kgwe_packed_attn_fwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
                                   int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const void* pk,
                                   int64_t pk_row, int64_t pk_head, const void* pv, int64_t pv_row, int64_t pv_head,
-                                  int P, void* o, void* o_low, float* lse, const int* cu, const int* jobs, int J, int N, int T,
+                                  int P, void* o, void* o_low, float* lse, const int* jobs, int J, int T,
                                   int Hq, int Hkv, int D, float scale, int causal, int dtype, hipStream_t s) {
-  if (!shape_ok(N, T, J, Hq, Hkv, D, dtype) || P < 0) return -1;
+  if (!shape_ok(T, J, Hq, Hkv, D, dtype) || P < 0) return -1;
   if (!view_ok(q, q_row, q_head) || !view_ok(k, k_row, k_head) || !view_ok(v, v_row, v_head)) return -1;
   if (P > 0 && (!pk || !pv || !view_ok(pk, pk_row, pk_head) || !view_ok(pv, pv_row, pv_head))) return -1;
   if ((reinterpret_cast<uintptr_t>(o) | reinterpret_cast<uintptr_t>(o_low)) & 15) return -1;
-  const FwdArgs a{{cu, reinterpret_cast<const int2*>(jobs), N, T, Hq, Hkv},
+  const FwdArgs a{{reinterpret_cast<const int4*>(jobs), T, Hq, Hkv},
                   {static_cast<const u16*>(q), q_row, q_head}, {static_cast<const u16*>(k), k_row, k_head},
                   {static_cast<const u16*>(v), v_row, v_head}, {static_cast<const u16*>(pk), pk_row, pk_head},
                   {static_cast<const u16*>(pv), pv_row, pv_head}, static_cast<u16*>(o), static_cast<u16*>(o_low), lse, P, causal,
@@ -523,13 +529,13 @@ KGWE_API int kgwe_packed_attn_fwd(const void* q, int64_t q_row, int64_t q_head, 
 KGWE_API int kgwe_packed_attn_bwd(const void* q, int64_t q_row, int64_t q_head, const void* k, int64_t k_row,
                                   int64_t k_head, const void* v, int64_t v_row, int64_t v_head, const void* o,
                                   const void* o_low, const float* lse, const void* dout, float* delta, void* dq, void* dk, void* dv,
-                                  const int* cu, const int* jobs, int J, int N, int T, int Hq, int Hkv, int D,
+                                  const int* jobs, int J, int T, int Hq, int Hkv, int D,
                                   float scale, int causal, int dtype, hipStream_t s) {
-  if (!shape_ok(N, T, J, Hq, Hkv, D, dtype) || !lse || !delta) return -1;
+  if (!shape_ok(T, J, Hq, Hkv, D, dtype) || !lse || !delta) return -1;
   if (!view_ok(q, q_row, q_head) || !view_ok(k, k_row, k_head) || !view_ok(v, v_row, v_head)) return -1;
   for (const void* p : {o, o_low, dout, static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv)})
     if (!p || (reinterpret_cast<uintptr_t>(p) & 15)) return -1;
-  const BwdArgs a{{cu, reinterpret_cast<const int2*>(jobs), N, T, Hq, Hkv},
+  const BwdArgs a{{reinterpret_cast<const int4*>(jobs), T, Hq, Hkv},
                   {static_cast<const u16*>(q), q_row, q_head}, {static_cast<const u16*>(k), k_row, k_head},
                   {static_cast<const u16*>(v), v_row, v_head}, static_cast<const u16*>(o),
                   static_cast<const u16*>(o_low), static_cast<const u16*>(dout), lse, delta, static_cast<u16*>(dq), static_cast<u16*>(dk),

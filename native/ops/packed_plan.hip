@@ -6,11 +6,13 @@
 //                  rows cu[N] .. cu[N + 1] = T are padding ("sequence" N)
 //   pos [T]        position of a row inside its sequence, -1 for padding
 //   seq [T]        its sequence, -1 for padding
-//   jobs [J] int2  (sequence, block of 128 rows), longest sweep first: a causal
-//                  query block b sweeps b + 1 key blocks, and its mirror image
-//                  (the key block nblk - 1 - b) is swept by as many query
-//                  blocks, so one table orders forward and backward.  Slots
-//                  past the last job hold sequence -1.
+//   jobs [J] int4  (first row, rows, block of 128 rows, keys) of a sequence's
+//                  blocks (keys = rows, 0 for the padding), longest sweep
+//                  first: a causal query block b sweeps b + 1 key blocks, and
+//                  its mirror image (the key block nblk - 1 - b) is swept by
+//                  as many query blocks, so one table orders forward and
+//                  backward.  All a workgroup needs is in its slot: one load,
+//                  not a chain of two.  Slots past the last job hold rows = 0.
 //
 // Lengths below zero count as zero, and what passes T is cut off, so no table
 // entry ever points outside the batch's rows.
@@ -59,7 +61,7 @@ __device__ __forceinline__ int last_at_most(const int* a, int n, int x) {
 
 // first [N + 2]: workspace, the number of each sequence's first job.
 __global__ __launch_bounds__(kThreads) void plan_kernel(const int* __restrict__ lengths, int N, int T, int* cu,
-                                                        int* first, int2* __restrict__ jobs, int J) {
+                                                        int* first, int4* __restrict__ jobs, int J) {
   __shared__ int sh[kThreads / kWave];
   __shared__ int count[kBuckets];
   // 1. rows: running sum of the lengths, cut at T
@@ -125,9 +127,10 @@ __global__ __launch_bounds__(kThreads) void plan_kernel(const int* __restrict__ 
   for (int j = threadIdx.x; j < njobs; j += kThreads) {
     const int s = last_at_most(first, N + 1, j);
     const int b = j - first[s];
-    jobs[atomicAdd(&count[bucket(s, b)], 1)] = make_int2(s, b);
+    const int row0 = cu[s], rows = cu[s + 1] - row0;
+    jobs[atomicAdd(&count[bucket(s, b)], 1)] = make_int4(row0, rows, b, s < N ? rows : 0);
   }
-  for (int j = njobs + threadIdx.x; j < J; j += kThreads) jobs[j] = make_int2(-1, 0);
+  for (int j = njobs + threadIdx.x; j < J; j += kThreads) jobs[j] = make_int4(0, 0, 0, 0);
 }
 static_assert(kBuckets == 2 * kThreads, "two buckets per thread");
 
@@ -149,12 +152,12 @@ KGWE_API int kgwe_packed_plan_jobs(int N, int T) {
   return static_cast<int>(most < T ? most : T);
 }
 
-// cu and first: int32 [N + 2]; jobs: int32 [jobs, 2]; pos, seq: int32 [T].
+// cu and first: int32 [N + 2]; jobs: int32 [jobs, 4], 16-byte aligned; pos, seq: int32 [T].
 KGWE_API int kgwe_packed_plan(const int* lengths, int N, int T, int* cu, int* first, int* jobs, int J, int* pos,
                               int* seq, hipStream_t s) {
   if (N < 0 || T <= 0 || J < kgwe_packed_plan_jobs(N, T) || N > (1 << 24) || T > 0x7fffffff - 256) return -1;
   hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(kThreads), 0, s, lengths, N, T, cu, first,
-                     reinterpret_cast<int2*>(jobs), J);
+                     reinterpret_cast<int4*>(jobs), J);
   if (int rc = KGWE_CHECK_LAUNCH()) return rc;
   hipLaunchKernelGGL(rows_kernel, dim3((T + 255) / 256), dim3(256), 0, s, cu, N, T, pos, seq);
   return KGWE_CHECK_LAUNCH();

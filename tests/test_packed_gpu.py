@@ -45,10 +45,11 @@ def test_plan_tables(lengths, total):
                   PackedBatch(torch.tensor(lengths, dtype=torch.int32, device="cuda"), total=total)):
         for name in ("cu", "positions", "seq_ids", "last_rows"):
             assert torch.equal(getattr(batch, name).cpu(), getattr(host, name)), name
-        jobs = [tuple(j) for j in batch.jobs.tolist() if j[0] >= 0]
+        jobs = [tuple(j) for j in batch.jobs.tolist() if j[1] > 0]
         full = [*lengths, total - sum(lengths)]
-        assert sorted(jobs) == [(s, b) for s, n in enumerate(full) for b in range((n + 127) // 128)]
-        sweep = [-1 if s == len(lengths) else min(b, 2046) for s, b in jobs]
+        assert sorted(jobs) == sorted((sum(full[:s]), n, b, n if s < len(lengths) else 0)
+                                      for s, n in enumerate(full) for b in range((n + 127) // 128))
+        sweep = [-1 if keys == 0 else min(b, 2046) for _, _, b, keys in jobs]
         assert sweep == sorted(sweep, reverse=True)  # longest first, padding last
 
 
@@ -56,7 +57,7 @@ def test_plan_of_lengths_that_do_not_fit_stays_inside():
     lengths = torch.tensor([5, -7, 2**31 - 1, 2**31 - 1, 4], dtype=torch.int32, device="cuda")
     batch = PackedBatch(lengths, total=300)
     assert batch.cu.tolist() == [0, 5, 5, 300, 300, 300, 300]
-    assert sorted(j for j in batch.jobs.tolist() if j[0] >= 0) == [[0, 0], [2, 0], [2, 1], [2, 2]]
+    assert sorted(j for j in batch.jobs.tolist() if j[1] > 0) == [[0, 5, 0, 5], *([5, 295, b, 295] for b in range(3))]
     with pytest.raises(ValueError):
         PackedBatch(lengths)
 
