@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 import torch
@@ -73,18 +74,11 @@ _SIGS = {
                                 c_int, c_int, c_int, c_int, c_void_p]),
     "kgwe_wgrad_splits": (c_int, [c_int, c_int, c_int]),
     "kgwe_wgrad_workspace": (c_int64, [c_int, c_int, c_int]),
-    "kgwe_norm_rope_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_int, *[c_void_p] * 10, *[c_int] * 8, c_float, c_int, c_void_p]),
     "kgwe_norm_rope_bwd_blocks": (c_int, [c_int, c_int, c_int, c_int]),
-    "kgwe_norm_rope_bwd": (c_int, [c_void_p, c_int64, c_void_p, c_int, *[c_void_p] * 11, *[c_int] * 6, c_float, c_int, c_void_p]),
     "kgwe_packed_plan_jobs": (c_int, [c_int, c_int]),
     "kgwe_packed_plan": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
                                  c_void_p]),
-    "kgwe_packed_attn_fwd": (c_int, [*[c_void_p, c_int64, c_int64] * 5, c_int, *[c_void_p] * 4, *[c_int] * 5, c_float, c_int, c_int, c_void_p]),
     "kgwe_prefix_attn_workspace": (c_int64, [c_int] * 6),
-    "kgwe_prefix_attn": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, *[c_void_p] * 5, *[c_int] * 6,
-                                 c_float, c_int, c_void_p]),
-    "kgwe_packed_attn_bwd": (c_int, [*[c_void_p, c_int64, c_int64] * 3, *[c_void_p] * 9, *[c_int] * 5, c_float,
-                                     c_int, c_int, c_void_p]),
 }
 _OPTIONAL_SIGS = {
     "kgwe_flash_attn_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -96,6 +90,17 @@ _OPTIONAL_SIGS = {
                                     c_int, c_void_p]),
     "kgwe_flash_attn_bwd_workspace": (c_int64, [c_int, c_int, c_int, c_int, c_int]),
 }
+
+
+# Entries that take one packed record and the stream (the record's C struct
+# stands beside the entry): pointers, then int64, then int32, then fp32 fields.
+RECORDS = {name: struct.Struct(f"@{p}Q{q}q{i}i{f}f0q") for name, (p, q, i, f) in {
+    "kgwe_packed_attn_fwd": (9, 10, 8, 1),
+    "kgwe_packed_attn_bwd": (12, 6, 7, 1),
+    "kgwe_norm_rope_fwd": (12, 1, 10, 1),
+    "kgwe_norm_rope_bwd": (13, 1, 8, 1),
+    "kgwe_prefix_attn": (8, 2, 7, 1),
+}.items()}
 
 
 class KernelLibraryMissing(RuntimeError):
@@ -124,6 +129,12 @@ def lib():
         if fn is not None:
             fn.restype = res
             fn.argtypes = args
+    for name, rec in RECORDS.items():
+        fn, size = getattr(L, name), getattr(L, name + "_bytes")
+        fn.restype, fn.argtypes = c_int, [ctypes.c_char_p, c_void_p]
+        size.restype, size.argtypes = c_int, []
+        if size() != rec.size:
+            raise KernelLibraryMissing(f"{_LIB_PATH}: {name} takes {size()} bytes, expected {rec.size}; rebuild it")
     _lib = L
     return L
 
@@ -174,19 +185,25 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def launch(fn, what: str, device: torch.device, *args) -> None:
-    """fn(*args, current stream of ``device``) with ``device`` current, whatever
-    the caller's current device is.  (Small calls are host-bound: switching the
-    device only where it differs, and the raw stream handle in place of a Stream
-    object, save about 5 of 18 us.)"""
-    index = device.index
+def launch(name: str, device: torch.device, *fields) -> None:
+    """Call the record entry ``name`` on the current stream of ``device``, with
+    ``device`` current whatever the caller's current device is.  (Small calls
+    are host-bound: the device is switched only where it differs, the raw stream
+    handle stands in for a Stream object, and one packed record for up to 29
+    arguments that ctypes converts one by one.)"""
+    fn, record, index = getattr(_lib or lib(), name), RECORDS[name].pack(*fields), device.index
     if index == torch.cuda.current_device():
-        rc = fn(*args, _raw_stream(index))
+        rc = fn(record, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, _raw_stream(index))
+            rc = fn(record, _raw_stream(index))
     if rc != 0:
-        raise RuntimeError(f"{what} failed with code {rc}")
+        raise RuntimeError(f"{name} failed with code {rc}")
+
+
+def addr(t: torch.Tensor | None) -> int:
+    """Address for a record field: 0 for no tensor."""
+    return 0 if t is None else t.data_ptr()
 
 
 def use_hip(*tensors: torch.Tensor) -> bool:

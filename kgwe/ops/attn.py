@@ -18,7 +18,7 @@ import torch
 import torch.nn.functional as F
 
 from . import reference as ref
-from ._lib import HALF_TYPES, check, dense16, has_symbol, launch, lib, ptr, rows16, stream, use_hip
+from ._lib import HALF_TYPES, addr, check, dense16, has_symbol, launch, lib, ptr, rows16, stream, use_hip
 from .packed import PackedBatch
 
 
@@ -98,19 +98,26 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
 # --------------------------------------------------------------------------
 # Packed sequences
 # --------------------------------------------------------------------------
+_dense = {"memory_format": torch.contiguous_format}
+
+
 def _packed_fwd(q, k, v, batch, causal, prefix, train):
     T, Hq, D = q.shape
-    o = torch.empty((T, Hq, D), device=q.device, dtype=q.dtype)
-    lse = torch.empty((Hq, T), device=q.device, dtype=torch.float32) if train else None
-    low = torch.empty_like(o) if train else None  # what the rounding of o drops
+    o = torch.empty_like(q, **_dense)
+    low = lse = None
+    if train:
+        lse = torch.empty((Hq, T), device=q.device, dtype=torch.float32)
+        low = torch.empty_like(o)  # what the rounding of o drops
     (qr, qh, _), (kr, kh, _), (vr, vh, _) = q.stride(), k.stride(), v.stride()
-    pre = (None, 0, 0, None, 0, 0, 0)
-    if prefix is not None:  # [Hkv, P, D]: row stride, head stride
-        pk, pv = prefix
-        pre = (pk.data_ptr(), pk.stride(1), pk.stride(0), pv.data_ptr(), pv.stride(1), pv.stride(0), pk.shape[1])
-    launch(lib().kgwe_packed_attn_fwd, "packed_attn_fwd", q.device, q.data_ptr(), qr, qh, k.data_ptr(), kr, kh,
-           v.data_ptr(), vr, vh, *pre, o.data_ptr(), ptr(low), ptr(lse), *batch.tables, T, Hq, k.shape[1], D, D ** -0.5, causal,
-           HALF_TYPES[q.dtype])
+    jobs, slots = batch.tables
+    if prefix is None:
+        pk = pv = pkr = pkh = pvr = pvh = P = 0
+    else:  # [Hkv, P, D]: row stride, head stride
+        (pkh, pkr, _), (pvh, pvr, _), P = prefix[0].stride(), prefix[1].stride(), prefix[0].shape[1]
+        pk, pv = prefix[0].data_ptr(), prefix[1].data_ptr()
+    launch("kgwe_packed_attn_fwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), pk, pv, o.data_ptr(), addr(low),
+           addr(lse), jobs, qr, qh, kr, kh, vr, vh, pkr, pkh, pvr, pvh, P, slots, T, Hq, k.shape[1], D, causal,
+           HALF_TYPES[q.dtype], D ** -0.5)
     return o, low, lse
 
 
@@ -130,14 +137,13 @@ class _PackedAttn(torch.autograd.Function):
         T, Hq, D = q.shape
         Hkv = k.shape[1]
         do = dense16(do)
-        dq = torch.empty((T, Hq, D), device=q.device, dtype=q.dtype)
-        dk = torch.empty((T, Hkv, D), device=q.device, dtype=q.dtype)
-        dv = torch.empty_like(dk)
+        dq, dk, dv = (torch.empty_like(t, **_dense) for t in (q, k, k))
         delta = torch.empty_like(lse)
         (qr, qh, _), (kr, kh, _), (vr, vh, _) = q.stride(), k.stride(), v.stride()
-        launch(lib().kgwe_packed_attn_bwd, "packed_attn_bwd", q.device, q.data_ptr(), qr, qh, k.data_ptr(), kr, kh,
-               v.data_ptr(), vr, vh, o.data_ptr(), low.data_ptr(), lse.data_ptr(), do.data_ptr(), delta.data_ptr(), dq.data_ptr(),
-               dk.data_ptr(), dv.data_ptr(), *batch.tables, T, Hq, Hkv, D, D ** -0.5, ctx.causal, HALF_TYPES[q.dtype])
+        jobs, slots = batch.tables
+        launch("kgwe_packed_attn_bwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), low.data_ptr(),
+               lse.data_ptr(), do.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), jobs, qr, qh,
+               kr, kh, vr, vh, slots, T, Hq, Hkv, D, ctx.causal, HALF_TYPES[q.dtype], D ** -0.5)
         return dq, dk, dv, None, None
 
 

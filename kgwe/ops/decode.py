@@ -25,7 +25,7 @@ import math
 import torch
 
 from . import reference as ref
-from ._lib import HALF_TYPES, check, dense16, launch, lib, ptr, rows16, stream, use_hip
+from ._lib import HALF_TYPES, addr, check, dense16, launch, lib, ptr, rows16, stream, use_hip
 from .functional import check_norm_rope
 
 
@@ -143,7 +143,7 @@ def norm_rope_append(qkv: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, si
     k = v = None
     if keep_kv:
         k = torch.empty((T, hkv, d), device=device, dtype=dtype)
-        v = torch.empty((T, hkv, d), device=device, dtype=dtype)
+        v = torch.empty_like(k)
     if T > 0 and kc.numel() > 0:
         if (kc.data_ptr() | vc.data_ptr()) & 15:
             raise ValueError("norm_rope_append: caches must be 16-byte aligned")
@@ -151,9 +151,9 @@ def norm_rope_append(qkv: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, si
         if q_weight is not None:
             q_weight, k_weight = dense16(q_weight), dense16(k_weight)
         rows = None if rows is None else rows.contiguous()
-        launch(lib().kgwe_norm_rope_fwd, "norm_rope_append", device, qkv.data_ptr(), qkv.stride(0), pos.data_ptr(), 0,
-               cos.data_ptr(), sin.data_ptr(), ptr(q_weight), ptr(k_weight), q.data_ptr(), ptr(k), ptr(v), kc.data_ptr(),
-               vc.data_ptr(), ptr(rows), T, offset, cos.shape[0], hq, hkv, d, cache[2], cache[0], eps, HALF_TYPES[dtype])
+        launch("kgwe_norm_rope_fwd", device, qkv.data_ptr(), pos.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+               addr(q_weight), addr(k_weight), q.data_ptr(), addr(k), addr(v), kc.data_ptr(), vc.data_ptr(), addr(rows),
+               qkv.stride(0), T, 0, offset, cos.shape[0], hq, hkv, d, cache[2], cache[0], HALF_TYPES[dtype], eps)
     return (q, k, v) if keep_kv else q
 
 
@@ -261,9 +261,9 @@ class PrefixDecodeAttention:
             pk, pv = dense16(pk), dense16(pv)
         out = torch.empty_like(q)
         work = torch.empty(self.words, device=device, dtype=torch.float32) if self.words else None
-        launch(lib().kgwe_prefix_attn, "prefix_attn", device, q.data_ptr(), pk.data_ptr(), pv.data_ptr(),
-               max(pk.stride(1), d), pk.stride(0), kc.data_ptr(), vc.data_ptr(), lens.data_ptr(), ptr(work),
-               out.data_ptr(), B, hq, hkv, d, P, smax, d ** -0.5, HALF_TYPES[dtype])
+        launch("kgwe_prefix_attn", device, q.data_ptr(), pk.data_ptr(), pv.data_ptr(), kc.data_ptr(), vc.data_ptr(),
+               lens.data_ptr(), addr(work), out.data_ptr(), max(pk.stride(1), d), pk.stride(0), B, hq, hkv, d, P, smax,
+               HALF_TYPES[dtype], d ** -0.5)
         return out
 
 

@@ -11,7 +11,7 @@ import os
 import torch
 
 from . import reference as ref
-from ._lib import HALF_TYPES, check, dense16, launch, lib, ptr, rows16, stream, use_hip
+from ._lib import HALF_TYPES, addr, check, dense16, launch, lib, ptr, rows16, stream, use_hip
 from .gemm import wgrad, wgrad_supported
 
 
@@ -246,11 +246,11 @@ def _norm_rope_fwd(qkv, qw, kw, cos, sin, positions, hq, hkv, d, eps, offset):
     T, dtype, device = qkv.shape[0], qkv.dtype, qkv.device
     q = torch.empty((T, hq, d), device=device, dtype=dtype)
     k = torch.empty((T, hkv, d), device=device, dtype=dtype)
-    v = torch.empty((T, hkv, d), device=device, dtype=dtype)
-    pos, period = (None, positions) if isinstance(positions, int) else (positions.data_ptr(), 0)
-    launch(lib().kgwe_norm_rope_fwd, "norm_rope_fwd", device, qkv.data_ptr(), qkv.stride(0), pos, period,
-           cos.data_ptr(), sin.data_ptr(), ptr(qw), ptr(kw), q.data_ptr(), k.data_ptr(), v.data_ptr(), None, None, None,
-           T, offset, cos.shape[0], hq, hkv, d, 0, 0, eps, HALF_TYPES[dtype])
+    v = torch.empty_like(k)
+    pos, period = (0, positions) if isinstance(positions, int) else (positions.data_ptr(), 0)
+    launch("kgwe_norm_rope_fwd", device, qkv.data_ptr(), pos, cos.data_ptr(), sin.data_ptr(), addr(qw), addr(kw),
+           q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, 0, 0, qkv.stride(0), T, period, offset, cos.shape[0], hq, hkv, d,
+           0, 0, HALF_TYPES[dtype], eps)
     return q, k, v
 
 
@@ -275,10 +275,10 @@ class _NormRopeQKV(torch.autograd.Function):
             blocks = int(lib().kgwe_norm_rope_bwd_blocks(T, hq, hkv, d))
             part = torch.empty((blocks, 2, d), device=dq.device, dtype=torch.float32)
             dqw, dkw = torch.empty_like(qw), torch.empty_like(kw)
-        launch(lib().kgwe_norm_rope_bwd, "norm_rope_bwd", dq.device, ptr(qkv), 0 if qkv is None else qkv.stride(0),
-               ptr(at), period, cos.data_ptr(), sin.data_ptr(), ptr(qw), ptr(kw), dq.data_ptr(), dk.data_ptr(),
-               dv.data_ptr(), dqkv.data_ptr(), ptr(part), ptr(dqw), ptr(dkw), T, offset, cos.shape[0], hq, hkv, d, eps,
-               HALF_TYPES[dq.dtype])
+        launch("kgwe_norm_rope_bwd", dq.device, addr(qkv), addr(at), cos.data_ptr(), sin.data_ptr(), addr(qw), addr(kw),
+               dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dqkv.data_ptr(), addr(part), addr(dqw), addr(dkw),
+               0 if qkv is None else qkv.stride(0), T, period, offset, cos.shape[0], hq, hkv, d, HALF_TYPES[dq.dtype],
+               eps)
         return dqkv, dqw, dkw, None, None, None, None, None, None, None, None
 
 

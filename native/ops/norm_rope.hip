@@ -366,26 +366,56 @@ int bwd(const BwdArgs& a, int D, int grid, unsigned short* dwq, unsigned short* 
 
 }  // namespace
 
-// pos null: row t is at t % period.  wq / wk null: rotation alone.  k / v null: the rotated keys and the values go
+// One record per call (see packed_attn.hip).  pos null: row t is at t % period.
+// wq / wk null: rotation alone.  k / v null: the rotated keys and the values go
 // to the cache only (kc, vc then required).  cache_row null: row t of the cache.
-KGWE_API int kgwe_norm_rope_fwd(const void* qkv, int64_t row_stride, const int* pos, int period, const float* cos_t,
-                                const float* sin_t, const void* wq, const void* wk, void* q, void* k, void* v,
-                                void* kc, void* vc, const int* cache_row, int T, int offset, int table_rows,
-                                int Hq, int Hkv, int D, int Smax, int cache_rows, float eps, int dtype,
-                                hipStream_t s) {
-  if (!shape_ok(T, Hq, Hkv, D, dtype, row_stride) || offset < 0 || table_rows <= 0 || (!pos && period <= 0)) return -1;
-  if ((wq == nullptr) != (wk == nullptr) || (k == nullptr) != (v == nullptr) || (kc == nullptr) != (vc == nullptr) ||
-      (k == nullptr && kc == nullptr) || q == nullptr || (kc != nullptr && (Smax <= 0 || cache_rows <= 0)))
+struct NormRopeFwdCall {
+  const void* qkv;
+  const int* pos;
+  const float *cos_t, *sin_t;
+  const void *wq, *wk;
+  void *q, *k, *v, *kc, *vc;
+  const int* cache_row;
+  int64_t row_stride;
+  int T, period, offset, table_rows, Hq, Hkv, D, Smax, cache_rows, dtype;
+  float eps;
+};
+
+// dq, dk, dv contiguous; dqkv contiguous [T, (Hq + 2 Hkv) D].  With norms also
+// qkv, part [blocks, 2, D] fp32 and dwq, dwk [D] (always both).
+struct NormRopeBwdCall {
+  const void* qkv;
+  const int* pos;
+  const float *cos_t, *sin_t;
+  const void *wq, *wk, *dq, *dk, *dv;
+  void* dqkv;
+  float* part;
+  void *dwq, *dwk;
+  int64_t row_stride;
+  int T, period, offset, table_rows, Hq, Hkv, D, dtype;
+  float eps;
+};
+
+KGWE_API int kgwe_norm_rope_fwd_bytes() { return sizeof(NormRopeFwdCall); }
+KGWE_API int kgwe_norm_rope_bwd_bytes() { return sizeof(NormRopeBwdCall); }
+
+KGWE_API int kgwe_norm_rope_fwd(const NormRopeFwdCall* c, hipStream_t s) {
+  if (!shape_ok(c->T, c->Hq, c->Hkv, c->D, c->dtype, c->row_stride) || c->offset < 0 || c->table_rows <= 0 ||
+      (!c->pos && c->period <= 0))
     return -1;
-  if (!aligned16(qkv) || !aligned16(wq) || !aligned16(wk) || !aligned16(q) || !aligned16(k) || !aligned16(v) ||
-      !aligned16(kc) || !aligned16(vc) || !aligned16(cos_t) || !aligned16(sin_t))
+  if (!c->wq != !c->wk || !c->k != !c->v || !c->kc != !c->vc || (!c->k && !c->kc) || !c->q ||
+      (c->kc && (c->Smax <= 0 || c->cache_rows <= 0)))
+    return -1;
+  if (!aligned16(c->qkv) || !aligned16(c->wq) || !aligned16(c->wk) || !aligned16(c->q) || !aligned16(c->k) ||
+      !aligned16(c->v) || !aligned16(c->kc) || !aligned16(c->vc) || !aligned16(c->cos_t) || !aligned16(c->sin_t))
     return -1;
   using u16 = unsigned short;
-  const FwdArgs a{static_cast<const u16*>(qkv), row_stride, pos, cos_t, sin_t, static_cast<const u16*>(wq),
-                  static_cast<const u16*>(wk), static_cast<u16*>(q), static_cast<u16*>(k), static_cast<u16*>(v),
-                  static_cast<u16*>(kc), static_cast<u16*>(vc), cache_row, T, period, offset, table_rows, Hq, Hkv, Smax,
-                  cache_rows, eps};
-  return dtype == kTypeBf16 ? fwd<Bf16>(a, D, s) : fwd<Fp16>(a, D, s);
+  const FwdArgs a{static_cast<const u16*>(c->qkv), c->row_stride, c->pos, c->cos_t, c->sin_t,
+                  static_cast<const u16*>(c->wq), static_cast<const u16*>(c->wk), static_cast<u16*>(c->q),
+                  static_cast<u16*>(c->k), static_cast<u16*>(c->v), static_cast<u16*>(c->kc),
+                  static_cast<u16*>(c->vc), c->cache_row, c->T, c->period, c->offset, c->table_rows, c->Hq, c->Hkv,
+                  c->Smax, c->cache_rows, c->eps};
+  return c->dtype == kTypeBf16 ? fwd<Bf16>(a, c->D, s) : fwd<Fp16>(a, c->D, s);
 }
 
 // Workgroups of the gradient's launch = rows [2, D] of its fp32 workspace.
@@ -394,22 +424,20 @@ KGWE_API int kgwe_norm_rope_bwd_blocks(int T, int Hq, int Hkv, int D) {
   return grid_for(static_cast<int64_t>(T) * (Hq + 2 * Hkv) * (D / 16), kDwBlocks);
 }
 
-// dq, dk, dv contiguous; dqkv contiguous [T, (Hq + 2 Hkv) D].  With norms also
-// part [blocks, 2, D] fp32 and dwq, dwk [D] (always both).
-KGWE_API int kgwe_norm_rope_bwd(const void* qkv, int64_t row_stride, const int* pos, int period, const float* cos_t,
-                                const float* sin_t, const void* wq, const void* wk, const void* dq, const void* dk,
-                                const void* dv, void* dqkv, float* part, void* dwq, void* dwk, int T, int offset,
-                                int table_rows, int Hq, int Hkv, int D, float eps, int dtype, hipStream_t s) {
-  if (!shape_ok(T, Hq, Hkv, D, dtype, row_stride) || offset < 0 || table_rows <= 0 || (!pos && period <= 0)) return -1;
-  if ((wq == nullptr) != (wk == nullptr) || (wq != nullptr && (!part || !dwq || !dwk || !qkv))) return -1;
-  if (!aligned16(qkv) || !aligned16(wq) || !aligned16(wk) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv) ||
-      !aligned16(dqkv) || !aligned16(cos_t) || !aligned16(sin_t))
+KGWE_API int kgwe_norm_rope_bwd(const NormRopeBwdCall* c, hipStream_t s) {
+  if (!shape_ok(c->T, c->Hq, c->Hkv, c->D, c->dtype, c->row_stride) || c->offset < 0 || c->table_rows <= 0 ||
+      (!c->pos && c->period <= 0))
+    return -1;
+  if (!c->wq != !c->wk || (c->wq && (!c->part || !c->dwq || !c->dwk || !c->qkv))) return -1;
+  if (!aligned16(c->qkv) || !aligned16(c->wq) || !aligned16(c->wk) || !aligned16(c->dq) || !aligned16(c->dk) ||
+      !aligned16(c->dv) || !aligned16(c->dqkv) || !aligned16(c->cos_t) || !aligned16(c->sin_t))
     return -1;
   using u16 = unsigned short;
-  const BwdArgs a{static_cast<const u16*>(qkv), row_stride, pos, cos_t, sin_t, static_cast<const u16*>(wq),
-                  static_cast<const u16*>(wk), static_cast<const u16*>(dq), static_cast<const u16*>(dk),
-                  static_cast<const u16*>(dv), static_cast<u16*>(dqkv), part, T, period, offset, table_rows, Hq, Hkv, eps};
-  const int grid = kgwe_norm_rope_bwd_blocks(T, Hq, Hkv, D);
-  return dtype == kTypeBf16 ? bwd<Bf16>(a, D, grid, static_cast<u16*>(dwq), static_cast<u16*>(dwk), s)
-                            : bwd<Fp16>(a, D, grid, static_cast<u16*>(dwq), static_cast<u16*>(dwk), s);
+  const BwdArgs a{static_cast<const u16*>(c->qkv), c->row_stride, c->pos, c->cos_t, c->sin_t,
+                  static_cast<const u16*>(c->wq), static_cast<const u16*>(c->wk), static_cast<const u16*>(c->dq),
+                  static_cast<const u16*>(c->dk), static_cast<const u16*>(c->dv), static_cast<u16*>(c->dqkv), c->part,
+                  c->T, c->period, c->offset, c->table_rows, c->Hq, c->Hkv, c->eps};
+  const int grid = kgwe_norm_rope_bwd_blocks(c->T, c->Hq, c->Hkv, c->D);
+  u16 *dwq = static_cast<u16*>(c->dwq), *dwk = static_cast<u16*>(c->dwk);
+  return c->dtype == kTypeBf16 ? bwd<Bf16>(a, c->D, grid, dwq, dwk, s) : bwd<Fp16>(a, c->D, grid, dwq, dwk, s);
 }

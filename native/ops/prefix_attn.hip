@@ -429,24 +429,38 @@ KGWE_API int64_t kgwe_prefix_attn_workspace(int B, int Hq, int Hkv, int D, int P
   return p.direct || slots == 1 ? 0 : static_cast<int64_t>(B) * Hq * slots * (D + 2);
 }
 
-// q, out contiguous [B, Hq, D]; prefix [Hkv, P, D] by strides (elements, both
-// tensors alike); caches contiguous [B, Hkv, Smax, D]; lens int32 [B], cut to
-// [0, Smax].  The workspace needs no clearing and is the call's own.
-KGWE_API int kgwe_prefix_attn(const void* q, const void* pk, const void* pv, int64_t p_row, int64_t p_head,
-                              const void* kc, const void* vc, const int* lens, float* work, void* out, int B, int Hq,
-                              int Hkv, int D, int P, int Smax, float scale, int dtype, hipStream_t s) {
-  if (!shape_ok(B, Hq, Hkv, D, P, Smax) || (dtype != kTypeBf16 && dtype != kTypeFp16)) return -1;
-  if (P > 0 && (!pk || !pv || !aligned16(pk) || !aligned16(pv) || p_row % 8 || p_head % 8 || p_row < D ||
-                p_row > (1 << 22) || p_head < 0))
+// One record per call (see packed_attn.hip).  q, out contiguous [B, Hq, D];
+// prefix [Hkv, P, D] by strides (elements, both tensors alike); caches
+// contiguous [B, Hkv, Smax, D]; lens int32 [B], cut to [0, Smax].  The
+// workspace needs no clearing and is the call's own.
+struct PrefixCall {
+  const void *q, *pk, *pv, *kc, *vc;
+  const int* lens;
+  float* work;
+  void* out;
+  int64_t p_row, p_head;
+  int B, Hq, Hkv, D, P, Smax, dtype;
+  float scale;
+};
+
+KGWE_API int kgwe_prefix_attn_bytes() { return sizeof(PrefixCall); }
+
+KGWE_API int kgwe_prefix_attn(const PrefixCall* c, hipStream_t s) {
+  const int B = c->B, Hq = c->Hq, Hkv = c->Hkv, D = c->D, P = c->P, Smax = c->Smax;
+  if (!shape_ok(B, Hq, Hkv, D, P, Smax) || (c->dtype != kTypeBf16 && c->dtype != kTypeFp16)) return -1;
+  if (P > 0 && (!c->pk || !c->pv || !aligned16(c->pk) || !aligned16(c->pv) || c->p_row % 8 || c->p_head % 8 ||
+                c->p_row < D || c->p_row > (1 << 22) || c->p_head < 0))
     return -1;
-  if (!aligned16(q) || !aligned16(out) || !aligned16(kc) || !aligned16(vc) || !aligned16(work)) return -1;
+  if (!aligned16(c->q) || !aligned16(c->out) || !aligned16(c->kc) || !aligned16(c->vc) || !aligned16(c->work))
+    return -1;
   const Plan p = make_plan(B, Hq, Hkv, P, Smax);
   const int slots = p.p_splits + p.o_splits;
-  if (!p.direct && slots > 1 && !work) return -2;
-  float* ml = work + static_cast<int64_t>(B) * Hq * slots * D;
-  const Args a{static_cast<const u16*>(q), static_cast<const u16*>(pk), static_cast<const u16*>(pv), p_row, p_head,
-               static_cast<const u16*>(kc), static_cast<const u16*>(vc), lens, static_cast<u16*>(out), work, ml, B,
-               Hq, Hkv, P, Smax, p.p_chunk, p.p_splits, p.o_chunk, p.o_splits, p.direct, scale * kLog2e};
-  if (dtype == kTypeBf16) return D == 64 ? launch<Bf16, 64>(a, s) : launch<Bf16, 128>(a, s);
+  if (!p.direct && slots > 1 && !c->work) return -2;
+  float* ml = c->work + static_cast<int64_t>(B) * Hq * slots * D;
+  const Args a{static_cast<const u16*>(c->q), static_cast<const u16*>(c->pk), static_cast<const u16*>(c->pv),
+               c->p_row, c->p_head, static_cast<const u16*>(c->kc), static_cast<const u16*>(c->vc), c->lens,
+               static_cast<u16*>(c->out), c->work, ml, B, Hq, Hkv, P, Smax, p.p_chunk, p.p_splits, p.o_chunk,
+               p.o_splits, p.direct, c->scale * kLog2e};
+  if (c->dtype == kTypeBf16) return D == 64 ? launch<Bf16, 64>(a, s) : launch<Bf16, 128>(a, s);
   return D == 64 ? launch<Fp16, 64>(a, s) : launch<Fp16, 128>(a, s);
 }
