@@ -115,7 +115,8 @@ __device__ __forceinline__ buf_t row_buffer(const void* p, int rows, int row_byt
 }
 
 // BYTES (4 or 16) per lane from src + offset to consecutive LDS from dst on
-// (wave-uniform); zeros where the offset is past the descriptor's extent.
+// (wave-uniform); zeros where the offset is past the descriptor's extent.  (The
+// instruction's immediate offset would move the LDS address along.)
 template <int BYTES>
 __device__ __forceinline__ void dma_lane(buf_t src, int offset, void* dst) {
 #ifdef __HIP_DEVICE_COMPILE__
@@ -126,26 +127,33 @@ __device__ __forceinline__ void dma_lane(buf_t src, int offset, void* dst) {
 #endif
 }
 
-// One wave's share (of W) of a tile of ROWS rows: kN instructions.
+// One wave's share (of W) of a tile of ROWS rows: kN instructions, each of 1024
+// bytes of the image = 8 rows x 64 columns, 8 rows further on every one (D =
+// 64) or two (D = 128).  The swizzle of a chunk depends on the parity of its
+// row group alone, so two lane offsets serve all of them.
 template <int D, int ROWS, int W = 4>
 struct TileDma {
   static constexpr int kBytes = ROWS * D * 2;
   static constexpr int kN = kBytes / 1024 / W;
-  static_assert(kN >= 1 && kBytes % (1024 * W) == 0, "tile divides evenly over the waves");
-  int row[kN], chunk[kN];
+  static constexpr int kPer = D / 64;  // instructions per row group
+  static_assert(kN >= kPer && kN % kPer == 0 && kBytes % (1024 * W) == 0, "whole row groups per wave");
+  int row, chunk[2];
   int first;  // wave-uniform byte offset of the wave's share
   __device__ __forceinline__ TileDma(int wave, int lane) : first(wave * kN * 1024) {
+    const int group = wave * (kN / kPer), r7 = (lane >> 2) & 7;
+    row = 8 * group + r7;
 #pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      const int n = wave * kN + i;
-      const int sub = D == 128 ? 2 * (n & 1) + (lane >> 5) : lane >> 5;
-      row[i] = 8 * (D == 128 ? n >> 1 : n) + ((lane >> 2) & 7);
-      chunk[i] = 16 * (4 * sub + ((lane & 3) ^ ((row[i] >> 2) & 3)));
-    }
+    for (int p = 0; p < 2; ++p)
+      chunk[p] = 64 * (lane >> 5) + 16 * ((lane & 3) ^ ((2 * (group + p) + (r7 >> 2)) & 3));
   }
   __device__ __forceinline__ void load(buf_t src, int row_bytes, char* img) const {
+    const int at = row * row_bytes;
 #pragma unroll
-    for (int i = 0; i < kN; ++i) dma_lane<16>(src, row[i] * row_bytes + chunk[i], img + first + 1024 * i);
+    for (int g = 0; g < kN / kPer; ++g) {
+      const int off = at + 8 * g * row_bytes + chunk[g & 1];
+      dma_lane<16>(src, off, img + first + 1024 * kPer * g);
+      if constexpr (kPer == 2) dma_lane<16>(src, off + 128, img + first + 1024 * kPer * g + 1024);
+    }
   }
 };
 
@@ -154,6 +162,16 @@ __device__ __forceinline__ void dma_join() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
 }
+
+// Division by a host-known divisor: n / d for n * d < 2^32 by one multiply
+// (an integer division is some 20 instructions, which count in short kernels).
+struct Div {
+  unsigned mul;  // ceil(2^32 / d); 0 for d = 1
+  __host__ explicit Div(int d = 1) : mul(d == 1 ? 0u : static_cast<unsigned>(0xffffffffu / d + 1)) {}
+  __device__ __forceinline__ int operator()(int n) const {
+    return mul == 0 ? n : static_cast<int>(__umulhi(static_cast<unsigned>(n), mul));
+  }
+};
 
 // Store one row of transposed accumulators (acc[db] register r holds column
 // 32 db + tile_row(r, hh) of this lane's row) times `mul` with 16-byte stores:

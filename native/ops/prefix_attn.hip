@@ -38,8 +38,10 @@ struct Args {
   const int* lens;
   u16* out;            // [B, Hq, D]
   float *part_o, *part_ml;  // [B * Hq, slots, D], [B * Hq, slots, 2]
-  int B, Hq, Hkv, P, Smax;
+  int B, Hq, Hkv, G, P, Smax;
+  Div by_g, by_hkv;
   int p_chunk, p_splits, o_chunk, o_splits;  // splits 0: no workgroups of that kind
+  int o_wgs;           // workgroups that share the own chunks
   int direct;          // one workgroup walks prefix and own keys and writes out
   float c;
 };
@@ -109,70 +111,53 @@ struct Walk {
   int n0, n1, row0, row1;
 };
 
-template <class T, int D>
+// WIDE: more than 32 rows a key head. (Two kernels: with both forms of the
+// prefix walk in one, scalar registers spill and the short cases lose 15 %.)
+template <class T, int D, bool WIDE>
 __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(Args a) {
   constexpr int NB = D / 32, NT = D / 16;
   constexpr int kImg = kWide * D * 2;  // = two waves' slim tiles
+  // The shared tiles of the wide form; of the slim form wave w's K and V halves of piece w.
   __shared__ __attribute__((aligned(1024))) char K0[kImg], V0[kImg], K1[kImg], V1[kImg];
   __shared__ float ml[4][32][2], joined[32][2];  // (max, sum) of each wave's rows; of all four
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lq = lane & 31, hh = lane >> 5;
-  const int G = a.Hq / a.Hkv, rows_all = a.B * G, slots = a.p_splits + a.o_splits;
-  const bool wide = !a.direct && rows_all > 32;
-  const int tiles = wide ? (rows_all + 127) / 128 : 1;
+  const int G = a.G, rows_all = a.B * G, slots = a.p_splits + a.o_splits;
+  const bool direct = !WIDE && a.direct;
+  const int tiles = WIDE ? (rows_all + 127) / 128 : 1;
   const TileAddr<D> ad(lane);
 
+  const bool final = direct || slots == 1;
   // ---- which work: chunk of the prefix (all row tiles of one chunk on one XCD), or of a sequence's own keys
   const int units = a.p_splits * a.Hkv;
   const int prefix_wgs = (units + 7) / 8 * 8 * tiles;
   int i = blockIdx.x;
-  int slot, kvh, nrows, first_row = 0, b = 0;  // first_row: of the rows b * G + g
+  const bool prefix_job = !direct && i < prefix_wgs;
+  int slot = 0, kvh = 0, nrows = G, first_row = 0;  // first_row: of the rows b * G + g
   Walk wk{};
   wk.row0 = static_cast<int>(2 * a.p_row);
   wk.row1 = 2 * D;
-  if (!a.direct && i < prefix_wgs) {
-    const int base = i / (8 * tiles), rem = i - base * 8 * tiles;
+  if (prefix_job) {
+    const int base = tiles == 1 ? i / 8 : i / (8 * tiles), rem = i - base * 8 * tiles;
     const int unit = base * 8 + rem % 8;
     if (unit >= units) return;
-    slot = unit / a.Hkv;
+    slot = a.by_hkv(unit);
     kvh = unit - slot * a.Hkv;
     first_row = rem / 8 * 128;
-    nrows = min(rows_all - first_row, wide ? 128 : 32);
+    nrows = min(rows_all - first_row, WIDE ? 128 : 32);
     const int64_t at = kvh * a.p_head + static_cast<int64_t>(slot) * a.p_chunk * a.p_row;
     wk.k0 = a.pk + at;
     wk.v0 = a.pv + at;
     wk.n0 = min(a.p_chunk, a.P - slot * a.p_chunk);
-  } else {
-    if (!a.direct) i -= prefix_wgs;
-    const int per = a.direct ? 1 : a.o_splits;
-    const int split = i % per;
-    kvh = i / per % a.Hkv;
-    b = i / per / a.Hkv;
-    first_row = b * G;
-    nrows = G;
-    slot = a.direct ? 0 : a.p_splits + split;
-    const int len = min(max(a.lens[b], 0), a.Smax);
-    const int start = a.direct ? 0 : split * a.o_chunk;
-    wk.n1 = __builtin_amdgcn_readfirstlane(a.direct ? len : min(a.o_chunk, len - start));
-    if (!a.direct && wk.n1 <= 0 && slots > 1) return;
-    wk.n1 = max(wk.n1, 0);
-    const int64_t at = ((static_cast<int64_t>(b) * a.Hkv + kvh) * a.Smax + start) * D;
-    wk.k1 = a.kc + at;
-    wk.v1 = a.vc + at;
-    if (a.direct) {
-      wk.k0 = a.pk + kvh * a.p_head;
-      wk.v0 = a.pv + kvh * a.p_head;
-      wk.n0 = a.P;
-    }
+  } else if (!direct) {
+    i -= prefix_wgs;
   }
-  const bool final = a.direct || slots == 1;
 
   bf16x8 qf[NT];
-  State<T, D> st;
-
-  if (wide && wk.n0 > 0) {
+  if (WIDE && prefix_job) {
+    State<T, D> st;
     // 128 rows, 32 per wave, on tiles of 64 keys that the waves share.
-    const int r = first_row + 32 * w + lq, rb = r / G;
+    const int r = first_row + 32 * w + lq, rb = a.by_g(r);
     const bool ok = 32 * w + lq < nrows;
     const int64_t qi = static_cast<int64_t>(rb) * a.Hq + kvh * G + (r - rb * G);
     load_q<T, D>(a.q + qi * D, ok, hh, qf);
@@ -236,25 +221,80 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(Args a) {
   // At most 32 rows: every wave walks tiles of its own (tile index = wave mod
   // 4) with its own K and V buffer and no barrier: the next K tile is on its
   // way from the S product on, the next V tile from the O product on.
+  const TileDma<D, kSlim, 1> dma(0, lane);
+  for (;; i += a.o_wgs) {
+  State<T, D> st;
+  if (WIDE || !prefix_job) {
+    // The i-th (chunk of a sequence's own keys, key head): the chunks that hold
+    // keys, counted by every wave from lens, 64 sequences at a time.
+    int b, len, start = 0;
+    if (direct) {
+      b = a.by_hkv(i);
+      kvh = i - b * a.Hkv;
+      len = min(max(a.lens[b], 0), a.Smax);
+    } else {
+      int left = a.by_hkv(i), b0 = 0;
+      kvh = i - left * a.Hkv;
+      for (;; b0 += 64) {
+        if (b0 >= a.B) return;  // every chunk is taken
+        const int n = b0 + lane < a.B ? min(max(a.lens[b0 + lane], 0), a.Smax) : 0;
+        // where nothing is joined an empty row's zeros have to be written, too
+        const int chunks = final ? (b0 + lane < a.B ? 1 : 0) : (n + a.o_chunk - 1) / a.o_chunk;
+        int upto = chunks;
+#pragma unroll
+        for (int off = 1; off < kWave; off <<= 1) {
+          const int y = __shfl_up(upto, off, kWave);
+          if (lane >= off) upto += y;
+        }
+        const unsigned long long past = __ballot(upto > left);
+        if (past != 0) {
+          const int f = __builtin_ctzll(past);
+          b = b0 + f;
+          len = __shfl(n, f, kWave);
+          start = left - __shfl(upto - chunks, f, kWave);
+          break;
+        }
+        left -= __shfl(upto, 63, kWave);
+      }
+      slot = a.p_splits + start;
+      start *= a.o_chunk;
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    slot = __builtin_amdgcn_readfirstlane(slot);
+    start = __builtin_amdgcn_readfirstlane(start);
+    first_row = b * G;
+    wk.n1 = __builtin_amdgcn_readfirstlane(direct ? len : min(a.o_chunk, len - start));
+    const int64_t at = ((static_cast<int64_t>(b) * a.Hkv + kvh) * a.Smax + start) * D;
+    wk.k1 = a.kc + at;
+    wk.v1 = a.vc + at;
+    if (direct) {
+      wk.k0 = a.pk + kvh * a.p_head;
+      wk.v0 = a.pv + kvh * a.p_head;
+      wk.n0 = a.P;
+    }
+  }
   {
-    const int r = first_row + lq, rb = r / G;
+    const int r = first_row + lq, rb = a.by_g(r);
     const int64_t qi = static_cast<int64_t>(rb) * a.Hq + kvh * G + (r - rb * G);
     load_q<T, D>(a.q + qi * D, lq < nrows, hh, qf);
   }
-  const TileDma<D, kSlim, 1> dma(0, lane);
-  const int t0 = (wk.n0 + kSlim - 1) / kSlim, nt = t0 + (wk.n1 + kSlim - 1) / kSlim;
+  const int t0 = WIDE ? 0 : (wk.n0 + kSlim - 1) / kSlim, nt = t0 + (wk.n1 + kSlim - 1) / kSlim;
   auto load = [&](bool keys, char* dst, int t) {
-    const bool own = t >= t0;
+    const bool own = WIDE || t >= t0;
     const int at = (own ? t - t0 : t) * kSlim, rows = min(kSlim, (own ? wk.n1 : wk.n0) - at);
     const int row = own ? wk.row1 : wk.row0;
     const u16* base = own ? (keys ? wk.k1 : wk.v1) : (keys ? wk.k0 : wk.v0);
     dma.load(row_buffer(base + static_cast<int64_t>(at) * (row / 2), rows, row), row, dst);
   };
   constexpr int kDma = TileDma<D, kSlim, 1>::kN;
-  auto walk = [&](char* Kb, char* Vb) {
-    if (w >= nt) return;
+  char* const piece_w = w == 0 ? K0 : w == 1 ? V0 : w == 2 ? K1 : V1;
+  char* const Kb = piece_w;
+  char* const Vb = Kb + kImg / 2;
+  if (w < nt) {
     load(true, Kb, w);
     load(false, Vb, w);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) asm volatile("" ::"v"(qf[t]));  // Q has landed before the loop (see packed_attn.hip)
     for (int t = w; t < nt; t += 4) {
       const bool more = t + 4 < nt;
       f32x16 s[1];
@@ -265,7 +305,7 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(Args a) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read: its buffer is free
       if (more) load(true, Kb, t + 4);
       u32x4 pb[2];
-      st.template soften<1>(s, t >= t0 ? wk.n1 - (t - t0) * kSlim : wk.n0 - t * kSlim, a.c, hh, pb);
+      st.template soften<1>(s, WIDE || t >= t0 ? wk.n1 - (t - t0) * kSlim : wk.n0 - t * kSlim, a.c, hh, pb);
       if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kDma) : "memory");  // V has landed, the next K may be on its way
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
@@ -275,10 +315,7 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(Args a) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       if (more) load(false, Vb, t + 4);
     }
-  };
-  // Each wave pair in an LDS object of its own, known at compile time.
-  if (w < 2) walk(K0 + (w & 1) * (kImg / 2), V0 + (w & 1) * (kImg / 2));
-  else walk(K1 + (w & 1) * (kImg / 2), V1 + (w & 1) * (kImg / 2));
+  }
 
   // Join the four waves through LDS: a common max, then the scaled outputs.
   const float lw = half_add(st.l);
@@ -297,7 +334,7 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(Args a) {
     // Row lq of this wave's [32][D] fp32 region, its 16-byte pieces XOR-swizzled
     // by the row (rows are a multiple of all banks apart).
     constexpr int kPieces = D / 4;
-    char* reg = w == 0 ? K0 : w == 1 ? V0 : w == 2 ? K1 : V1;
+    char* reg = piece_w;
     const float mul = exp2_fast(st.m - M_use);
     if (lq < nrows) {
 #pragma unroll
@@ -321,7 +358,7 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(Args a) {
       const int off = row * D * 4 + 16 * (piece ^ (row & (kPieces - 1)));
       const f32x4 v = (*reinterpret_cast<const f32x4*>(K0 + off) + *reinterpret_cast<const f32x4*>(V0 + off)) +
                       (*reinterpret_cast<const f32x4*>(K1 + off) + *reinterpret_cast<const f32x4*>(V1 + off));
-      const int rr = first_row + row, rb = rr / G;
+      const int rr = first_row + row, rb = a.by_g(rr);
       const int64_t qi = static_cast<int64_t>(rb) * a.Hq + kvh * G + (rr - rb * G);
       const float Lr = joined[row][1];
       if (final) {
@@ -339,61 +376,123 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(Args a) {
       }
     }
   }
+  if (!WIDE && (prefix_job || direct)) return;
+  __syncthreads();  // the tile buffers are read before the next chunk fills them
+  }
 }
 
-// Join the slots of one (b, h) per wave: the prefix's, then those of the own
-// chunks that hold keys.
-template <class T, int D>
+// Join the slots of one (b, h): the prefix's, then those of the own chunks that
+// hold keys.  W waves share a row; wave w of them takes every W-th slot, lane i
+// of it the (max, sum) of the i-th of those.  Few rows have many slots and want
+// 4 waves each (1 row x 32 heads, 66 slots: 21.2 -> 16.5 us with the launch
+// before it), many rows one (32 x 32 heads, 12 slots: 12.2 -> 10.7 us).  The first loads of a wave are issued before
+// anything is known of n: what lies past it is the workspace's own memory, and
+// is dropped by selection.
+template <class T, int D, int W>
 __global__ __launch_bounds__(256) void prefix_join_kernel(Args a) {
   constexpr int E = D / 64;  // outputs per lane
-  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-  if (row >= a.B * a.Hq) return;
-  const int b = row / a.Hq, slots = a.p_splits + a.o_splits;
-  const int len = min(max(a.lens[b], 0), a.Smax);
-  const int n = a.p_splits + (a.o_splits > 0 ? (len + a.o_chunk - 1) / a.o_chunk : 0);
-  const float* ml = a.part_ml + static_cast<int64_t>(row) * slots * 2;
+  const int lane = threadIdx.x & 63, w = (threadIdx.x >> 6) % W;
+  const int row = blockIdx.x * (4 / W) + (threadIdx.x >> 6) / W;
+  if (row >= a.B * a.Hq) return;  // W = 4: never
+  const int slots = a.p_splits + a.o_splits;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + static_cast<int64_t>(row) * slots;
   const float* po = a.part_o + static_cast<int64_t>(row) * slots * D + E * lane;
-  float M = -INFINITY;
-  for (int s = lane; s < n; s += 64) M = fmaxf(M, ml[2 * s]);
-  M = wave_max(M);
-  if (M == -INFINITY) M = 0.f;
-  float L = 0.f, o[E];
+  const int len = min(max(a.lens[row / a.Hq], 0), a.Smax);
+  const int n = a.p_splits + (a.o_splits > 0 ? (len + a.o_chunk - 1) / a.o_chunk : 0);
+  float M = -INFINITY, L = 0.f, o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-#pragma unroll 8
-  for (int s = 0; s < n; ++s) {
-    const float f = exp2_fast(ml[2 * s] - M);
-    L += f * ml[2 * s + 1];
+  for (int s0 = w; s0 < slots; s0 += 64 * W) {  // up to 64 slots of this wave
+    const int mine = s0 + W * lane;
+    const float2 x = mine < slots ? ml[mine] : float2{-INFINITY, 0.f};
+    const bool used = mine < n;
+    const float M2 = fmaxf(M, wave_max(used ? x.x : -INFINITY));
+    const float M_use = M2 == -INFINITY ? 0.f : M2;
+    const float f = used ? exp2_fast(x.x - M_use) : 0.f, keep = exp2_fast(M - M_use);
+    L = L * keep + wave_sum(used ? f * x.y : 0.f);
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] += f * po[static_cast<int64_t>(s) * D + e];
+    for (int e = 0; e < E; ++e) o[e] *= keep;
+    M = M2;
+    const int some = min(64, (slots - s0 + W - 1) / W);
+    for (int j0 = 0; j0 < some; j0 += 8) {
+      float v[8][E];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[j][e] = po[static_cast<int64_t>(s0 + W * min(j0 + j, some - 1)) * D + e];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float fj = __shfl(f, min(j0 + j, 63), kWave);
+        const bool use = j0 + j < some && s0 + W * (j0 + j) < n;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += use ? fj * v[j][e] : 0.f;
+      }
+    }
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
+  if constexpr (W == 1) {
+    const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
-  for (int e = 0; e < E; ++e) a.out[static_cast<int64_t>(row) * D + E * lane + e] = T::down(o[e] * inv);
+    for (int e = 0; e < E; ++e) a.out[static_cast<int64_t>(row) * D + E * lane + e] = T::down(o[e] * inv);
+    return;
+  }
+  __shared__ float wave_ml[4][2], wave_o[4][D];
+  if (lane == 0) {
+    wave_ml[w][0] = M;
+    wave_ml[w][1] = L;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) wave_o[w][E * lane + e] = o[e];
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  float M4 = -INFINITY, L4 = 0.f, y = 0.f;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) M4 = fmaxf(M4, wave_ml[v][0]);
+  if (M4 == -INFINITY) M4 = 0.f;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    const float f = exp2_fast(wave_ml[v][0] - M4);
+    L4 += f * wave_ml[v][1];
+    y += f * wave_o[v][threadIdx.x];
+  }
+  a.out[static_cast<int64_t>(row) * D + threadIdx.x] = T::down(L4 == 0.f ? 0.f : y / L4);
 }
 
-// Chunks.  Numbers of workgroups are per (key head, row tile) or (key head,
-// sequence); the chip holds 512 of them (2 per CU).
+// Chunks, for 256 CUs that hold two workgroups each.
+//
+// Prefix: 256 workgroups in all where its length allows (one per CU; the other
+// half of each CU walks own keys meanwhile).  Every chunk leaves a state of
+// (D + 2) floats per row to write and to join: 512 chunks-times-tiles instead
+// of 256 read 53.9 -> 61.1 us at 64 rows x 32,768 keys (32 / 8 heads x 128) and
+// 25.8 -> 33.9 us at 60 x 20,000 (8 / 8 heads); 128 leave half the chip idle
+// (83 us).  A chunk has at least 256 keys (128: 10.5 -> 11.2 us at 32 x 2,048,
+// 32 / 8 heads x 64), 384 for a wave's own tiles (1 x 8,192, 32 / 8 heads x
+// 128: 11.4 us against 12.7 with 256 and 15.8 with 128).
+//
+// Own keys: chunks of 256 that 512 workgroups share out among them by counting
+// (a workgroup for every possible chunk, most of them empty, cost 8 us more at
+// 64 rows of 2,048).
+//
+// One workgroup per (sequence, key head), no join: while prefix and cache hold
+// at most 1,024 keys and the workgroups fit the chip at once (48 rows, 16 / 2
+// heads x 128, 500 + 300 keys: 9.9 against 13.2 us; at 4 rows of 1,000 + 500
+// the split form is the faster, 8.9 against 10.6), else 512 keys.
 struct Plan {
-  int direct, p_chunk, p_splits, o_chunk, o_splits;
+  int direct, p_chunk, p_splits, o_chunk, o_splits, o_wgs;
 };
 
 Plan make_plan(int B, int Hq, int Hkv, int P, int Smax) {
   Plan p{};
   const int rows = B * (Hq / Hkv), tiles = rows > 32 ? (rows + 127) / 128 : 1;
-  p.direct = P + Smax <= 512;
+  p.direct = P + Smax <= (B * Hkv <= 512 ? 1024 : 512);
   if (p.direct) return p;
-  auto split = [](int64_t n, int units, int least, int* chunk, int* splits) {
-    *splits = 0;
-    *chunk = least;
-    if (n <= 0) return;
-    const int64_t want = std::max<int64_t>(1, 512 / units);
-    const int64_t c = std::max<int64_t>(least, ((n + want - 1) / want + 63) / 64 * 64);
-    *chunk = static_cast<int>(c);
-    *splits = static_cast<int>((n + c - 1) / c);
-  };
-  split(P, Hkv * tiles, rows > 32 ? 256 : 128, &p.p_chunk, &p.p_splits);
-  split(Smax, B * Hkv, 256, &p.o_chunk, &p.o_splits);
+  if (P > 0) {
+    const int64_t want = std::max(1, 256 / (Hkv * tiles));
+    p.p_chunk = static_cast<int>(std::max<int64_t>(rows > 32 ? 256 : 384, ((P + want - 1) / want + 63) / 64 * 64));
+    p.p_splits = (P + p.p_chunk - 1) / p.p_chunk;
+  }
+  p.o_chunk = 256;
+  p.o_splits = (Smax + p.o_chunk - 1) / p.o_chunk;
+  p.o_wgs = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(B) * Hkv * p.o_splits, 512));
   return p;
 }
 
@@ -403,20 +502,24 @@ template <class T, int D>
 int launch(Args a, hipStream_t s) {
   const int G = a.Hq / a.Hkv, rows = a.B * G, tiles = !a.direct && rows > 32 ? (rows + 127) / 128 : 1;
   const int64_t grid = a.direct ? static_cast<int64_t>(a.B) * a.Hkv
-                                : static_cast<int64_t>((a.p_splits * a.Hkv + 7) / 8 * 8) * tiles +
-                                      static_cast<int64_t>(a.B) * a.Hkv * a.o_splits;
+                                : static_cast<int64_t>((a.p_splits * a.Hkv + 7) / 8 * 8) * tiles + a.o_wgs;
   if (grid <= 0 || grid > 0x7fffffff) return -1;
-  hipLaunchKernelGGL((prefix_attn_kernel<T, D>), dim3(static_cast<unsigned>(grid)), dim3(256), 0, s, a);
+  if (!a.direct && rows > 32)
+    hipLaunchKernelGGL((prefix_attn_kernel<T, D, true>), dim3(static_cast<unsigned>(grid)), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((prefix_attn_kernel<T, D, false>), dim3(static_cast<unsigned>(grid)), dim3(256), 0, s, a);
   int rc = KGWE_CHECK_LAUNCH();
   if (rc || a.direct || a.p_splits + a.o_splits == 1) return rc;
-  hipLaunchKernelGGL((prefix_join_kernel<T, D>), dim3((a.B * a.Hq + 3) / 4), dim3(256), 0, s, a);
+  const int n = a.B * a.Hq;
+  if (n <= 256) hipLaunchKernelGGL((prefix_join_kernel<T, D, 4>), dim3(n), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((prefix_join_kernel<T, D, 1>), dim3((n + 3) / 4), dim3(256), 0, s, a);
   return KGWE_CHECK_LAUNCH();
 }
 
 inline bool shape_ok(int B, int Hq, int Hkv, int D, int P, int Smax) {
   return B > 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= 32 && (D == 64 || D == 128) && P >= 0 &&
          Smax >= 0 && P + static_cast<int64_t>(Smax) > 0 && P < (1 << 30) && Smax < (1 << 30) &&
-         static_cast<int64_t>(B) * Hq < (1 << 24);
+         static_cast<int64_t>(B) * Hq < (1 << 24) && Hkv <= 1024;
 }
 
 }  // namespace
@@ -459,8 +562,9 @@ KGWE_API int kgwe_prefix_attn(const PrefixCall* c, hipStream_t s) {
   float* ml = c->work + static_cast<int64_t>(B) * Hq * slots * D;
   const Args a{static_cast<const u16*>(c->q), static_cast<const u16*>(c->pk), static_cast<const u16*>(c->pv),
                c->p_row, c->p_head, static_cast<const u16*>(c->kc), static_cast<const u16*>(c->vc), c->lens,
-               static_cast<u16*>(c->out), c->work, ml, B, Hq, Hkv, P, Smax, p.p_chunk, p.p_splits, p.o_chunk,
-               p.o_splits, p.direct, c->scale * kLog2e};
+               static_cast<u16*>(c->out), c->work, ml, B, Hq, Hkv, Hq / Hkv, P, Smax, Div(Hq / Hkv), Div(Hkv),
+               p.p_chunk, p.p_splits, p.o_chunk,
+               p.o_splits, p.o_wgs, p.direct, c->scale * kLog2e};
   if (c->dtype == kTypeBf16) return D == 64 ? launch<Bf16, 64>(a, s) : launch<Bf16, 128>(a, s);
   return D == 64 ? launch<Fp16, 64>(a, s) : launch<Fp16, 128>(a, s);
 }
