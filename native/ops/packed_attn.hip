@@ -38,7 +38,8 @@ struct View {
 
 struct Batch {
   const int4* jobs;
-  int T, Hq, Hkv;
+  int T, Hq, Hkv, G;
+  Div by_hq, by_hkv, by_g;
 };
 
 // A workgroup's block of a sequence: `rows` rows from `row0` on, of which it
@@ -50,8 +51,8 @@ struct Job {
 // Job and head of this workgroup: all heads of a job are neighbours, and on
 // Hq % 8 == 0 each of the 8 XCDs (workgroups go round them) takes a contiguous
 // run of heads, so the heads that share keys share an L2.
-__device__ __forceinline__ bool pick(const Batch& b, int heads, Job* job, int* head) {
-  const int j = blockIdx.x / heads, p = blockIdx.x - j * heads;
+__device__ __forceinline__ bool pick(const Batch& b, int heads, Div by_heads, Job* job, int* head) {
+  const int j = by_heads(blockIdx.x), p = blockIdx.x - j * heads;
   *head = heads % 8 == 0 ? (p % 8) * (heads / 8) + p / 8 : p;
   const int4 v = b.jobs[j];
   job->row0 = __builtin_amdgcn_readfirstlane(v.x);
@@ -59,6 +60,20 @@ __device__ __forceinline__ bool pick(const Batch& b, int heads, Job* job, int* h
   job->blk = __builtin_amdgcn_readfirstlane(v.z);
   job->keys = __builtin_amdgcn_readfirstlane(v.w);
   return job->rows > 0;
+}
+
+// A block of few rows (a short sequence, or the end of one) would keep one or
+// two of the workgroup's four waves busy, and always the same ones.  Where the
+// group has the heads for it, 4 heads share a workgroup at 32 rows or less and
+// 2 at 64 or less; the workgroups of the other heads leave.  Moves *head to
+// this wave's head; returns the wave's first row in the sequence, -1: leave.
+__device__ __forceinline__ int wave_rows(const Batch& b, const Job& job, int wave, int* head) {
+  const int here = job.rows - job.blk * kRows;
+  const int share = here <= 32 && b.G % 4 == 0 ? 2 : here <= 64 && b.G % 2 == 0 ? 1 : 0;  // log2
+  if (*head & ((1 << share) - 1)) return -1;
+  const int per = 2 - share;  // log2 of the waves per head
+  *head += wave >> per;
+  return job.blk * kRows + 32 * (wave & ((1 << per) - 1));
 }
 
 // Running max kept until a tile's max passes it by this much (log2 units), so
@@ -84,14 +99,16 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(FwdArgs a) {
   __shared__ __attribute__((aligned(1024))) char K0[kImg], V0[kImg], K1[kImg], V1[kImg];
   Job job;
   int h;
-  if (!pick(a.b, a.b.Hq, &job, &h)) return;
-  const int hkv = h / (a.b.Hq / a.b.Hkv);
+  if (!pick(a.b, a.b.Hq, a.b.by_hq, &job, &h)) return;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hkv = a.b.by_g(h), q0 = wave_rows(a.b, job, w, &h);
+  if (q0 < 0) return;
   const int row0 = job.row0, len = job.rows, blk = job.blk;
   const int klen = job.keys;  // padding rows see nothing
   const int plen = PREFIX && klen > 0 ? a.P : 0;
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
   const int lq = lane & 31, hh = lane >> 5;
-  const int q0 = blk * kRows + w * 32, qrow = q0 + lq;
+  const int qrow = q0 + lq;
   const bool mine = q0 < len;  // wave-uniform: this wave has rows
 
   bf16x8 qf[NT];
@@ -242,12 +259,14 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(BwdArgs a) {
   __shared__ __attribute__((aligned(1024))) char K0[kImg], V0[kImg], K1[kImg], V1[kImg];
   Job job;
   int h;
-  if (!pick(a.b, a.b.Hq, &job, &h)) return;
-  const int hkv = h / (a.b.Hq / a.b.Hkv);
+  if (!pick(a.b, a.b.Hq, a.b.by_hq, &job, &h)) return;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int hkv = a.b.by_g(h), q0 = wave_rows(a.b, job, w, &h);
+  if (q0 < 0) return;
   const int row0 = job.row0, len = job.rows, blk = job.blk, klen = job.keys;
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
   const int lq = lane & 31, hh = lane >> 5;
-  const int q0 = blk * kRows + w * 32, qrow = q0 + lq;
+  const int qrow = q0 + lq;
   const bool mine = q0 < len;
   const bool ok = qrow < len;
   const int64_t row = static_cast<int64_t>(row0) + qrow;
@@ -356,8 +375,8 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(BwdArgs a) {
   __shared__ __attribute__((aligned(256))) float L0[64], L1[64];  // lse and -D of a tile's 32 rows
   Job job;
   int hkv;
-  if (!pick(a.b, a.b.Hkv, &job, &hkv)) return;
-  const int G = a.b.Hq / a.b.Hkv;
+  if (!pick(a.b, a.b.Hkv, a.b.by_hkv, &job, &hkv)) return;
+  const int G = a.b.G;
   const int row0 = job.row0, len = job.rows;
   const int qlen = job.keys;  // nothing looks at padding
   const int nblk = (len + kRows - 1) / kRows;
@@ -481,6 +500,7 @@ inline bool view_ok(const void* p, int64_t row, int64_t head) {
 inline bool shape_ok(int T, int J, int Hq, int Hkv, int D, int dtype) {
   return T > 0 && J > 0 && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && (D == 64 || D == 128) &&
          (dtype == kTypeBf16 || dtype == kTypeFp16) && static_cast<int64_t>(J) * Hq < (1LL << 31) &&
+         static_cast<int64_t>(J) * Hq * Hq < (1LL << 32) &&
          static_cast<int64_t>(Hq) * D < (1 << 22);
 }
 
@@ -500,6 +520,12 @@ int bwd(const BwdArgs& a, int J, hipStream_t s) {
   return KGWE_CHECK_LAUNCH();
 }
 
+}  // namespace
+
+namespace {
+inline Batch batch_of(const int* jobs, int T, int Hq, int Hkv) {
+  return {reinterpret_cast<const int4*>(jobs), T, Hq, Hkv, Hq / Hkv, Div(Hq), Div(Hkv), Div(Hq / Hkv)};
+}
 }  // namespace
 
 // One record per call in place of 27 and 25 arguments: converting them one by
@@ -542,7 +568,7 @@ KGWE_API int kgwe_packed_attn_fwd(const PackedFwdCall* c, hipStream_t s) {
        reinterpret_cast<uintptr_t>(c->jobs)) & 15)
     return -1;
   auto in = [](const void* p) { return static_cast<const u16*>(p); };
-  const FwdArgs a{{reinterpret_cast<const int4*>(c->jobs), c->T, c->Hq, c->Hkv},
+  const FwdArgs a{batch_of(c->jobs, c->T, c->Hq, c->Hkv),
                   {in(c->q), c->q_row, c->q_head}, {in(c->k), c->k_row, c->k_head}, {in(c->v), c->v_row, c->v_head},
                   {in(c->pk), c->pk_row, c->pk_head}, {in(c->pv), c->pv_row, c->pv_head},
                   static_cast<u16*>(c->o), static_cast<u16*>(c->o_low), c->lse, c->P, c->causal, c->scale * kLog2e};
@@ -559,7 +585,7 @@ KGWE_API int kgwe_packed_attn_bwd(const PackedBwdCall* c, hipStream_t s) {
                         static_cast<const void*>(c->dv), static_cast<const void*>(c->jobs)})
     if (!p || (reinterpret_cast<uintptr_t>(p) & 15)) return -1;
   auto in = [](const void* p) { return static_cast<const u16*>(p); };
-  const BwdArgs a{{reinterpret_cast<const int4*>(c->jobs), c->T, c->Hq, c->Hkv},
+  const BwdArgs a{batch_of(c->jobs, c->T, c->Hq, c->Hkv),
                   {in(c->q), c->q_row, c->q_head}, {in(c->k), c->k_row, c->k_head}, {in(c->v), c->v_row, c->v_head},
                   in(c->o), in(c->o_low), in(c->dout), c->lse, c->delta, static_cast<u16*>(c->dq),
                   static_cast<u16*>(c->dk), static_cast<u16*>(c->dv), c->causal, c->scale * kLog2e, c->scale};
