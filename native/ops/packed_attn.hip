@@ -159,12 +159,13 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(FwdArgs a) {
       const int kend = pre ? plen : klen;
       const bool edge = (causal && k0 + kTile - 1 > q0) || k0 + kTile > kend;  // wave-uniform
       if (edge) {
-        const int last = causal ? min(kend - 1, qrow) : kend - 1;  // last key this row sees
+        // Last key this row sees, counted as tile_row counts without its lane part.
+        const int last = (causal ? min(kend - 1, qrow) : kend - 1) - k0 - 4 * hh;
 #pragma unroll
         for (int st = 0; st < 2; ++st)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (k0 + 32 * st + tile_row(r, hh) > last) s[st][r] = -INFINITY;
+            if (32 * st + tile_row(r, 0) > last) s[st][r] = -INFINITY;
       }
       float mx = -INFINITY;
 #pragma unroll
@@ -174,7 +175,7 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(FwdArgs a) {
       mx = half_max(mx) * a.c;
       const float m_new = mx > m + kDefer ? mx : m;
       const float m_use = m_new == -INFINITY ? 0.f : m_new;
-      if (__any(m_new > m)) {
+      if (__any(m_new > m && m > -INFINITY)) {  // before a row's first max there is nothing to rescale
         const float alpha = exp2_fast(m - m_use);
         l *= alpha;
 #pragma unroll
@@ -314,7 +315,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(BwdArgs a) {
     const int k0 = t * kTile;
     if (mine && (!a.causal || k0 <= q0 + 31)) {
       const bool edge = (a.causal && k0 + kTile - 1 > q0) || k0 + kTile > klen;
-      const int last = a.causal ? min(klen - 1, qrow) : klen - 1;
+      const int last = (a.causal ? min(klen - 1, qrow) : klen - 1) - k0 - 4 * hh;  // as in the forward
       // Two 32-key halves in turn: one S^T / dP^T pair live at a time.
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
@@ -331,7 +332,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(BwdArgs a) {
         if (edge) {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            if (k0 + 32 * st + tile_row(r, hh) > last) p[r] = 0.f;
+            if (32 * st + tile_row(r, 0) > last) p[r] = 0.f;
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -451,9 +452,10 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(BwdArgs a) {
       // A branch around the masking: selected element by element in the line
       // above it cost 80 of the step's 185 vector instructions.
       if (a.causal && key0 + 31 > qb) {
+        const int before = key - qb - 4 * hh;
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (key > qb + tile_row(r, hh)) s[r] = p[r] = 0.f;
+          if (tile_row(r, 0) < before) s[r] = p[r] = 0.f;
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {

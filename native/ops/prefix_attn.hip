@@ -65,7 +65,7 @@ struct State {
       for (int st = 0; st < NS; ++st)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          if (32 * st + tile_row(r, hh) >= valid) s[st][r] = -INFINITY;
+          if (32 * st + tile_row(r, 0) >= valid - 4 * hh) s[st][r] = -INFINITY;
     }
     float mx = -INFINITY;
 #pragma unroll
@@ -75,7 +75,7 @@ struct State {
     mx = half_max(mx) * c;
     const float m_new = mx > m + kDefer ? mx : m;
     const float m_use = m_new == -INFINITY ? 0.f : m_new;
-    if (__any(m_new > m)) {
+    if (__any(m_new > m && m > -INFINITY)) {  // before a row's first max there is nothing to rescale
       const float alpha = exp2_fast(m - m_use);
       l *= alpha;
 #pragma unroll
