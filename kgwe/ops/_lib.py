@@ -165,10 +165,10 @@ HALF_TYPES = {torch.bfloat16: 0, torch.float16: 1}
 
 
 def rows16(t: torch.Tensor) -> torch.Tensor:
-    """t itself where its last dimension is dense and every row starts on 16
+    """t (2 or 3 dimensions) itself where its last dimension is dense and every row starts on 16
     bytes (what the strided kernels read), else a contiguous copy."""
     s = t.stride()
-    if s[-1] == 1 and not t.data_ptr() & 15 and not any([x & 7 or x < 0 for x in s[:-1]]):
+    if s[-1] == 1 and not t.data_ptr() & 15 and not (s[0] | s[-2]) & 7 and len(s) <= 3:
         return t
     return dense16(t)
 

@@ -139,11 +139,10 @@ def norm_rope_append(qkv: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, si
         kc[at[ok], :, pos[ok].long()] = k[ok]
         vc[at[ok], :, pos[ok].long()] = v[ok]
         return (q, k, v) if keep_kv else q
-    q = torch.empty((T, hq, d), device=device, dtype=dtype)
+    q = qkv.new_empty((T, hq, d))
     k = v = None
     if keep_kv:
-        k = torch.empty((T, hkv, d), device=device, dtype=dtype)
-        v = torch.empty_like(k)
+        k, v = qkv.new_empty((T, hkv, d)), qkv.new_empty((T, hkv, d))
     if T > 0 and kc.numel() > 0:
         if (kc.data_ptr() | vc.data_ptr()) & 15:
             raise ValueError("norm_rope_append: caches must be 16-byte aligned")

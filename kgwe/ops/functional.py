@@ -244,9 +244,7 @@ def check_norm_rope(what, qkv, positions, cos, sin, hq, hkv, d, q_weight, k_weig
 
 def _norm_rope_fwd(qkv, qw, kw, cos, sin, positions, hq, hkv, d, eps, offset):
     T, dtype, device = qkv.shape[0], qkv.dtype, qkv.device
-    q = torch.empty((T, hq, d), device=device, dtype=dtype)
-    k = torch.empty((T, hkv, d), device=device, dtype=dtype)
-    v = torch.empty_like(k)
+    q, k, v = qkv.new_empty((T, hq, d)), qkv.new_empty((T, hkv, d)), qkv.new_empty((T, hkv, d))
     pos, period = (0, positions) if isinstance(positions, int) else (positions.data_ptr(), 0)
     launch("kgwe_norm_rope_fwd", device, qkv.data_ptr(), pos, cos.data_ptr(), sin.data_ptr(), addr(qw), addr(kw),
            q.data_ptr(), k.data_ptr(), v.data_ptr(), 0, 0, 0, qkv.stride(0), T, period, offset, cos.shape[0], hq, hkv, d,
@@ -269,7 +267,7 @@ class _NormRopeQKV(torch.autograd.Function):
         qkv, qw, kw, cos, sin, at = ctx.saved_tensors
         T, hq, hkv, d, eps, offset, period = ctx.meta
         dq, dk, dv = dense16(dq), dense16(dk), dense16(dv)
-        dqkv = torch.empty((T, (hq + 2 * hkv) * d), device=dq.device, dtype=dq.dtype)
+        dqkv = dq.new_empty((T, (hq + 2 * hkv) * d))
         part = dqw = dkw = None
         if qw is not None:
             blocks = int(lib().kgwe_norm_rope_bwd_blocks(T, hq, hkv, d))
