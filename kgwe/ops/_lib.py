@@ -173,6 +173,13 @@ def rows16(t: torch.Tensor) -> torch.Tensor:
     return dense16(t)
 
 
+def tokens16(t: torch.Tensor) -> torch.Tensor:
+    """rows16 of [T, H, D], with a row stride that the kernels' 32-bit offsets
+    inside a tile of rows can hold."""
+    t = rows16(t)
+    return t if t.stride(0) <= 1 << 22 else t.contiguous()
+
+
 def dense16(t: torch.Tensor) -> torch.Tensor:
     """t itself where it is contiguous from a 16-byte boundary on, else a copy."""
     if t.is_contiguous() and not t.data_ptr() & 15:
@@ -181,7 +188,7 @@ def dense16(t: torch.Tensor) -> torch.Tensor:
     return t.clone(memory_format=torch.contiguous_format) if t.data_ptr() & 15 else t
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
@@ -193,10 +200,10 @@ def launch(name: str, device: torch.device, *fields) -> None:
     arguments that ctypes converts one by one.)"""
     fn, record, index = getattr(_lib or lib(), name), RECORDS[name].pack(*fields), device.index
     if index == torch.cuda.current_device():
-        rc = fn(record, _raw_stream(index))
+        rc = fn(record, raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(record, _raw_stream(index))
+            rc = fn(record, raw_stream(index))
     if rc != 0:
         raise RuntimeError(f"{name} failed with code {rc}")
 

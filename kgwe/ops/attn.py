@@ -18,7 +18,7 @@ import torch
 import torch.nn.functional as F
 
 from . import reference as ref
-from ._lib import HALF_TYPES, addr, check, dense16, has_symbol, launch, lib, ptr, rows16, stream, use_hip
+from ._lib import HALF_TYPES, addr, check, dense16, has_symbol, launch, lib, ptr, rows16, stream, tokens16, use_hip
 from .packed import PackedBatch
 
 
@@ -157,8 +157,10 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: P
     (behind the last sequence) give zeros and get zero gradients, whatever they
     hold.  On a GPU: bf16 or fp16, D 64 or 128; q / k / v may be views with
     dense 16-byte aligned rows (slices of a fused projection), others are
-    copied.  A NaN or infinity in v reaches the rows that see it and may reach
-    up to 63 rows before it in its own sequence, never another sequence."""
+    copied.  Never does anything of one sequence enter another, NaN and infinities
+    included.  Inside its own sequence a non-finite value (in v; for gradients
+    also in q, k or the incoming gradient) reaches what depends on it, and may
+    also reach up to 63 rows on its other side of the causal diagonal."""
     qs, ks = q.shape, k.shape
     if not (len(qs) == len(ks) == 3 and v.shape == ks and qs[0] == ks[0] == batch.total and qs[2] == ks[2]
             and qs[1] > 0 and ks[1] > 0 and qs[1] % ks[1] == 0):
@@ -181,7 +183,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: P
         raise ValueError("attention_packed: bf16 or fp16 with head_dim 64 or 128")
     if batch.total == 0:
         return q.clone()
-    q, k, v = rows16(q), rows16(k), rows16(v)
+    q, k, v = tokens16(q), tokens16(k), tokens16(v)
     if grad:
         return _PackedAttn.apply(q, k, v, batch, bool(causal))
     if prefix is not None:

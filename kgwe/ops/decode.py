@@ -34,6 +34,11 @@ def _require(cond: bool, msg: str) -> None:
         raise ValueError(msg)
 
 
+def _forward_only(what: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors]):
+        raise ValueError(f"{what} has no gradient; call it under torch.no_grad()")
+
+
 # ------------------------------------------------------------------ references
 def rope_append_reference(qkv, pos, cos, sin, kc, vc, hq, hkv, d):
     B = qkv.shape[0]
@@ -126,6 +131,7 @@ def norm_rope_append(qkv: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, si
             and kc.data_ptr() != vc.data_ptr()):
         raise ValueError("norm_rope_append: caches must be two contiguous [R, hkv, Smax, d] of qkv's type and device")
     _require(isinstance(pos, torch.Tensor), "norm_rope_append: pos int32 [T]")
+    _forward_only("norm_rope_append", qkv, q_weight, k_weight)
     check_norm_rope("norm_rope_append", qkv, pos, cos, sin, hq, hkv, d, q_weight, k_weight, offset, cache[2] + offset)
     if rows is None:
         _require(T <= cache[0], "norm_rope_append: more rows than the cache has")
@@ -245,6 +251,7 @@ class PrefixDecodeAttention:
         if not (q.shape == (B, hq, d) and pk.shape == pv.shape == (hkv, P, d) and kc.shape == vc.shape == (B, hkv, smax, d)):
             raise ValueError(f"prefix attention: q {(B, hq, d)}, prefix {(hkv, P, d)}, caches {(B, hkv, smax, d)}, got "
                              f"{[tuple(t.shape) for t in (q, pk, pv, kc, vc)]}")
+        _forward_only("prefix attention", q, pk, pv)
         dtype, device = self.dtype, q.device
         if not (q.dtype == pk.dtype == pv.dtype == kc.dtype == vc.dtype == dtype and q.is_cuda == self.hip
                 and pk.device == pv.device == kc.device == vc.device == lens.device == device):

@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import check, lib, ptr, stream
+from ._lib import check, lib, ptr, raw_stream, stream
 
 _INT32_MAX = 2**31 - 1
 
@@ -104,9 +104,20 @@ class PackedBatch:
         slots = int(lib().kgwe_packed_plan_jobs(n, T))
         self.jobs = torch.empty(slots, 4, dtype=torch.int32, device=dev)
         first = torch.empty(n + 2, dtype=torch.int32, device=dev)
-        self.tables = (self.jobs.data_ptr(), slots)  # what the attention launches pass on
+        self._tables = (self.jobs.data_ptr(), slots)
+        self._stream = raw_stream(dev.index)
         check(lib().kgwe_packed_plan(ptr(self.lengths), n, T, ptr(self.cu), ptr(first), ptr(self.jobs), slots,
                                      ptr(self.positions), ptr(self.seq_ids), stream(self.cu)), "packed_plan")
+
+    @property
+    def tables(self) -> tuple:
+        """(job table, slots) for a launch on the current stream.  On another
+        stream than the one they were built on, the table is marked as in use
+        there: dropped while a kernel still reads it, its memory would be
+        handed out again under that kernel."""
+        if raw_stream(self.device.index) != self._stream:
+            self.jobs.record_stream(torch.cuda.current_stream(self.device))
+        return self._tables
 
     @property
     def last_rows(self) -> torch.Tensor:

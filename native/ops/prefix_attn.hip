@@ -120,6 +120,7 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(Args a) {
   // The shared tiles of the wide form; of the slim form wave w's K and V halves of piece w.
   __shared__ __attribute__((aligned(1024))) char K0[kImg], V0[kImg], K1[kImg], V1[kImg];
   __shared__ float ml[4][32][2], joined[32][2];  // (max, sum) of each wave's rows; of all four
+  __shared__ int4 job;  // found, sequence, its keys, chunk
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int lq = lane & 31, hh = lane >> 5;
   const int G = a.G, rows_all = a.B * G, slots = a.p_splits + a.o_splits;
@@ -226,41 +227,48 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(Args a) {
   State<T, D> st;
   if (WIDE || !prefix_job) {
     // The i-th (chunk of a sequence's own keys, key head): the chunks that hold
-    // keys, counted by every wave from lens, 64 sequences at a time.
+    // keys, counted from lens, 64 sequences at a time.
     int b, len, start = 0;
     if (direct) {
       b = a.by_hkv(i);
       kvh = i - b * a.Hkv;
       len = min(max(a.lens[b], 0), a.Smax);
     } else {
-      int left = a.by_hkv(i), b0 = 0;
-      kvh = i - left * a.Hkv;
-      for (;; b0 += 64) {
-        if (b0 >= a.B) return;  // every chunk is taken
-        const int n = b0 + lane < a.B ? min(max(a.lens[b0 + lane], 0), a.Smax) : 0;
-        // where nothing is joined an empty row's zeros have to be written, too
-        const int chunks = final ? (b0 + lane < a.B ? 1 : 0) : (n + a.o_chunk - 1) / a.o_chunk;
-        int upto = chunks;
+      const int unit = a.by_hkv(i);
+      kvh = i - unit * a.Hkv;
+      if (w == 0) {  // one wave decides for all four, whatever happens to lens meanwhile
+        int left = unit, b0 = 0, found = 0;
+        for (; b0 < a.B; b0 += 64) {
+          const int n = b0 + lane < a.B ? min(max(a.lens[b0 + lane], 0), a.Smax) : 0;
+          // where nothing is joined an empty row's zeros have to be written, too
+          const int chunks = final ? (b0 + lane < a.B ? 1 : 0) : (n + a.o_chunk - 1) / a.o_chunk;
+          int upto = chunks;
 #pragma unroll
-        for (int off = 1; off < kWave; off <<= 1) {
-          const int y = __shfl_up(upto, off, kWave);
-          if (lane >= off) upto += y;
+          for (int off = 1; off < kWave; off <<= 1) {
+            const int y = __shfl_up(upto, off, kWave);
+            if (lane >= off) upto += y;
+          }
+          const unsigned long long past = __ballot(upto > left);
+          if (past != 0) {
+            const int f = __builtin_ctzll(past);
+            const int first = left - __shfl(upto - chunks, f, kWave), own = __shfl(n, f, kWave);
+            if (lane == 0) job = make_int4(1, b0 + f, own, first);
+            found = 1;
+            break;
+          }
+          left -= __shfl(upto, 63, kWave);
         }
-        const unsigned long long past = __ballot(upto > left);
-        if (past != 0) {
-          const int f = __builtin_ctzll(past);
-          b = b0 + f;
-          len = __shfl(n, f, kWave);
-          start = left - __shfl(upto - chunks, f, kWave);
-          break;
-        }
-        left -= __shfl(upto, 63, kWave);
+        if (!found && lane == 0) job = make_int4(0, 0, 0, 0);
       }
-      slot = a.p_splits + start;
-      start *= a.o_chunk;
+      __syncthreads();
+      const int4 j = job;
+      if (j.x == 0) return;  // every chunk is taken
+      b = j.y;
+      len = j.z;
+      slot = __builtin_amdgcn_readfirstlane(a.p_splits + j.w);
+      start = j.w * a.o_chunk;
     }
     b = __builtin_amdgcn_readfirstlane(b);
-    slot = __builtin_amdgcn_readfirstlane(slot);
     start = __builtin_amdgcn_readfirstlane(start);
     first_row = b * G;
     wk.n1 = __builtin_amdgcn_readfirstlane(direct ? len : min(a.o_chunk, len - start));
@@ -516,10 +524,12 @@ int launch(Args a, hipStream_t s) {
   return KGWE_CHECK_LAUNCH();
 }
 
+// (The last term: numbers that the kernel divides by the head count, see Div.)
 inline bool shape_ok(int B, int Hq, int Hkv, int D, int P, int Smax) {
   return B > 0 && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && Hq / Hkv <= 32 && (D == 64 || D == 128) && P >= 0 &&
          Smax >= 0 && P + static_cast<int64_t>(Smax) > 0 && P < (1 << 30) && Smax < (1 << 30) &&
-         static_cast<int64_t>(B) * Hq < (1 << 24) && Hkv <= 1024;
+         static_cast<int64_t>(B) * Hq < (1 << 24) && Hkv <= 1024 &&
+         (static_cast<int64_t>(B) * (Smax / 256 + 1) * Hkv + 512) * Hkv < (1LL << 32);
 }
 
 }  // namespace

@@ -240,6 +240,37 @@ def test_repeats_bit_for_bit_and_on_another_stream():
         assert torch.equal(a, b) and torch.equal(a, c)
 
 
+def test_a_batch_dropped_while_another_stream_uses_it():
+    """The job table is marked as in use on the stream of the launch: memory handed out after the batch is
+    gone does not come from under the kernel."""
+    g = torch.Generator(device="cuda").manual_seed(14)
+    lengths = [3000, 2000, 1]
+    T = sum(lengths)
+    q, k, v = (_rnd(g, T, h, 64) for h in (16, 4, 4))
+    want = attention_packed(q, k, v, PackedBatch(lengths))
+    s = torch.cuda.Stream()
+    for _ in range(4):
+        batch = PackedBatch(lengths)
+        slots = batch.jobs.shape[0]
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got = attention_packed(q, k, v, batch)
+        del batch
+        other = [torch.zeros(slots, 4, dtype=torch.int32, device="cuda") for _ in range(8)]  # rows = 0 everywhere
+        torch.cuda.current_stream().wait_stream(s)
+        assert torch.equal(got, want)
+        del other
+
+
+def test_far_rows_are_copied():
+    """A row stride past the kernels' 32-bit tile offsets: a copy, not a refusal."""
+    base = torch.zeros(5 * ((1 << 22) + 8), device="cuda", dtype=torch.bfloat16)
+    q = base.as_strided((5, 2, 64), ((1 << 22) + 8, 64, 1))
+    q.copy_(torch.randn(5, 2, 64, device="cuda"))
+    b = PackedBatch([5])
+    assert torch.equal(attention_packed(q, q, q, b), attention_packed(*[q.contiguous()] * 3, b))
+
+
 def test_captured_with_its_plan_and_replayed():
     """The plan is built inside the capture from lengths on the GPU: a replay follows new lengths."""
     g = torch.Generator(device="cuda").manual_seed(9)

@@ -116,6 +116,7 @@ def test_norm_rope_refusals():
                 lambda: norm_rope_qkv(qkv, cos, sin, pos.long(), hq, hkv, d),
                 lambda: norm_rope_qkv(qkv, cos, sin, pos[:2], hq, hkv, d),
                 lambda: norm_rope_qkv(qkv, cos, sin, 0, hq, hkv, d),
+                lambda: dec.norm_rope_append(qkv.clone().requires_grad_(), pos, cos, sin, kc, kc.clone(), hq, hkv, d),
                 lambda: dec.norm_rope_append(qkv, 3, cos, sin, kc, kc.clone(), hq, hkv, d),
                 lambda: norm_rope_qkv(qkv, cos, sin, pos, hq, hkv, d, q_weight=w),
                 lambda: norm_rope_qkv(qkv, cos, sin, pos, hq, hkv, d, w[:4], w[:4]),
@@ -176,6 +177,7 @@ def test_prefix_attention_refusals():
     q, p, c = torch.zeros(1, 4, 16), torch.zeros(2, 5, 16), torch.zeros(1, 2, 8, 16)
     lens = torch.zeros(1, dtype=torch.int32)
     for args in ((q[:, :2], p, p, c, c, lens), (q, p[:, :4], p[:, :4], c, c, lens), (q, p, p, c[:, :, :7], c[:, :, :7], lens),
-                 (q, p, p, c, c, lens.long()), (q, p.double(), p, c, c, lens), (q, p, p, c, c, lens[:0])):
+                 (q, p, p, c, c, lens.long()), (q, p.double(), p, c, c, lens), (q, p, p, c, c, lens[:0]),
+                 (q.clone().requires_grad_(), p, p, c, c, lens)):
         with pytest.raises(ValueError):
             att(*args)
