@@ -173,11 +173,17 @@ def rows16(t: torch.Tensor) -> torch.Tensor:
     return dense16(t)
 
 
-def tokens16(t: torch.Tensor) -> torch.Tensor:
-    """rows16 of [T, H, D], with a row stride that the kernels' 32-bit offsets
-    inside a tile of rows can hold."""
-    t = rows16(t)
-    return t if t.stride(0) <= 1 << 22 else t.contiguous()
+def token_view(t: torch.Tensor) -> tuple:
+    """(tensor, address, row stride, head stride) of [T, H, D] as the strided
+    kernels read it: t itself where its last dimension is dense, every row
+    starts on 16 bytes and the row stride fits the kernels' 32-bit offsets
+    inside a tile of rows, else a contiguous copy."""
+    s0, s1, s2 = t.stride()
+    at = t.data_ptr()
+    if s2 != 1 or (s0 | s1) & 7 or at & 15 or s0 > 1 << 22:
+        t = dense16(t.contiguous())
+        (s0, s1, _), at = t.stride(), t.data_ptr()
+    return t, at, s0, s1
 
 
 def dense16(t: torch.Tensor) -> torch.Tensor:

@@ -18,7 +18,7 @@ import torch
 import torch.nn.functional as F
 
 from . import reference as ref
-from ._lib import HALF_TYPES, addr, check, dense16, has_symbol, launch, lib, ptr, rows16, stream, tokens16, use_hip
+from ._lib import HALF_TYPES, addr, check, dense16, has_symbol, launch, lib, ptr, rows16, stream, token_view, use_hip
 from .packed import PackedBatch
 
 
@@ -98,33 +98,32 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
 # --------------------------------------------------------------------------
 # Packed sequences
 # --------------------------------------------------------------------------
-_dense = {"memory_format": torch.contiguous_format}
-
-
-def _packed_fwd(q, k, v, batch, causal, prefix, train):
-    T, Hq, D = q.shape
-    o = torch.empty_like(q, **_dense)
+def _packed_fwd(qv, kv, vv, batch, causal, prefix, train):
+    """qv, kv, vv: token_view of q, k, v."""
+    (q, qp, qr, qh), (k, kp, kr, kh), (_, vp, vr, vh) = qv, kv, vv
+    (T, Hq, D), device = q.shape, q.device
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
     low = lse = None
     if train:
-        lse = torch.empty((Hq, T), device=q.device, dtype=torch.float32)
+        lse = torch.empty((Hq, T), device=device, dtype=torch.float32)
         low = torch.empty_like(o)  # what the rounding of o drops
-    (qr, qh, _), (kr, kh, _), (vr, vh, _) = q.stride(), k.stride(), v.stride()
-    jobs, slots = batch.tables
     if prefix is None:
         pk = pv = pkr = pkh = pvr = pvh = P = 0
     else:  # [Hkv, P, D]: row stride, head stride
         (pkh, pkr, _), (pvh, pvr, _), P = prefix[0].stride(), prefix[1].stride(), prefix[0].shape[1]
         pk, pv = prefix[0].data_ptr(), prefix[1].data_ptr()
-    launch("kgwe_packed_attn_fwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), pk, pv, o.data_ptr(), addr(low),
-           addr(lse), jobs, qr, qh, kr, kh, vr, vh, pkr, pkh, pvr, pvh, P, slots, T, Hq, k.shape[1], D, causal,
-           HALF_TYPES[q.dtype], D ** -0.5)
+    jobs, slots = batch.tables
+    launch("kgwe_packed_attn_fwd", device, qp, kp, vp, pk, pv, o.data_ptr(), addr(low), addr(lse), jobs, qr, qh, kr, kh,
+           vr, vh, pkr, pkh, pvr, pvh, P, slots, T, Hq, k.shape[1], D, causal, HALF_TYPES[q.dtype], D ** -0.5)
     return o, low, lse
 
 
 class _PackedAttn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, batch, causal):
-        o, low, lse = _packed_fwd(q, k, v, batch, causal, None, True)
+        views = token_view(q), token_view(k), token_view(v)
+        o, low, lse = _packed_fwd(*views, batch, causal, None, True)
+        q, k, v = (t[0] for t in views)
         ctx.save_for_backward(q, k, v, o, low, lse)
         ctx.batch, ctx.causal = batch, causal
         return o
@@ -137,7 +136,7 @@ class _PackedAttn(torch.autograd.Function):
         T, Hq, D = q.shape
         Hkv = k.shape[1]
         do = dense16(do)
-        dq, dk, dv = (torch.empty_like(t, **_dense) for t in (q, k, k))
+        dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
         delta = torch.empty_like(lse)
         (qr, qh, _), (kr, kh, _), (vr, vh, _) = q.stride(), k.stride(), v.stride()
         jobs, slots = batch.tables
@@ -177,15 +176,14 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: P
             raise ValueError("attention_packed: prefix keys and values must be [Hkv, P, D] of k's type and device")
         if grad or (torch.is_grad_enabled() and (pk.requires_grad or pv.requires_grad)):
             raise ValueError("attention_packed: a shared prefix has no gradient; call it under torch.no_grad()")
-    if not use_hip(q):
+    if not q.is_cuda:
         return ref.attention_packed(q, k, v, batch.lengths.tolist(), causal, prefix)
     if dtype not in HALF_TYPES or qs[2] not in (64, 128):
         raise ValueError("attention_packed: bf16 or fp16 with head_dim 64 or 128")
     if batch.total == 0:
         return q.clone()
-    q, k, v = tokens16(q), tokens16(k), tokens16(v)
     if grad:
         return _PackedAttn.apply(q, k, v, batch, bool(causal))
     if prefix is not None:
         prefix = (rows16(pk), rows16(pv)) if pk.shape[1] else None
-    return _packed_fwd(q, k, v, batch, bool(causal), prefix, False)[0]
+    return _packed_fwd(token_view(q), token_view(k), token_view(v), batch, bool(causal), prefix, False)[0]

@@ -35,7 +35,9 @@ def _require(cond: bool, msg: str) -> None:
 
 
 def _forward_only(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in tensors]):
+    if not torch.is_grad_enabled():
+        return
+    if any([t is not None and t.requires_grad for t in tensors]):
         raise ValueError(f"{what} has no gradient; call it under torch.no_grad()")
 
 
@@ -138,7 +140,7 @@ def norm_rope_append(qkv: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, si
     else:
         _require(rows.dtype == torch.int32 and rows.shape == (T,) and rows.device == device,
                  "norm_rope_append: rows int32 [T]")
-    if not use_hip(qkv):
+    if not qkv.is_cuda:
         q, k, v = ref.norm_rope_qkv(qkv, cos, sin, pos, hq, hkv, d, q_weight, k_weight, eps, offset)
         at = torch.arange(T, device=qkv.device) if rows is None else rows.long()
         ok = (pos >= 0) & (pos < kc.shape[2]) & (at >= 0) & (at < kc.shape[0])
@@ -263,12 +265,14 @@ class PrefixDecodeAttention:
         if not (kc.is_contiguous() and vc.is_contiguous()) or (kc.data_ptr() | vc.data_ptr()) & 15:
             raise ValueError("prefix attention: caches must be contiguous and 16-byte aligned")
         q, pk, pv, lens = dense16(q), rows16(pk), rows16(pv), lens.contiguous()
-        if P > 0 and pk.stride() != pv.stride():  # one pair of strides for both
+        strides = pk.stride()
+        if strides != pv.stride():  # one pair of strides for both
             pk, pv = dense16(pk), dense16(pv)
+            strides = pk.stride()
         out = torch.empty_like(q)
         work = torch.empty(self.words, device=device, dtype=torch.float32) if self.words else None
         launch("kgwe_prefix_attn", device, q.data_ptr(), pk.data_ptr(), pv.data_ptr(), kc.data_ptr(), vc.data_ptr(),
-               lens.data_ptr(), addr(work), out.data_ptr(), max(pk.stride(1), d), pk.stride(0), B, hq, hkv, d, P, smax,
+               lens.data_ptr(), addr(work), out.data_ptr(), max(strides[1], d), strides[0], B, hq, hkv, d, P, smax,
                HALF_TYPES[dtype], d ** -0.5)
         return out
 

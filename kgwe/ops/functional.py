@@ -291,7 +291,7 @@ def norm_rope_qkv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, posit
     or outside the tables gives zeros and takes no gradient.  Differentiable
     with regard to qkv and the weights."""
     check_norm_rope("norm_rope_qkv", qkv, positions, cos, sin, hq, hkv, d, q_weight, k_weight, offset, 1)
-    if not use_hip(qkv):
+    if not qkv.is_cuda:
         return ref.norm_rope_qkv(qkv, cos, sin, positions, hq, hkv, d, q_weight, k_weight, eps, offset)
     if qkv.shape[0] == 0:
         q, k, v = qkv.reshape(0, hq + 2 * hkv, d).split((hq, hkv, hkv), dim=1)
