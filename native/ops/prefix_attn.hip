@@ -8,14 +8,22 @@
 // step, not once per sequence.  The rows of one key head, B x G of them (G =
 // Hq / Hkv), are therefore one matrix: a workgroup takes a chunk of the
 // prefix's keys for 128 rows (or for all of them, where there are at most 32)
-// on the matrix cores, another one a chunk of one sequence's own keys for its
-// G rows; a second small launch joins the chunks' (max, sum, output) states.
-// Where prefix and cache are short, one workgroup per (sequence, key head)
-// walks both and nothing is joined.
+// on the matrix cores, another one chunks of single sequences' own keys for
+// their G rows; a second small launch joins the chunks' (max, sum, output)
+// states.  Where prefix and cache are short, one workgroup per (sequence, key
+// head) walks both and nothing is joined.
 //
-// Chunk counts depend on capacities only (P, Smax, B), never on lens, so a
-// step can be captured in a graph and replayed at any length; a workgroup
-// whose chunk lies past its sequence's end leaves at once.
+// The grid depends on capacities only (P, Smax, B), never on lens, so a step
+// can be captured in a graph and replayed at any length: the workgroups of the
+// own keys count the chunks that hold keys from lens and take every o_wgs-th.
+//
+// Measured (32 / 8 heads, bf16, GPU time of a call): 64 rows, 32,768 shared
+// keys and up to 1,500 own ones, D 128: 52.5 us, of which the join 7 us; the
+// 184 MB alone take 37 us at the card's copy rate, 3.5 TB/s is reached while
+// every prefix key is also multiplied with 256 rows.  32 rows, 2,048 + up to
+// 1,000 keys, D 64: 10.4 us for 14 MB, two launches' latency.  4 rows, 200 +
+// up to 60 keys: 4.8 us, one launch.  1,024 rows, 500 + up to 1,000 keys,
+// D 64: 123 us.
 #include <algorithm>
 
 #include "attn_tile.h"
@@ -111,8 +119,8 @@ struct Walk {
   int n0, n1, row0, row1;
 };
 
-// WIDE: more than 32 rows a key head. (Two kernels: with both forms of the
-// prefix walk in one, scalar registers spill and the short cases lose 15 %.)
+// WIDE: more than 32 rows a key head.  Two kernels, as with both forms of the
+// prefix walk in one the short cases take 15 % longer.
 template <class T, int D, bool WIDE>
 __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(Args a) {
   constexpr int NB = D / 32, NT = D / 16;
@@ -223,169 +231,173 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(Args a) {
   // 4) with its own K and V buffer and no barrier: the next K tile is on its
   // way from the S product on, the next V tile from the O product on.
   const TileDma<D, kSlim, 1> dma(0, lane);
+  int scan_b = 0, scan_chunks = 0;  // (wave 0) sequences counted so far, chunks that they hold
   for (;; i += a.o_wgs) {
-  State<T, D> st;
-  if (WIDE || !prefix_job) {
-    // The i-th (chunk of a sequence's own keys, key head): the chunks that hold
-    // keys, counted from lens, 64 sequences at a time.
-    int b, len, start = 0;
-    if (direct) {
-      b = a.by_hkv(i);
-      kvh = i - b * a.Hkv;
-      len = min(max(a.lens[b], 0), a.Smax);
-    } else {
-      const int unit = a.by_hkv(i);
-      kvh = i - unit * a.Hkv;
-      if (w == 0) {  // one wave decides for all four, whatever happens to lens meanwhile
-        int left = unit, b0 = 0, found = 0;
-        for (; b0 < a.B; b0 += 64) {
-          const int n = b0 + lane < a.B ? min(max(a.lens[b0 + lane], 0), a.Smax) : 0;
-          // where nothing is joined an empty row's zeros have to be written, too
-          const int chunks = final ? (b0 + lane < a.B ? 1 : 0) : (n + a.o_chunk - 1) / a.o_chunk;
-          int upto = chunks;
+    State<T, D> st;
+    if (WIDE || !prefix_job) {
+      // The i-th (chunk of a sequence's own keys, key head): the chunks that hold
+      // keys, counted from lens, 64 sequences at a time.
+      int b, len, start = 0;
+      if (direct) {
+        b = a.by_hkv(i);
+        kvh = i - b * a.Hkv;
+        len = min(max(a.lens[b], 0), a.Smax);
+      } else {
+        const int unit = a.by_hkv(i);
+        kvh = i - unit * a.Hkv;
+        if (w == 0) {  // one wave decides for all four, whatever happens to lens meanwhile
+          int left = unit - scan_chunks, b0 = scan_b, found = 0;
+          for (; b0 < a.B; b0 += 64) {
+            const int n = b0 + lane < a.B ? min(max(a.lens[b0 + lane], 0), a.Smax) : 0;
+            // where nothing is joined an empty row's zeros have to be written, too
+            const int chunks = final ? (b0 + lane < a.B ? 1 : 0) : (n + a.o_chunk - 1) / a.o_chunk;
+            int upto = chunks;
 #pragma unroll
-          for (int off = 1; off < kWave; off <<= 1) {
-            const int y = __shfl_up(upto, off, kWave);
-            if (lane >= off) upto += y;
+            for (int off = 1; off < kWave; off <<= 1) {
+              const int y = __shfl_up(upto, off, kWave);
+              if (lane >= off) upto += y;
+            }
+            const unsigned long long past = __ballot(upto > left);
+            if (past != 0) {
+              const int f = __builtin_ctzll(past);
+              const int first = left - __shfl(upto - chunks, f, kWave), own = __shfl(n, f, kWave);
+              if (lane == 0) job = make_int4(1, b0 + f, own, first);
+              scan_b = b0;  // the next chunk of this workgroup lies behind this one
+              scan_chunks = unit - left;
+              found = 1;
+              break;
+            }
+            left -= __shfl(upto, 63, kWave);
           }
-          const unsigned long long past = __ballot(upto > left);
-          if (past != 0) {
-            const int f = __builtin_ctzll(past);
-            const int first = left - __shfl(upto - chunks, f, kWave), own = __shfl(n, f, kWave);
-            if (lane == 0) job = make_int4(1, b0 + f, own, first);
-            found = 1;
-            break;
-          }
-          left -= __shfl(upto, 63, kWave);
+          if (!found && lane == 0) job = make_int4(0, 0, 0, 0);
         }
-        if (!found && lane == 0) job = make_int4(0, 0, 0, 0);
+        __syncthreads();
+        const int4 j = job;
+        if (j.x == 0) return;  // every chunk is taken
+        b = j.y;
+        len = j.z;
+        slot = __builtin_amdgcn_readfirstlane(a.p_splits + j.w);
+        start = j.w * a.o_chunk;
+      }
+      b = __builtin_amdgcn_readfirstlane(b);
+      start = __builtin_amdgcn_readfirstlane(start);
+      first_row = b * G;
+      wk.n1 = __builtin_amdgcn_readfirstlane(direct ? len : min(a.o_chunk, len - start));
+      const int64_t at = ((static_cast<int64_t>(b) * a.Hkv + kvh) * a.Smax + start) * D;
+      wk.k1 = a.kc + at;
+      wk.v1 = a.vc + at;
+      if (direct) {
+        wk.k0 = a.pk + kvh * a.p_head;
+        wk.v0 = a.pv + kvh * a.p_head;
+        wk.n0 = a.P;
+      }
+    }
+    {
+      const int r = first_row + lq, rb = a.by_g(r);
+      const int64_t qi = static_cast<int64_t>(rb) * a.Hq + kvh * G + (r - rb * G);
+      load_q<T, D>(a.q + qi * D, lq < nrows, hh, qf);
+    }
+    const int t0 = WIDE ? 0 : (wk.n0 + kSlim - 1) / kSlim, nt = t0 + (wk.n1 + kSlim - 1) / kSlim;
+    auto load = [&](bool keys, char* dst, int t) {
+      const bool own = WIDE || t >= t0;
+      const int at = (own ? t - t0 : t) * kSlim, rows = min(kSlim, (own ? wk.n1 : wk.n0) - at);
+      const int row = own ? wk.row1 : wk.row0;
+      const u16* base = own ? (keys ? wk.k1 : wk.v1) : (keys ? wk.k0 : wk.v0);
+      dma.load(row_buffer(base + static_cast<int64_t>(at) * (row / 2), rows, row), row, dst);
+    };
+    constexpr int kDma = TileDma<D, kSlim, 1>::kN;
+    char* const piece_w = w == 0 ? K0 : w == 1 ? V0 : w == 2 ? K1 : V1;
+    char* const Kb = piece_w;
+    char* const Vb = Kb + kImg / 2;
+    if (w < nt) {
+      load(true, Kb, w);
+      load(false, Vb, w);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) asm volatile("" ::"v"(qf[t]));  // Q has landed before the loop (see packed_attn.hip)
+      for (int t = w; t < nt; t += 4) {
+        const bool more = t + 4 < nt;
+        f32x16 s[1];
+        s[0] = f32x16{};
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kDma) : "memory");  // K has landed, V may be on its way
+#pragma unroll
+        for (int u = 0; u < NT; ++u) s[0] = mfma32<T>(ad.rows(Kb, 0, u), qf[u], s[0]);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read: its buffer is free
+        if (more) load(true, Kb, t + 4);
+        u32x4 pb[2];
+        st.template soften<1>(s, WIDE || t >= t0 ? wk.n1 - (t - t0) * kSlim : wk.n0 - t * kSlim, a.c, hh, pb);
+        // V has landed, the next K may be on its way
+        if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kDma) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int db = 0; db < NB; ++db) st.o[db] = mfma32<T>(ad.cols(Vb, 16 * u, db), as_op(pb[u]), st.o[db]);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (more) load(false, Vb, t + 4);
+      }
+    }
+
+    // Join the four waves through LDS: a common max, then the scaled outputs.
+    const float lw = half_add(st.l);
+    if (hh == 0) {
+      ml[w][lq][0] = st.m;
+      ml[w][lq][1] = lw;
+    }
+    __syncthreads();  // also: every wave is done with the tile buffers
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) M = fmaxf(M, ml[v][lq][0]);
+    const float M_use = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) L += ml[v][lq][1] * exp2_fast(ml[v][lq][0] - M_use);
+    {
+      // Row lq of this wave's [32][D] fp32 region, its 16-byte pieces XOR-swizzled
+      // by the row (rows are a multiple of all banks apart).
+      constexpr int kPieces = D / 4;
+      char* reg = piece_w;
+      const float mul = exp2_fast(st.m - M_use);
+      if (lq < nrows) {
+#pragma unroll
+        for (int db = 0; db < NB; ++db)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            f32x4 v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = st.o[db][4 * g + j] * mul;
+            const int piece = 8 * db + 2 * g + hh;
+            *reinterpret_cast<f32x4*>(reg + lq * D * 4 + 16 * (piece ^ (lq & (kPieces - 1)))) = v;
+          }
+        if (w == 0 && hh == 0) {
+          joined[lq][0] = M;
+          joined[lq][1] = L;
+        }
       }
       __syncthreads();
-      const int4 j = job;
-      if (j.x == 0) return;  // every chunk is taken
-      b = j.y;
-      len = j.z;
-      slot = __builtin_amdgcn_readfirstlane(a.p_splits + j.w);
-      start = j.w * a.o_chunk;
-    }
-    b = __builtin_amdgcn_readfirstlane(b);
-    start = __builtin_amdgcn_readfirstlane(start);
-    first_row = b * G;
-    wk.n1 = __builtin_amdgcn_readfirstlane(direct ? len : min(a.o_chunk, len - start));
-    const int64_t at = ((static_cast<int64_t>(b) * a.Hkv + kvh) * a.Smax + start) * D;
-    wk.k1 = a.kc + at;
-    wk.v1 = a.vc + at;
-    if (direct) {
-      wk.k0 = a.pk + kvh * a.p_head;
-      wk.v0 = a.pv + kvh * a.p_head;
-      wk.n0 = a.P;
-    }
-  }
-  {
-    const int r = first_row + lq, rb = a.by_g(r);
-    const int64_t qi = static_cast<int64_t>(rb) * a.Hq + kvh * G + (r - rb * G);
-    load_q<T, D>(a.q + qi * D, lq < nrows, hh, qf);
-  }
-  const int t0 = WIDE ? 0 : (wk.n0 + kSlim - 1) / kSlim, nt = t0 + (wk.n1 + kSlim - 1) / kSlim;
-  auto load = [&](bool keys, char* dst, int t) {
-    const bool own = WIDE || t >= t0;
-    const int at = (own ? t - t0 : t) * kSlim, rows = min(kSlim, (own ? wk.n1 : wk.n0) - at);
-    const int row = own ? wk.row1 : wk.row0;
-    const u16* base = own ? (keys ? wk.k1 : wk.v1) : (keys ? wk.k0 : wk.v0);
-    dma.load(row_buffer(base + static_cast<int64_t>(at) * (row / 2), rows, row), row, dst);
-  };
-  constexpr int kDma = TileDma<D, kSlim, 1>::kN;
-  char* const piece_w = w == 0 ? K0 : w == 1 ? V0 : w == 2 ? K1 : V1;
-  char* const Kb = piece_w;
-  char* const Vb = Kb + kImg / 2;
-  if (w < nt) {
-    load(true, Kb, w);
-    load(false, Vb, w);
+      for (int e = threadIdx.x; e < nrows * kPieces; e += 256) {
+        const int row = e / kPieces, piece = e - row * kPieces;
+        const int off = row * D * 4 + 16 * (piece ^ (row & (kPieces - 1)));
+        const f32x4 v = (*reinterpret_cast<const f32x4*>(K0 + off) + *reinterpret_cast<const f32x4*>(V0 + off)) +
+                        (*reinterpret_cast<const f32x4*>(K1 + off) + *reinterpret_cast<const f32x4*>(V1 + off));
+        const int rr = first_row + row, rb = a.by_g(rr);
+        const int64_t qi = static_cast<int64_t>(rb) * a.Hq + kvh * G + (rr - rb * G);
+        const float Lr = joined[row][1];
+        if (final) {
+          const float inv = Lr == 0.f ? 0.f : 1.f / Lr;
+          u16x4 y;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) asm volatile("" ::"v"(qf[t]));  // Q has landed before the loop (see packed_attn.hip)
-    for (int t = w; t < nt; t += 4) {
-      const bool more = t + 4 < nt;
-      f32x16 s[1];
-      s[0] = f32x16{};
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kDma) : "memory");  // K has landed, V may be on its way
-#pragma unroll
-      for (int u = 0; u < NT; ++u) s[0] = mfma32<T>(ad.rows(Kb, 0, u), qf[u], s[0]);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read: its buffer is free
-      if (more) load(true, Kb, t + 4);
-      u32x4 pb[2];
-      st.template soften<1>(s, WIDE || t >= t0 ? wk.n1 - (t - t0) * kSlim : wk.n0 - t * kSlim, a.c, hh, pb);
-      if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kDma) : "memory");  // V has landed, the next K may be on its way
-      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int db = 0; db < NB; ++db) st.o[db] = mfma32<T>(ad.cols(Vb, 16 * u, db), as_op(pb[u]), st.o[db]);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (more) load(false, Vb, t + 4);
-    }
-  }
-
-  // Join the four waves through LDS: a common max, then the scaled outputs.
-  const float lw = half_add(st.l);
-  if (hh == 0) {
-    ml[w][lq][0] = st.m;
-    ml[w][lq][1] = lw;
-  }
-  __syncthreads();  // also: every wave is done with the tile buffers
-  float M = -INFINITY, L = 0.f;
-#pragma unroll
-  for (int v = 0; v < 4; ++v) M = fmaxf(M, ml[v][lq][0]);
-  const float M_use = M == -INFINITY ? 0.f : M;
-#pragma unroll
-  for (int v = 0; v < 4; ++v) L += ml[v][lq][1] * exp2_fast(ml[v][lq][0] - M_use);
-  {
-    // Row lq of this wave's [32][D] fp32 region, its 16-byte pieces XOR-swizzled
-    // by the row (rows are a multiple of all banks apart).
-    constexpr int kPieces = D / 4;
-    char* reg = piece_w;
-    const float mul = exp2_fast(st.m - M_use);
-    if (lq < nrows) {
-#pragma unroll
-      for (int db = 0; db < NB; ++db)
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          f32x4 v;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = st.o[db][4 * g + j] * mul;
-          const int piece = 8 * db + 2 * g + hh;
-          *reinterpret_cast<f32x4*>(reg + lq * D * 4 + 16 * (piece ^ (lq & (kPieces - 1)))) = v;
-        }
-      if (w == 0 && hh == 0) {
-        joined[lq][0] = M;
-        joined[lq][1] = L;
-      }
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < nrows * kPieces; e += 256) {
-      const int row = e / kPieces, piece = e - row * kPieces;
-      const int off = row * D * 4 + 16 * (piece ^ (row & (kPieces - 1)));
-      const f32x4 v = (*reinterpret_cast<const f32x4*>(K0 + off) + *reinterpret_cast<const f32x4*>(V0 + off)) +
-                      (*reinterpret_cast<const f32x4*>(K1 + off) + *reinterpret_cast<const f32x4*>(V1 + off));
-      const int rr = first_row + row, rb = a.by_g(rr);
-      const int64_t qi = static_cast<int64_t>(rb) * a.Hq + kvh * G + (rr - rb * G);
-      const float Lr = joined[row][1];
-      if (final) {
-        const float inv = Lr == 0.f ? 0.f : 1.f / Lr;
-        u16x4 y;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = T::down(v[j] * inv);
-        *reinterpret_cast<u16x4*>(a.out + qi * D + 4 * piece) = y;
-      } else {
-        *reinterpret_cast<f32x4*>(a.part_o + (qi * slots + slot) * D + 4 * piece) = v;
-        if (piece == 0) {
-          a.part_ml[(qi * slots + slot) * 2] = joined[row][0];
-          a.part_ml[(qi * slots + slot) * 2 + 1] = Lr;
+          for (int j = 0; j < 4; ++j) y[j] = T::down(v[j] * inv);
+          *reinterpret_cast<u16x4*>(a.out + qi * D + 4 * piece) = y;
+        } else {
+          *reinterpret_cast<f32x4*>(a.part_o + (qi * slots + slot) * D + 4 * piece) = v;
+          if (piece == 0) {
+            a.part_ml[(qi * slots + slot) * 2] = joined[row][0];
+            a.part_ml[(qi * slots + slot) * 2 + 1] = Lr;
+          }
         }
       }
     }
-  }
-  if (!WIDE && (prefix_job || direct)) return;
-  __syncthreads();  // the tile buffers are read before the next chunk fills them
+    if (!WIDE && (prefix_job || direct)) return;
+    __syncthreads();  // the tile buffers are read before the next chunk fills them
   }
 }
 
@@ -393,9 +405,9 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(Args a) {
 // hold keys.  W waves share a row; wave w of them takes every W-th slot, lane i
 // of it the (max, sum) of the i-th of those.  Few rows have many slots and want
 // 4 waves each (1 row x 32 heads, 66 slots: 21.2 -> 16.5 us with the launch
-// before it), many rows one (32 x 32 heads, 12 slots: 12.2 -> 10.7 us).  The first loads of a wave are issued before
-// anything is known of n: what lies past it is the workspace's own memory, and
-// is dropped by selection.
+// before it), many rows one (32 x 32 heads, 12 slots: 12.2 -> 10.7 us).  The
+// first loads of a wave are issued before anything is known of n: what lies
+// past it is the workspace's own memory, and is dropped by selection.
 template <class T, int D, int W>
 __global__ __launch_bounds__(256) void prefix_join_kernel(Args a) {
   constexpr int E = D / 64;  // outputs per lane
@@ -478,7 +490,8 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(Args a) {
 //
 // Own keys: chunks of 256 that 512 workgroups share out among them by counting
 // (a workgroup for every possible chunk, most of them empty, cost 8 us more at
-// 64 rows of 2,048).
+// 64 rows of 2,048).  A workgroup counts on from its last chunk; from the first
+// sequence each time, 1,024 rows took 194 us instead of 123.
 //
 // One workgroup per (sequence, key head), no join: while prefix and cache hold
 // at most 1,024 keys and the workgroups fit the chip at once (48 rows, 16 / 2

@@ -489,6 +489,21 @@ def test_prefix_attention(B, hq, hkv, d, smax, P, lens, dtype):
     assert torch.equal(got, again)
 
 
+@pytest.mark.parametrize("P", [0, 513])
+def test_prefix_attention_of_many_sequences(P):
+    """Workgroups that take several chunks each, counted over several groups of 64 sequences, long and empty ones."""
+    g = torch.Generator(device="cuda").manual_seed(P)
+    B, hq, hkv, d, smax = 331, 8, 4, 64, 530
+    lens = [(0, 530, 1, 256, 257, 0, 40)[(b * b + b // 64) % 7] if not 128 <= b < 200 else 0 for b in range(B)]
+    q, pk, pv = _rnd(g, B, hq, d), _rnd(g, hkv, P, d), _rnd(g, hkv, P, d)
+    kc, vc = _rnd(g, B, hkv, smax, d), _rnd(g, B, hkv, smax, d)
+    ln = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    att = dec.PrefixDecodeAttention(B, hq, hkv, d, smax, P, "cuda")
+    for _ in range(2):
+        _within(att(q, pk, pv, kc, vc, ln), *_exact_prefix(q, pk, pv, kc, vc, ln), "o")
+        ln = ln.flip(0).contiguous()
+
+
 def test_prefix_attention_growing_scores_and_replays():
     g = torch.Generator(device="cuda").manual_seed(3)
     B, hq, hkv, d, smax, P = 20, 16, 4, 64, 600, 2000
