@@ -20,6 +20,22 @@
 // LDS by DMA, double buffered, one barrier per tile; a tile that straddles the
 // sequence's end is loaded with zeros past it, so what the next sequence (or
 // nothing) holds there never enters.
+//
+// Bounds, measured in bf16 with 32 / 8 heads: one sequence of 16,384 rows,
+// causal, D 128, runs at 1.11 PF/s forward (1.98 ms), 1.25 in dQ (2.64 ms) and
+// 1.12 in dK / dV (3.91 ms), a plain matrix product of 8,192^3 at 1.37; the
+// clock is then down to 1.77 GHz at the card's power limit (operands of zeros
+// run 25 % faster), so fewer operations would help, a better schedule does
+// not.  At D 64 the softmax weighs twice as much: 32 exponentials and as many
+// multiply-adds per 16 matrix instructions: 0.94 PF/s at 8,000 rows.  Ragged batches
+// lose to blocks of few rows and to the last workgroups (24 documents of 64 to
+// 4,096 rows: 0.25 + 0.35 + 0.39 ms, 599 TF/s over all three).
+//
+// Tried and slower: 8 waves and 256 rows per tile (documents 210 -> 235 us),
+// two workgroup halves on alternate tiles (32 prompts of 16 to 1,024 rows, D
+// 64: 39.8 -> 46.8 us, though 46.5 -> 42 for a single one of 2,000), the next
+// tile's S product under this tile's exponentials (40.7 -> 43.3 us: registers),
+// row sums as dot products of the packed pairs (1.98 -> 2.01 ms).
 #include "attn_tile.h"
 
 using namespace kgwe;
@@ -252,7 +268,9 @@ struct BwdArgs {
 };
 
 // dQ: the forward's geometry (query on the lane).  Recomputes S^T and dP^T and
-// accumulates dQ^T += K^T dS^T, K^T read transposed from the K image.
+// accumulates dQ^T += K^T dS^T, K^T read transposed from the K image.  dQ and
+// dK / dV are two kernels, 7 products where one kernel would need 5: that one
+// would have to add dQ up by atomics, in an order that changes from run to run.
 template <class T, int D>
 __global__ __launch_bounds__(256, 2) void packed_dq_kernel(BwdArgs a) {
   constexpr int NB = D / 32, NT = D / 16;
