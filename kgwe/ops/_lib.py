@@ -164,26 +164,37 @@ def check(rc: int, what: str) -> None:
 HALF_TYPES = {torch.bfloat16: 0, torch.float16: 1}
 
 
+_FAR = 1 << 22  # elements between rows that the kernels' 32-bit offsets inside a tile of rows reach
+
+
 def rows16(t: torch.Tensor) -> torch.Tensor:
     """t (2 or 3 dimensions) itself where its last dimension is dense and every row starts on 16
-    bytes (what the strided kernels read), else a contiguous copy."""
+    bytes, behind the one before and not too far from it (what the strided kernels read), else a
+    contiguous copy."""
     s = t.stride()
-    if s[-1] == 1 and not t.data_ptr() & 15 and not (s[0] | s[-2]) & 7 and len(s) <= 3:
+    if s[-1] == 1 and not t.data_ptr() & 15 and not (s[0] | s[-2]) & 7 and t.shape[-1] <= s[-2] <= _FAR:
         return t
-    return dense16(t)
+    return _plain_strides(dense16(t))
 
 
 def token_view(t: torch.Tensor) -> tuple:
     """(tensor, address, row stride, head stride) of [T, H, D] as the strided
-    kernels read it: t itself where its last dimension is dense, every row
-    starts on 16 bytes and the row stride fits the kernels' 32-bit offsets
-    inside a tile of rows, else a contiguous copy."""
+    kernels read it: t itself where its last dimension is dense and every row
+    starts on 16 bytes, behind the one before (a row stride of 0 is a broadcast
+    input) and no further than the kernels' 32-bit offsets reach, else a
+    contiguous copy."""
     s0, s1, s2 = t.stride()
     at = t.data_ptr()
-    if s2 != 1 or (s0 | s1) & 7 or at & 15 or s0 > 1 << 22:
-        t = dense16(t.contiguous())
+    if s2 != 1 or (s0 | s1) & 7 or at & 15 or not t.shape[2] <= s0 <= _FAR:
+        t = _plain_strides(dense16(t))
         (s0, s1, _), at = t.stride(), t.data_ptr()
     return t, at, s0, s1
+
+
+def _plain_strides(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor with the strides of its shape (torch calls one
+    contiguous whatever the strides of its dimensions of size 1)."""
+    return t.view(-1).view(t.shape)
 
 
 def dense16(t: torch.Tensor) -> torch.Tensor:

@@ -253,7 +253,7 @@ class PrefixDecodeAttention:
         if not (q.shape == (B, hq, d) and pk.shape == pv.shape == (hkv, P, d) and kc.shape == vc.shape == (B, hkv, smax, d)):
             raise ValueError(f"prefix attention: q {(B, hq, d)}, prefix {(hkv, P, d)}, caches {(B, hkv, smax, d)}, got "
                              f"{[tuple(t.shape) for t in (q, pk, pv, kc, vc)]}")
-        _forward_only("prefix attention", q, pk, pv)
+        _forward_only("prefix attention", q, pk, pv, kc, vc)
         dtype, device = self.dtype, q.device
         if not (q.dtype == pk.dtype == pv.dtype == kc.dtype == vc.dtype == dtype and q.is_cuda == self.hip
                 and pk.device == pv.device == kc.device == vc.device == lens.device == device):
@@ -267,12 +267,12 @@ class PrefixDecodeAttention:
         q, pk, pv, lens = dense16(q), rows16(pk), rows16(pv), lens.contiguous()
         strides = pk.stride()
         if strides != pv.stride():  # one pair of strides for both
-            pk, pv = dense16(pk), dense16(pv)
-            strides = pk.stride()
+            pk, pv = pk.contiguous(), pv.contiguous()
+            strides = (P * d, d)
         out = torch.empty_like(q)
         work = torch.empty(self.words, device=device, dtype=torch.float32) if self.words else None
         launch("kgwe_prefix_attn", device, q.data_ptr(), pk.data_ptr(), pv.data_ptr(), kc.data_ptr(), vc.data_ptr(),
-               lens.data_ptr(), addr(work), out.data_ptr(), max(strides[1], d), strides[0], B, hq, hkv, d, P, smax,
+               lens.data_ptr(), addr(work), out.data_ptr(), strides[1], strides[0], B, hq, hkv, d, P, smax,
                HALF_TYPES[dtype], d ** -0.5)
         return out
 

@@ -511,9 +511,10 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(BwdArgs a) {
   store_row<T, NB>(a.dv + off, dva, 1.f, hh, ok);
 }
 
-// Strides fit the kernels' 32-bit offsets inside a tile of 128 rows.
-inline bool view_ok(const void* p, int64_t row, int64_t head) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && row % 8 == 0 && head % 8 == 0 && row >= 0 && head >= 0 &&
+// Strides fit the kernels' 32-bit offsets inside a tile of 128 rows, and rows
+// do not overlap: a descriptor's extent is counted in row strides.
+inline bool view_ok(const void* p, int64_t row, int64_t head, int D) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && row % 8 == 0 && head % 8 == 0 && row >= D && head >= 0 &&
          row <= (1 << 22);
 }
 
@@ -578,11 +579,11 @@ KGWE_API int kgwe_packed_attn_bwd_bytes() { return sizeof(PackedBwdCall); }
 
 KGWE_API int kgwe_packed_attn_fwd(const PackedFwdCall* c, hipStream_t s) {
   if (!shape_ok(c->T, c->J, c->Hq, c->Hkv, c->D, c->dtype) || c->P < 0 || !c->o || !c->jobs) return -1;
-  if (!view_ok(c->q, c->q_row, c->q_head) || !view_ok(c->k, c->k_row, c->k_head) ||
-      !view_ok(c->v, c->v_row, c->v_head))
+  if (!view_ok(c->q, c->q_row, c->q_head, c->D) || !view_ok(c->k, c->k_row, c->k_head, c->D) ||
+      !view_ok(c->v, c->v_row, c->v_head, c->D))
     return -1;
-  if (c->P > 0 && (!c->pk || !c->pv || !view_ok(c->pk, c->pk_row, c->pk_head) ||
-                   !view_ok(c->pv, c->pv_row, c->pv_head)))
+  if (c->P > 0 && (!c->pk || !c->pv || !view_ok(c->pk, c->pk_row, c->pk_head, c->D) ||
+                   !view_ok(c->pv, c->pv_row, c->pv_head, c->D)))
     return -1;
   if ((reinterpret_cast<uintptr_t>(c->o) | reinterpret_cast<uintptr_t>(c->o_low) |
        reinterpret_cast<uintptr_t>(c->jobs)) & 15)
@@ -598,8 +599,8 @@ KGWE_API int kgwe_packed_attn_fwd(const PackedFwdCall* c, hipStream_t s) {
 
 KGWE_API int kgwe_packed_attn_bwd(const PackedBwdCall* c, hipStream_t s) {
   if (!shape_ok(c->T, c->J, c->Hq, c->Hkv, c->D, c->dtype) || !c->lse || !c->delta || !c->jobs) return -1;
-  if (!view_ok(c->q, c->q_row, c->q_head) || !view_ok(c->k, c->k_row, c->k_head) ||
-      !view_ok(c->v, c->v_row, c->v_head))
+  if (!view_ok(c->q, c->q_row, c->q_head, c->D) || !view_ok(c->k, c->k_row, c->k_head, c->D) ||
+      !view_ok(c->v, c->v_row, c->v_head, c->D))
     return -1;
   for (const void* p : {c->o, c->o_low, c->dout, static_cast<const void*>(c->dq), static_cast<const void*>(c->dk),
                         static_cast<const void*>(c->dv), static_cast<const void*>(c->jobs)})

@@ -157,6 +157,48 @@ def test_packed_attention_behind_a_prefix(P, d, dtype, causal):
     assert torch.equal(none, attention_packed(q, k, v, PackedBatch(lengths, total=T), causal=causal))
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_broadcast_rows_and_single_rows(d):
+    """Inputs whose rows are one row (stride 0), overlap, or lie alone in a row of odd width."""
+    g = torch.Generator(device="cuda").manual_seed(d)
+    lengths, hq, hkv = [3, 130], 4, 2
+    T, batch = sum(lengths), PackedBatch(lengths)
+    q1, k1, v1 = _rnd(g, 1, hq, d), _rnd(g, 1, hkv, d), _rnd(g, T, 1, d)
+    do = _rnd(g, T, hq, d)
+    leaves = [t.requires_grad_(True) for t in (q1, k1, v1)]
+
+    def call(make):
+        x = [make(t.expand(T, h, d)) for t, h in zip(leaves, (hq, hkv, hkv))]
+        o = attention_packed(*x, batch)
+        return o, *torch.autograd.grad(o, leaves, do)
+
+    for a, b in zip(call(lambda t: t), call(lambda t: t.contiguous())):
+        assert torch.equal(a, b)
+    # a prefix of one row repeated, in both calls that take one
+    row, P = _rnd(g, hkv, 1, d), 70
+    pk = pv = row.expand(hkv, P, d)
+    with torch.no_grad():
+        q, k, v = (t.detach().expand(T, h, d).contiguous() for t, h in zip(leaves, (hq, hkv, hkv)))
+        assert torch.equal(attention_packed(q, k, v, batch, prefix=(pk, pv)),
+                           attention_packed(q, k, v, batch, prefix=(pk.contiguous(), pv.contiguous())))
+        kc, vc = _rnd(g, T, hkv, 16, d), _rnd(g, T, hkv, 16, d)
+        lens = torch.arange(T, device="cuda", dtype=torch.int32) % 17
+        for B in (3, T):
+            att = dec.PrefixDecodeAttention(B, hq, hkv, d, 16, P, "cuda")
+            args = kc[:B], vc[:B], lens[:B]
+            assert torch.equal(att(q[:B], pk, pv, *args), att(q[:B], pk.contiguous(), pv.contiguous(), *args))
+        # one row of a wider, odd buffer
+        wide = _rnd(g, 2, (hq + 2 * hkv) * d + 3)
+        one = wide[:1, :(hq + 2 * hkv) * d]
+        cos, sin = torch.rand(2, 8, d // 2, device="cuda").unbind()
+        pos = torch.tensor([5], dtype=torch.int32, device="cuda")
+        got = norm_rope_qkv(one, cos, sin, pos, hq, hkv, d)
+        for a, b in zip(got, norm_rope_qkv(one.clone(), cos, sin, pos, hq, hkv, d)):
+            assert torch.equal(a, b)
+        x = [one.view(1, -1, d)[:, i:i + h] for i, h in ((0, hq), (hq, hkv), (hq + hkv, hkv))]
+        assert torch.equal(attention_packed(*x, PackedBatch([1])), x[2].repeat_interleave(hq // hkv, 1))
+
+
 def test_neighbours_do_not_enter():
     """A sequence's outputs and gradients are its own: the same bits whatever the others hold, NaN included."""
     g = torch.Generator(device="cuda").manual_seed(5)

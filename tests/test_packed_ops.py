@@ -181,3 +181,30 @@ def test_prefix_attention_refusals():
                  (q.clone().requires_grad_(), p, p, c, c, lens)):
         with pytest.raises(ValueError):
             att(*args)
+
+
+def test_rows_that_the_kernels_read_in_place():
+    """What is passed on with its strides: dense rows from 16 bytes on, which do not overlap and lie no further apart
+    than the kernels' offsets reach; everything else is copied, and a copy has the strides of its shape."""
+    from kgwe.ops._lib import rows16, token_view
+
+    x = torch.randn(6, 4, 64, dtype=torch.bfloat16)
+    wide = torch.randn(6, 3 * 4 * 64, dtype=torch.bfloat16)
+    odd = torch.randn(6, 4 * 64 + 3, dtype=torch.bfloat16)
+    for t in (x, x.transpose(0, 1), x[:, :1].expand(6, 4, 64), wide[:, 256:512].view(6, 4, 64)):
+        got, at, row, head = token_view(t)
+        assert got is t and at == t.data_ptr() and (row, head) == t.stride()[:2]
+    overlapping = torch.randn(512, dtype=torch.bfloat16).as_strided((6, 4, 64), (8, 64, 1))
+    far = torch.randn((1 << 22) + 200, dtype=torch.bfloat16).as_strided((2, 2, 64), ((1 << 22) + 8, 64, 1))
+    for t in (x[:1].expand(6, 4, 64), overlapping, odd[:, :256].view(6, 4, 64), odd[:1, :256].view(1, 4, 64),
+              odd[:1, 3:259].view(1, 4, 64), far):
+        got, at, row, head = token_view(t)
+        assert torch.equal(got, t) and at == got.data_ptr() and at % 16 == 0
+        assert (row, head) == tuple(got.stride()[:2]) == (t.shape[1] * 64, 64)
+    for t in (x, x.transpose(0, 1), x[:1].expand(6, 4, 64), wide[:, :512], wide[:, :512][:1]):
+        assert rows16(t) is t
+    for t in (odd[:1, :256], odd[:, 8:264], wide[:1, :256].expand(6, 256), x[:, :1].expand(6, 4, 64),
+              x[0, :1].expand(4, 64)[None], overlapping.transpose(0, 1), far.transpose(0, 1)):
+        got = rows16(t)
+        assert torch.equal(got, t) and got.data_ptr() % 16 == 0 and got.is_contiguous()
+        assert got.stride() == torch.empty(t.shape).stride()
