@@ -78,6 +78,7 @@ _SIGS = {
     "kgwe_packed_plan_jobs": (c_int, [c_int, c_int]),
     "kgwe_packed_plan": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p,
                                  c_void_p]),
+    "kgwe_packed_attn_bwd_workspace": (c_int64, [c_int] * 5),
     "kgwe_prefix_attn_workspace": (c_int64, [c_int] * 6),
 }
 _OPTIONAL_SIGS = {
@@ -96,7 +97,7 @@ _OPTIONAL_SIGS = {
 # stands beside the entry): pointers, then int64, then int32, then fp32 fields.
 RECORDS = {name: struct.Struct(f"@{p}Q{q}q{i}i{f}f0q") for name, (p, q, i, f) in {
     "kgwe_packed_attn_fwd": (9, 10, 8, 1),
-    "kgwe_packed_attn_bwd": (12, 6, 7, 1),
+    "kgwe_packed_attn_bwd": (13, 6, 7, 1),
     "kgwe_norm_rope_fwd": (12, 1, 10, 1),
     "kgwe_norm_rope_bwd": (13, 1, 8, 1),
     "kgwe_prefix_attn": (8, 2, 7, 1),

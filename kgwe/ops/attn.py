@@ -140,9 +140,11 @@ class _PackedAttn(torch.autograd.Function):
         delta = torch.empty_like(lse)
         (qr, qh, _), (kr, kh, _), (vr, vh, _) = q.stride(), k.stride(), v.stride()
         jobs, slots = batch.tables
+        words = int(lib().kgwe_packed_attn_bwd_workspace(slots, T, Hq, Hkv, D))
+        work = torch.empty(words, device=q.device, dtype=torch.float32) if words else None
         launch("kgwe_packed_attn_bwd", q.device, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), low.data_ptr(),
-               lse.data_ptr(), do.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), jobs, qr, qh,
-               kr, kh, vr, vh, slots, T, Hq, Hkv, D, ctx.causal, HALF_TYPES[q.dtype], D ** -0.5)
+               lse.data_ptr(), do.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), addr(work),
+               jobs, qr, qh, kr, kh, vr, vh, slots, T, Hq, Hkv, D, ctx.causal, HALF_TYPES[q.dtype], D ** -0.5)
         return dq, dk, dv, None, None
 
 

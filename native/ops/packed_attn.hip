@@ -22,20 +22,22 @@
 // nothing) holds there never enters.
 //
 // Bounds, measured in bf16 with 32 / 8 heads: one sequence of 16,384 rows,
-// causal, D 128, runs at 1.11 PF/s forward (1.98 ms), 1.25 in dQ (2.64 ms) and
+// causal, D 128, runs at 1.16 PF/s forward (1.89 ms), 1.25 in dQ (2.64 ms) and
 // 1.12 in dK / dV (3.91 ms), a plain matrix product of 8,192^3 at 1.37; the
 // clock is then down to 1.77 GHz at the card's power limit (operands of zeros
 // run 25 % faster), so fewer operations would help, a better schedule does
 // not.  At D 64 the softmax weighs twice as much: 32 exponentials and as many
 // multiply-adds per 16 matrix instructions: 0.94 PF/s at 8,000 rows.  Ragged batches
 // lose to blocks of few rows and to the last workgroups (24 documents of 64 to
-// 4,096 rows: 0.25 + 0.35 + 0.39 ms, 599 TF/s over all three).
+// 4,096 rows: 0.23 + 0.34 + 0.39 ms, 610 TF/s over all three).
 //
 // Tried and slower: 8 waves and 256 rows per tile (documents 210 -> 235 us),
 // two workgroup halves on alternate tiles (32 prompts of 16 to 1,024 rows, D
 // 64: 39.8 -> 46.8 us, though 46.5 -> 42 for a single one of 2,000), the next
 // tile's S product under this tile's exponentials (40.7 -> 43.3 us: registers),
 // row sums as dot products of the packed pairs (1.98 -> 2.01 ms).
+#include <algorithm>
+
 #include "attn_tile.h"
 
 using namespace kgwe;
@@ -106,13 +108,18 @@ struct FwdArgs {
   float c;     // scale * log2 e
 };
 
-template <class T, int D, bool PREFIX>
-__global__ __launch_bounds__(256, 2) void packed_fwd_kernel(FwdArgs a) {
+// TWO_V: V tiles are double-buffered as K tiles are.  At D = 128 one V buffer
+// (V(t) is fetched during the tile's own scores, one more barrier) leaves room
+// for a third workgroup on the CU, which is worth more where there are
+// workgroups enough (see fwd()).
+template <class T, int D, bool PREFIX, bool TWO_V>
+__global__ __launch_bounds__(256, TWO_V ? 2 : 3) void packed_fwd_kernel(FwdArgs a) {
   constexpr int NB = D / 32, NT = D / 16;
   constexpr int kImg = kTile * D * 2;
   // One array per stage: the compiler orders an LDS read after every DMA in
   // flight that it cannot prove to go to another object.
-  __shared__ __attribute__((aligned(1024))) char K0[kImg], V0[kImg], K1[kImg], V1[kImg];
+  __shared__ __attribute__((aligned(1024))) char K0[kImg], V0[kImg], K1[kImg], V2[TWO_V ? kImg : 16];
+  char* const V1 = TWO_V ? V2 : V0;
   Job job;
   int h;
   if (!pick(a.b, a.b.Hq, a.b.by_hq, &job, &h)) return;
@@ -149,22 +156,28 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(FwdArgs a) {
   const u16* pkb = PREFIX ? a.pk.p + hkv * a.pk.head : nullptr;
   const u16* pvb = PREFIX ? a.pv.p + hkv * a.pv.head : nullptr;
 
-  auto load = [&](char* Kd, char* Vd, int t) {
+  auto load = [&](bool keys, char* dst, int t) {
     const bool pre = PREFIX && t < ntp;
     const int k0 = (pre ? t : t - ntp) * kTile;
     const int rows = min(kTile, (pre ? plen : klen) - k0);
-    const int64_t krow = pre ? a.pk.row : a.k.row, vrow = pre ? a.pv.row : a.v.row;
-    const int kbytes = static_cast<int>(2 * krow), vbytes = static_cast<int>(2 * vrow);
-    dma.load(row_buffer((pre ? pkb : kb) + k0 * krow, rows, kbytes), kbytes, Kd);
-    dma.load(row_buffer((pre ? pvb : vb) + k0 * vrow, rows, vbytes), vbytes, Vd);
+    const int64_t row = keys ? (pre ? a.pk.row : a.k.row) : (pre ? a.pv.row : a.v.row);
+    const u16* from = keys ? (pre ? pkb : kb) : (pre ? pvb : vb);
+    const int bytes = static_cast<int>(2 * row);
+    dma.load(row_buffer(from + k0 * row, rows, bytes), bytes, dst);
   };
 
   auto tile = [&](const char* Kc, const char* Vc, char* Kn, char* Vn, int t) {
-    if (t + 1 < nt) load(Kn, Vn, t + 1);  // lands during this tile's work
+    if constexpr (!TWO_V) load(false, Vn, t);
+    if (t + 1 < nt) {  // lands during this tile's work
+      load(true, Kn, t + 1);
+      if constexpr (TWO_V) load(false, Vn, t + 1);
+    }
     const bool pre = PREFIX && t < ntp;
     const int k0 = (pre ? t : t - ntp) * kTile;
     const bool causal = a.causal && !pre;
-    if (mine && (!causal || k0 <= q0 + 31)) {  // else: the tile is past this wave's diagonal
+    const bool sees = mine && (!causal || k0 <= q0 + 31);  // else: the tile is past this wave's diagonal
+    u32x4 pb[4];
+    if (sees) {
       // S^T = K Q^T: key on the accumulator's rows, query on the lane
       f32x16 s[2];
       s[0] = s[1] = f32x16{};
@@ -201,7 +214,6 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(FwdArgs a) {
       }
       m = m_new;
       // P = 2^(S c - m) in pairs; the accumulator tile is the next product's operand as it is
-      u32x4 pb[4];
       float r0 = 0.f, r1 = 0.f;
 #pragma unroll
       for (int st = 0; st < 2; ++st)
@@ -214,7 +226,13 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(FwdArgs a) {
           pb[2 * st + (r >> 3)][(r & 7) >> 1] = pack2<T>(p0, p1);
         }
       l += r0 + r1;  // this lane half's keys; the halves meet in the epilogue
-      // O^T += V^T P
+    }
+    if constexpr (!TWO_V) {  // V(t) has landed, K(t + 1) may be on its way
+      if (t + 1 < nt) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(TileDma<D, kTile>::kN) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+    }
+    if (sees) {  // O^T += V^T P
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -224,7 +242,8 @@ __global__ __launch_bounds__(256, 2) void packed_fwd_kernel(FwdArgs a) {
   };
 
   if (nt > 0) {
-    load(K0, V0, 0);
+    load(true, K0, 0);
+    if constexpr (TWO_V) load(false, V0, 0);
     // The Q loads end before the loop: sunk into it, they would make the
     // first products of every tile wait for the next tile's DMA.
 #pragma unroll
@@ -263,7 +282,9 @@ struct BwdArgs {
   u16* dq;            // [T, Hq, D]
   u16* dk;            // [T, Hkv, D]
   u16* dv;
-  int causal;
+  float* part;        // [2, parts, T, Hkv, D], dK's then dV's; parts > 1 only
+  int causal, parts, per;  // workgroups per key head, query heads of each
+  Div by_parts, by_hkv_parts;
   float c, scale;
 };
 
@@ -384,7 +405,9 @@ constexpr int kQt = 32;  // query rows per step of the dK / dV sweep
 // dK, dV: 128 keys of one sequence and key head, 32 per wave (key on the
 // lane), swept by every query head of the group and every query tile that sees
 // them, last tile first.  P and dS feed the next products as they are; Q and
-// dO are read by rows for S and dP and by columns for dV and dK.
+// dO are read by rows for S and dP and by columns for dV and dK.  Where that
+// would leave the chip short of workgroups, `parts` of them share a group's
+// query heads and their sums are joined by packed_join_kernel (see bwd()).
 template <class T, int D>
 __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(BwdArgs a) {
   constexpr int NB = D / 32, NT = D / 16;
@@ -394,8 +417,11 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(BwdArgs a) {
   __shared__ __attribute__((aligned(256))) float L0[64], L1[64];  // lse and -D of a tile's 32 rows
   Job job;
   int hkv;
-  if (!pick(a.b, a.b.Hkv, a.b.by_hkv, &job, &hkv)) return;
-  const int G = a.b.G;
+  if (!pick(a.b, a.b.Hkv * a.parts, a.by_hkv_parts, &job, &hkv)) return;
+  const int unit = hkv;
+  hkv = a.by_parts(unit);
+  const int part = unit - hkv * a.parts;
+  const int G = a.b.G, g_begin = part * a.per, g_end = min(G, g_begin + a.per);
   const int row0 = job.row0, len = job.rows;
   const int qlen = job.keys;  // nothing looks at padding
   const int nblk = (len + kRows - 1) / kRows;
@@ -428,7 +454,7 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(BwdArgs a) {
 
   const int nq = (qlen + kQt - 1) / kQt;
   const int first = a.causal ? kb * (kRows / kQt) : 0;
-  const int total = max(0, nq - first) * G;
+  const int total = max(0, nq - first) * (g_end - g_begin);
   auto load = [&](char* Qd, char* Od, float* Ld, int qt, int g) {
     const int h = hkv * G + g, s0 = qt * kQt, rows = min(kQt, qlen - s0);
     const int64_t r = static_cast<int64_t>(row0) + s0;
@@ -439,9 +465,10 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(BwdArgs a) {
       dma_lane<4>(row_buffer(src, rows, 4), 4 * lane, Ld + 32 * w);
     }
   };
-  int qt = nq - 1, g = 0;
+  int qt = nq - 1, g = g_begin;
   auto step = [&](const char* Qc, const char* Oc, const float* Lc, char* Qn, char* On, float* Ln, bool more) {
-    const int g2 = g + 1 == G ? 0 : g + 1, qt2 = g2 == 0 ? qt - 1 : qt;
+    const bool wrap = g + 1 == g_end;
+    const int g2 = wrap ? g_begin : g + 1, qt2 = wrap ? qt - 1 : qt;
     if (more) load(Qn, On, Ln, qt2, g2);
     const int qb = qt * kQt;
     if (key0 < len && (!a.causal || qb + kQt - 1 >= key0)) {  // else every query here precedes our keys
@@ -507,8 +534,49 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(BwdArgs a) {
     dma_join();  // the V image's DMA ends before the workgroup does
   }
   const int64_t off = (krow * a.b.Hkv + hkv) * D;
-  store_row<T, NB>(a.dk + off, dka, a.scale, hh, ok);
-  store_row<T, NB>(a.dv + off, dva, 1.f, hh, ok);
+  if (a.parts == 1) {
+    store_row<T, NB>(a.dk + off, dka, a.scale, hh, ok);
+    store_row<T, NB>(a.dv + off, dva, 1.f, hh, ok);
+  } else if (ok) {
+    const int64_t all = static_cast<int64_t>(a.b.T) * a.b.Hkv * D;
+    float* pk = a.part + part * all + off + 4 * hh;
+    float* pv = pk + a.parts * all;
+#pragma unroll
+    for (int db = 0; db < NB; ++db)
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4) {
+        f32x4 x, y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          x[j] = dka[db][4 * g4 + j];
+          y[j] = dva[db][4 * g4 + j];
+        }
+        *reinterpret_cast<f32x4*>(pk + 32 * db + 8 * g4) = x;
+        *reinterpret_cast<f32x4*>(pv + 32 * db + 8 * g4) = y;
+      }
+  }
+}
+
+// dK (y = 0) and dV (y = 1) of the parts' sums, in the parts' order; `all`
+// elements of each.
+template <class T>
+__global__ __launch_bounds__(256) void packed_join_kernel(const float* __restrict__ part, int parts, int64_t all,
+                                                          u16* dk, u16* dv, float scale) {
+  const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8;
+  if (i >= all) return;
+  const float* p = part + blockIdx.y * parts * all + i;
+  f32x4 lo = {}, hi = {};
+  for (int j = 0; j < parts; ++j, p += all) {
+    lo += *reinterpret_cast<const f32x4*>(p);
+    hi += *reinterpret_cast<const f32x4*>(p + 4);
+  }
+  const float mul = blockIdx.y == 0 ? scale : 1.f;
+  u32x4 v;
+  v[0] = pack2<T>(lo[0] * mul, lo[1] * mul);
+  v[1] = pack2<T>(lo[2] * mul, lo[3] * mul);
+  v[2] = pack2<T>(hi[0] * mul, hi[1] * mul);
+  v[3] = pack2<T>(hi[2] * mul, hi[3] * mul);
+  *reinterpret_cast<u32x4*>((blockIdx.y == 0 ? dk : dv) + i) = v;
 }
 
 // Strides fit the kernels' 32-bit offsets inside a tile of 128 rows, and rows
@@ -525,20 +593,53 @@ inline bool shape_ok(int T, int J, int Hq, int Hkv, int D, int dtype) {
          static_cast<int64_t>(Hq) * D < (1 << 22);
 }
 
+template <class T, int D, bool TWO_V>
+int fwd_as(const FwdArgs& a, int J, hipStream_t s) {
+  const dim3 grid(static_cast<unsigned>(J) * a.b.Hq);
+  if (a.P > 0) hipLaunchKernelGGL((packed_fwd_kernel<T, D, true, TWO_V>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((packed_fwd_kernel<T, D, false, TWO_V>), grid, dim3(256), 0, s, a);
+  return KGWE_CHECK_LAUNCH();
+}
+
+// At D = 64 four workgroups fit a CU with two V buffers.  At D = 128 two do,
+// three with one V buffer: taken from 2.5 workgroups a CU on (32 heads, bf16,
+// two against one buffer: 16,384 rows 1.96 / 1.89 ms, 4,000 rows 140 / 132 us,
+// 16 short prompts behind 3,000 shared keys 146 / 119 us; below, 2,000 rows
+// 47.4 / 49.7 us, 500 rows 13.4 / 14.6 us).
 template <class T, int D>
 int fwd(const FwdArgs& a, int J, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>(J) * a.b.Hq);
-  if (a.P > 0) hipLaunchKernelGGL((packed_fwd_kernel<T, D, true>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((packed_fwd_kernel<T, D, false>), grid, dim3(256), 0, s, a);
-  return KGWE_CHECK_LAUNCH();
+  if constexpr (D == 128) {
+    if (static_cast<int64_t>(J) * a.b.Hq >= 640) return fwd_as<T, D, false>(a, J, s);
+  }
+  return fwd_as<T, D, true>(a, J, s);
 }
 
 template <class T, int D>
 int bwd(const BwdArgs& a, int J, hipStream_t s) {
   hipLaunchKernelGGL((packed_dq_kernel<T, D>), dim3(static_cast<unsigned>(J) * a.b.Hq), dim3(256), 0, s, a);
   if (int rc = KGWE_CHECK_LAUNCH()) return rc;
-  hipLaunchKernelGGL((packed_dkv_kernel<T, D>), dim3(static_cast<unsigned>(J) * a.b.Hkv), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((packed_dkv_kernel<T, D>), dim3(static_cast<unsigned>(J) * a.b.Hkv * a.parts), dim3(256), 0, s, a);
+  int rc = KGWE_CHECK_LAUNCH();
+  if (rc || a.parts == 1) return rc;
+  const int64_t all = static_cast<int64_t>(a.b.T) * a.b.Hkv * D;
+  hipLaunchKernelGGL((packed_join_kernel<T>), dim3(static_cast<unsigned>((all / 8 + 255) / 256), 2), dim3(256), 0, s,
+                     a.part, a.parts, all, a.dk, a.dv, a.scale);
   return KGWE_CHECK_LAUNCH();
+}
+
+// Workgroups per key head of the dK / dV kernel: the query heads of a group are
+// shared out until there are 4 workgroups a CU (two run at a time, and their
+// sweeps differ in length).  What the parts cost is fp32 sums, written and read
+// once.  Forward + gradient, 32 / 8 heads x 128, without and with: 500 rows 105
+// / 70 us, 2,000 rows 371 / 220 us, 4,096 rows 856 / 643 us, 8,192 rows 2.51 /
+// 2.27 ms; 4,000 rows of 14 / 2 heads 1,057 / 363 us.  Up to 8 workgroups a CU:
+// 16,384 rows 8.69 / 8.44 ms, but 8 documents of 500 to 2,000 rows 632 / 693 us.
+constexpr int kFill = 1024;
+inline int dkv_parts(int J, int Hkv, int G) {
+  const int64_t have = static_cast<int64_t>(J) * Hkv;
+  const int want = static_cast<int>(std::min<int64_t>(G, (kFill + have - 1) / have));
+  const int per = (G + want - 1) / want;
+  return (G + per - 1) / per;
 }
 
 }  // namespace
@@ -568,6 +669,7 @@ struct PackedBwdCall {
   const void* dout;        // contiguous [T, Hq, D]
   float* delta;            // [Hq, T] workspace
   void *dq, *dk, *dv;      // [T, Hq, D], [T, Hkv, D]: contiguous, every row written
+  float* work;             // kgwe_packed_attn_bwd_workspace words
   const int* jobs;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;
   int J, T, Hq, Hkv, D, causal, dtype;
@@ -576,6 +678,13 @@ struct PackedBwdCall {
 
 KGWE_API int kgwe_packed_attn_fwd_bytes() { return sizeof(PackedFwdCall); }
 KGWE_API int kgwe_packed_attn_bwd_bytes() { return sizeof(PackedBwdCall); }
+
+// fp32 words of workspace that a gradient needs besides delta; 0: none.
+KGWE_API int64_t kgwe_packed_attn_bwd_workspace(int J, int T, int Hq, int Hkv, int D) {
+  if (!shape_ok(T, J, Hq, Hkv, D, kTypeBf16)) return 0;  // refused by the call itself
+  const int parts = dkv_parts(J, Hkv, Hq / Hkv);
+  return parts == 1 ? 0 : 2 * static_cast<int64_t>(parts) * T * Hkv * D;
+}
 
 KGWE_API int kgwe_packed_attn_fwd(const PackedFwdCall* c, hipStream_t s) {
   if (!shape_ok(c->T, c->J, c->Hq, c->Hkv, c->D, c->dtype) || c->P < 0 || !c->o || !c->jobs) return -1;
@@ -605,11 +714,14 @@ KGWE_API int kgwe_packed_attn_bwd(const PackedBwdCall* c, hipStream_t s) {
   for (const void* p : {c->o, c->o_low, c->dout, static_cast<const void*>(c->dq), static_cast<const void*>(c->dk),
                         static_cast<const void*>(c->dv), static_cast<const void*>(c->jobs)})
     if (!p || (reinterpret_cast<uintptr_t>(p) & 15)) return -1;
+  const int G = c->Hq / c->Hkv, parts = dkv_parts(c->J, c->Hkv, G);
+  if (parts > 1 && (!c->work || (reinterpret_cast<uintptr_t>(c->work) & 15))) return -2;
   auto in = [](const void* p) { return static_cast<const u16*>(p); };
   const BwdArgs a{batch_of(c->jobs, c->T, c->Hq, c->Hkv),
                   {in(c->q), c->q_row, c->q_head}, {in(c->k), c->k_row, c->k_head}, {in(c->v), c->v_row, c->v_head},
                   in(c->o), in(c->o_low), in(c->dout), c->lse, c->delta, static_cast<u16*>(c->dq),
-                  static_cast<u16*>(c->dk), static_cast<u16*>(c->dv), c->causal, c->scale * kLog2e, c->scale};
+                  static_cast<u16*>(c->dk), static_cast<u16*>(c->dv), c->work, c->causal, parts,
+                  (G + parts - 1) / parts, Div(parts), Div(c->Hkv * parts), c->scale * kLog2e, c->scale};
   if (c->dtype == kTypeBf16) return c->D == 64 ? bwd<Bf16, 64>(a, c->J, s) : bwd<Bf16, 128>(a, c->J, s);
   return c->D == 64 ? bwd<Fp16, 64>(a, c->J, s) : bwd<Fp16, 128>(a, c->J, s);
 }

@@ -139,6 +139,28 @@ def test_packed_attention_and_gradient(lengths, pad, hq, hkv, d, causal, dtype):
         _within(got, *exact[name], name)
 
 
+@pytest.mark.parametrize("hq,hkv", [(32, 16), (21, 3)])  # no join of dK / dV; four parts, the last of one head
+@pytest.mark.parametrize("d,dtype,causal", [(128, torch.bfloat16, True), (128, torch.float16, False),
+                                            (64, torch.float16, True)])
+def test_packed_attention_and_gradient_of_many_blocks(hq, hkv, d, dtype, causal):
+    """Workgroups enough for every CU: at D = 128 the form with one V buffer."""
+    g = torch.Generator(device="cuda").manual_seed(hq + d)
+    lengths, pad = [20] * 30 + [300, 0, 150] + [1, 33] * 14, 7
+    T = sum(lengths) + pad
+    q, k, v = (_rnd(g, T, h, d, dtype=dtype).requires_grad_(True) for h in (hq, hkv, hkv))
+    do = _rnd(g, T, hq, d, dtype=dtype)
+    o = attention_packed(q, k, v, PackedBatch(lengths, total=T), causal=causal)
+    grads = torch.autograd.grad(o, (q, k, v), do)
+    want, tol, exact = _exact_attention(q, k, v, lengths, causal, do=do)
+    _within(o, want, tol, "o")
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        _within(got, *exact[name], name)
+    prefix = _rnd(g, hkv, 150, d, dtype=dtype), _rnd(g, hkv, 150, d, dtype=dtype)
+    with torch.no_grad():
+        o = attention_packed(q, k, v, PackedBatch(lengths, total=T), causal=causal, prefix=prefix)
+    _within(o, *_exact_attention(q, k, v, lengths, causal, prefix=prefix), "o")
+
+
 @pytest.mark.parametrize("P", [1, 63, 64, 200])
 @pytest.mark.parametrize("d,dtype", [(64, torch.bfloat16), (128, torch.float16), (128, torch.bfloat16)])
 @pytest.mark.parametrize("causal", [True, False])
