@@ -354,6 +354,39 @@ def test_captured_with_its_plan_and_replayed():
             assert torch.equal(out, attention_packed(q, k, v, PackedBatch(lengths, total=T))), new
 
 
+def test_gradients_captured_and_replayed():
+    """Rotation, attention and both gradients in one graph; every replay gives the eager call's bits."""
+    g = torch.Generator(device="cuda").manual_seed(10)
+    T, hq, hkv, d = 300, 8, 2, 128
+    x, w = _rnd(g, T, (hq + 2 * hkv) * d), [_rnd(g, d) for _ in range(2)]
+    cos, sin = torch.rand(2, T, d // 2, device="cuda", generator=g).unbind()
+    do, batch = _rnd(g, T, hq, d), PackedBatch([100, 3, 190], total=T)
+    leaves = [t.requires_grad_(True) for t in (x, *w)]
+
+    def call():
+        q, k, v = norm_rope_qkv(x, cos, sin, batch.positions, hq, hkv, d, *w)
+        o = attention_packed(q, k, v, batch)
+        return [o.detach(), *torch.autograd.grad(o, leaves, do)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = call()
+    for _ in range(4):
+        with torch.no_grad():
+            x.copy_(_rnd(g, *x.shape))
+            do.copy_(_rnd(g, *do.shape))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, call()):
+            assert torch.equal(a, b)
+
+
 def test_packed_attention_gpu_refusals():
     b = PackedBatch([4])
     q = torch.zeros(4, 2, 64, device="cuda")
