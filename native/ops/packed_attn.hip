@@ -22,20 +22,23 @@
 // nothing) holds there never enters.
 //
 // Bounds, measured in bf16 with 32 / 8 heads: one sequence of 16,384 rows,
-// causal, D 128, runs at 1.16 PF/s forward (1.89 ms), 1.25 in dQ (2.64 ms) and
-// 1.12 in dK / dV (3.91 ms), a plain matrix product of 8,192^3 at 1.37; the
+// causal, D 128, runs at 1.16 PF/s forward (1.90 ms), 1.24 in dQ (2.65 ms) and
+// 1.11 in dK / dV (3.95 ms), a plain matrix product of 8,192^3 at 1.37; the
 // clock is then down to 1.77 GHz at the card's power limit (operands of zeros
 // run 25 % faster), so fewer operations would help, a better schedule does
 // not.  At D 64 the softmax weighs twice as much: 32 exponentials and as many
 // multiply-adds per 16 matrix instructions: 0.94 PF/s at 8,000 rows.  Ragged batches
 // lose to blocks of few rows and to the last workgroups (24 documents of 64 to
-// 4,096 rows: 0.23 + 0.34 + 0.39 ms, 610 TF/s over all three).
+// 4,096 rows: 0.23 + 0.35 + 0.39 ms, 618 TF/s over all three).
 //
 // Tried and slower: 8 waves and 256 rows per tile (documents 210 -> 235 us),
 // two workgroup halves on alternate tiles (32 prompts of 16 to 1,024 rows, D
 // 64: 39.8 -> 46.8 us, though 46.5 -> 42 for a single one of 2,000), the next
 // tile's S product under this tile's exponentials (40.7 -> 43.3 us: registers),
-// row sums as dot products of the packed pairs (1.98 -> 2.01 ms).
+// row sums as dot products of the packed pairs (1.98 -> 2.01 ms), 64 rows per
+// wave for half the LDS reads (1.91 -> 2.37 ms), tiles of 32 keys (D 64: 33.9 ->
+// 39 us for 16 short prompts behind 1,000 shared keys), an L2 prefetch two
+// steps ahead in dK / dV (8.57 -> 8.82 ms, all three kernels).
 #include <algorithm>
 
 #include "attn_tile.h"
