@@ -405,8 +405,9 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(Args a) {
 // hold keys.  W waves share a row; wave w of them takes every W-th slot, lane i
 // of it the (max, sum) of the i-th of those.  Few rows have many slots and want
 // 4 waves each (1 row x 32 heads, 66 slots: 21.2 -> 16.5 us with the launch
-// before it), many rows one (32 x 32 heads, 12 slots: 12.2 -> 10.7 us).  The
-// first loads of a wave are issued before anything is known of n: what lies
+// before it), many rows one (32 x 32 heads, 12 slots: 12.2 -> 10.7 us), unless
+// 32 slots give each of 4 waves its 8 loads at once (60 x 8 heads, 34 slots:
+// 25.9 -> 24.3 us).  The first loads of a wave are issued before anything is known of n: what lies
 // past it is the workspace's own memory, and is dropped by selection.
 template <class T, int D, int W>
 __global__ __launch_bounds__(256) void prefix_join_kernel(Args a) {
@@ -532,8 +533,10 @@ int launch(Args a, hipStream_t s) {
   int rc = KGWE_CHECK_LAUNCH();
   if (rc || a.direct || a.p_splits + a.o_splits == 1) return rc;
   const int n = a.B * a.Hq;
-  if (n <= 256) hipLaunchKernelGGL((prefix_join_kernel<T, D, 4>), dim3(n), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((prefix_join_kernel<T, D, 1>), dim3((n + 3) / 4), dim3(256), 0, s, a);
+  if (n <= 256 || (n <= 1024 && a.p_splits + a.o_splits >= 32))
+    hipLaunchKernelGGL((prefix_join_kernel<T, D, 4>), dim3(n), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((prefix_join_kernel<T, D, 1>), dim3((n + 3) / 4), dim3(256), 0, s, a);
   return KGWE_CHECK_LAUNCH();
 }
 

@@ -565,7 +565,8 @@ def _exact_prefix(q, pk, pv, kc, vc, lens):
     (4, 8, 2, 64, 700, 129, [1, 700, 256, 0]), (2, 14, 2, 128, 64, 1000, [64, 3]),  # at most 32 rows a key head
     (40, 8, 4, 128, 300, 515, [0, 300, 257, 256] * 10), (33, 4, 4, 64, 16, 4000, [16, 0, 5] * 11),
     (70, 12, 4, 64, 260, 1030, [260, 1] * 35), (9, 32, 1, 128, 600, 300, [600, 0, 1] * 3),  # row tiles of 128
-    (3, 4, 4, 64, 900, 0, [0, 900, 5]), (5, 64, 8, 64, 0, 600, [0] * 5), (2, 4, 4, 128, 0, 9, [0, 0]),
+    (3, 4, 4, 64, 900, 0, [0, 900, 5]), (40, 8, 8, 64, 1000, 9000, [1000, 0, 3, 700] * 10),
+    (5, 64, 8, 64, 0, 600, [0] * 5), (2, 4, 4, 128, 0, 9, [0, 0]),
 ])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_prefix_attention(B, hq, hkv, d, smax, P, lens, dtype):
