@@ -32,9 +32,9 @@
 // 4,096 rows: 0.23 + 0.35 + 0.39 ms, 618 TF/s over all three).
 //
 // Tried and slower: 8 waves and 256 rows per tile (documents 210 -> 235 us),
-// two workgroup halves on alternate tiles (32 prompts of 16 to 1,024 rows, D
-// 64: 39.8 -> 46.8 us, though 46.5 -> 42 for a single one of 2,000), the next
-// tile's S product under this tile's exponentials (40.7 -> 43.3 us: registers),
+// two workgroup halves on alternate tiles where there are workgroups enough (32
+// prompts of 16 to 1,024 rows, D 64: 39.8 -> 46.8 us), the next tile's S product
+// under this tile's exponentials (40.7 -> 43.3 us: registers),
 // row sums as dot products of the packed pairs (1.98 -> 2.01 ms), 64 rows per
 // wave for half the LDS reads (1.91 -> 2.37 ms), tiles of 32 keys (D 64: 33.9 ->
 // 39 us for 16 short prompts behind 1,000 shared keys), an L2 prefetch two
@@ -115,18 +115,22 @@ struct FwdArgs {
 // (V(t) is fetched during the tile's own scores, one more barrier) leaves room
 // for a third workgroup on the CU, which is worth more where there are
 // workgroups enough (see fwd()).
-template <class T, int D, bool PREFIX, bool TWO_V>
-__global__ __launch_bounds__(256, TWO_V ? 2 : 3) void packed_fwd_kernel(FwdArgs a) {
+// HALVES = 2: 8 waves, of which the second four walk every other tile of the
+// same rows; the halves' states meet in LDS at the end.
+template <class T, int D, bool PREFIX, bool TWO_V, int HALVES>
+__global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 1 : TWO_V ? 2 : 3) void packed_fwd_kernel(FwdArgs a) {
   constexpr int NB = D / 32, NT = D / 16;
   constexpr int kImg = kTile * D * 2;
   // One array per stage: the compiler orders an LDS read after every DMA in
   // flight that it cannot prove to go to another object.
-  __shared__ __attribute__((aligned(1024))) char K0[kImg], V0[kImg], K1[kImg], V2[TWO_V ? kImg : 16];
+  constexpr int kStage = HALVES * kImg;
+  __shared__ __attribute__((aligned(1024))) char K0[kStage], V0[kStage], K1[kStage], V2[TWO_V ? kStage : 16];
   char* const V1 = TWO_V ? V2 : V0;
   Job job;
   int h;
   if (!pick(a.b, a.b.Hq, a.b.by_hq, &job, &h)) return;
-  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int w8 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int w = w8 & 3, half = HALVES == 1 ? 0 : w8 >> 2;  // row group, key half
   const int hkv = a.b.by_g(h), q0 = wave_rows(a.b, job, w, &h);
   if (q0 < 0) return;
   const int row0 = job.row0, len = job.rows, blk = job.blk;
@@ -169,16 +173,19 @@ __global__ __launch_bounds__(256, TWO_V ? 2 : 3) void packed_fwd_kernel(FwdArgs 
     dma.load(row_buffer(from + k0 * row, rows, bytes), bytes, dst);
   };
 
-  auto tile = [&](const char* Kc, const char* Vc, char* Kn, char* Vn, int t) {
+  const int mine_at = half * kImg;  // this half's tile of a stage
+  auto tile = [&](const char* Ks, const char* Vs, char* Kn, char* Vn, int t) {
+    const char *Kc = Ks + mine_at, *Vc = Vs + mine_at;
     if constexpr (!TWO_V) load(false, Vn, t);
-    if (t + 1 < nt) {  // lands during this tile's work
-      load(true, Kn, t + 1);
-      if constexpr (TWO_V) load(false, Vn, t + 1);
+    if (t + HALVES < nt) {  // lands during this tile's work
+      load(true, Kn + mine_at, t + HALVES);
+      if constexpr (TWO_V) load(false, Vn + mine_at, t + HALVES);
     }
     const bool pre = PREFIX && t < ntp;
     const int k0 = (pre ? t : t - ntp) * kTile;
     const bool causal = a.causal && !pre;
-    const bool sees = mine && (!causal || k0 <= q0 + 31);  // else: the tile is past this wave's diagonal
+    // else: the tile is past this wave's diagonal, or the other half had the last one
+    const bool sees = mine && (HALVES == 1 || t < nt) && (!causal || k0 <= q0 + 31);
     u32x4 pb[4];
     if (sees) {
       // S^T = K Q^T: key on the accumulator's rows, query on the lane
@@ -245,17 +252,50 @@ __global__ __launch_bounds__(256, TWO_V ? 2 : 3) void packed_fwd_kernel(FwdArgs 
   };
 
   if (nt > 0) {
-    load(true, K0, 0);
-    if constexpr (TWO_V) load(false, V0, 0);
+    if (half < nt) {
+      load(true, K0 + mine_at, half);
+      if constexpr (TWO_V) load(false, V0 + mine_at, half);
+    }
     // The Q loads end before the loop: sunk into it, they would make the
     // first products of every tile wait for the next tile's DMA.
 #pragma unroll
     for (int t = 0; t < NT; ++t) asm volatile("" ::"v"(qf[t]));
     dma_join();
-    for (int t = 0; t < nt; t += 2) {
-      tile(K0, V0, K1, V1, t);
-      if (t + 1 < nt) tile(K1, V1, K0, V0, t + 1);
+    for (int t = 0; t < nt; t += 2 * HALVES) {
+      tile(K0, V0, K1, V1, t + half);
+      if (t + HALVES < nt) tile(K1, V1, K0, V0, t + HALVES + half);
     }
+  }
+  if constexpr (HALVES == 2) {
+    // The second half's state of each lane, lane after lane (every tile buffer
+    // is free: the last step ended with a barrier).
+    __shared__ float2 ml[4][64];
+    char* at = (w == 0 ? K0 : w == 1 ? V0 : w == 2 ? K1 : V1) + 16 * lane;
+    static_assert(NB * 4 * 1024 <= kStage, "a wave's state fits a stage buffer");
+    if (half == 1) {
+      ml[w][lane] = {m, l};
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(at + 1024 * (4 * i + g)) =
+              f32x4{oacc[i][4 * g], oacc[i][4 * g + 1], oacc[i][4 * g + 2], oacc[i][4 * g + 3]};
+    }
+    __syncthreads();
+    if (half == 1) return;
+    const float2 o = ml[w][lane];
+    const float M = fmaxf(m, o.x), M_use = M == -INFINITY ? 0.f : M;
+    const float f0 = exp2_fast(m - M_use), f1 = exp2_fast(o.x - M_use);
+    m = M;
+    l = l * f0 + o.y * f1;
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(at + 1024 * (4 * i + g));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) oacc[i][4 * g + j] = oacc[i][4 * g + j] * f0 + v[j] * f1;
+      }
   }
   const float lt = half_add(l);
   const bool ok = qrow < len;
@@ -596,25 +636,36 @@ inline bool shape_ok(int T, int J, int Hq, int Hkv, int D, int dtype) {
          static_cast<int64_t>(Hq) * D < (1 << 22);
 }
 
-template <class T, int D, bool TWO_V>
+template <class T, int D, bool TWO_V, int HALVES>
 int fwd_as(const FwdArgs& a, int J, hipStream_t s) {
-  const dim3 grid(static_cast<unsigned>(J) * a.b.Hq);
-  if (a.P > 0) hipLaunchKernelGGL((packed_fwd_kernel<T, D, true, TWO_V>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((packed_fwd_kernel<T, D, false, TWO_V>), grid, dim3(256), 0, s, a);
+  const dim3 grid(static_cast<unsigned>(J) * a.b.Hq), threads(256 * HALVES);
+  if (a.P > 0) hipLaunchKernelGGL((packed_fwd_kernel<T, D, true, TWO_V, HALVES>), grid, threads, 0, s, a);
+  else hipLaunchKernelGGL((packed_fwd_kernel<T, D, false, TWO_V, HALVES>), grid, threads, 0, s, a);
   return KGWE_CHECK_LAUNCH();
 }
 
-// At D = 64 four workgroups fit a CU with two V buffers.  At D = 128 two do,
-// three with one V buffer: taken from 2.5 workgroups a CU on (32 heads, bf16,
-// two against one buffer: 16,384 rows 1.96 / 1.89 ms, 4,000 rows 140 / 132 us,
-// 16 short prompts behind 3,000 shared keys 146 / 119 us; below, 2,000 rows
-// 47.4 / 49.7 us, 500 rows 13.4 / 14.6 us).
+// The form by the number of workgroups, 2.5 a CU being the border.
+//
+// Fewer: a workgroup's sweep is the call's time, so two halves share it where
+// it is long, by the sequences' mean length (32 heads, one against two halves:
+// 4 prompts of 20 to 200 rows behind 2,000 keys, D 64: 31.8 / 24.9 us, D 128:
+// 43.5 / 34.2; one prompt of 1,000 rows 15.9 / 13.7 and 23.1 / 20.7, of 2,000
+// 31.7 / 30.2 and 47.7 / 45.0; but 4 prompts of 200 to 800 rows 11.2 / 11.7 and
+// 16.7 / 19.1, 4 of 1 to 61 rows 4.1 / 4.8).
+//
+// More: at D = 64 four workgroups fit a CU with two V buffers.  At D = 128 two
+// do, three with one V buffer (two against one: 16,384 rows 1.96 / 1.89 ms,
+// 4,000 rows 140 / 132 us, 16 short prompts behind 3,000 shared keys 146 / 119
+// us; below the border 2,000 rows 47.4 / 49.7 us, 500 rows 13.4 / 14.6 us).
 template <class T, int D>
 int fwd(const FwdArgs& a, int J, hipStream_t s) {
-  if constexpr (D == 128) {
-    if (static_cast<int64_t>(J) * a.b.Hq >= 640) return fwd_as<T, D, false>(a, J, s);
+  if (static_cast<int64_t>(J) * a.b.Hq < 640) {
+    const int seqs = std::max(1, J - a.b.T / kRows - 1);  // how packed_plan.hip counts J
+    if (a.P + a.b.T / seqs >= 640) return fwd_as<T, D, true, 2>(a, J, s);
+  } else if (D == 128) {
+    return fwd_as<T, D, D != 128, 1>(a, J, s);
   }
-  return fwd_as<T, D, true>(a, J, s);
+  return fwd_as<T, D, true, 1>(a, J, s);
 }
 
 template <class T, int D>

@@ -252,6 +252,30 @@ def test_large_scores_and_growing_maximum():
     _within(o, *_exact_attention(q, k, v, [n], True), "o")
 
 
+@pytest.mark.parametrize("lengths,pad,P,hq,hkv,causal", [
+    ([700], 0, 0, 4, 1, True), ([1111], 3, 0, 3, 3, False), ([641, 640], 0, 0, 6, 2, True),
+    ([1, 130, 0, 64, 33], 2, 700, 8, 2, True), ([20], 0, 641, 4, 4, False), ([90], 0, 1000, 2, 1, True),
+])
+@pytest.mark.parametrize("d,dtype", [(64, torch.bfloat16), (128, torch.float16), (128, torch.bfloat16)])
+def test_long_sweeps_of_few_workgroups(lengths, pad, P, hq, hkv, causal, d, dtype):
+    """Sweeps that two halves of a workgroup share: odd and even tile counts, rows that see one half's tiles only."""
+    g = torch.Generator(device="cuda").manual_seed(P + hq)
+    T = sum(lengths) + pad
+    q, k, v = (_rnd(g, T, h, d, dtype=dtype) for h in (hq, hkv, hkv))
+    prefix = (_rnd(g, hkv, P, d, dtype=dtype), _rnd(g, hkv, P, d, dtype=dtype)) if P else None
+    o = attention_packed(q, k, v, PackedBatch(lengths, total=T), causal=causal, prefix=prefix)
+    _within(o, *_exact_attention(q, k, v, lengths, causal, prefix=prefix), "o")
+    if P == 0:
+        do = _rnd(g, T, hq, d, dtype=dtype)
+        for t in (q, k, v):
+            t.requires_grad_(True)
+        o = attention_packed(q, k, v, PackedBatch(lengths, total=T), causal=causal)
+        grads = torch.autograd.grad(o, (q, k, v), do)
+        exact = _exact_attention(q, k, v, lengths, causal, do=do)[2]
+        for name, got in zip(("dq", "dk", "dv"), grads):
+            _within(got, *exact[name], name)
+
+
 def test_gradient_matches_differences():
     g = torch.Generator(device="cuda").manual_seed(7)
     lengths, hq, hkv, d = [37, 80], 4, 2, 64
