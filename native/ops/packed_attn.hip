@@ -40,6 +40,7 @@
 // 39 us for 16 short prompts behind 1,000 shared keys), an L2 prefetch two
 // steps ahead in dK / dV (8.57 -> 8.82 ms, all three kernels).
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_tile.h"
 
@@ -48,6 +49,10 @@ using namespace kgwe;
 namespace {
 
 typedef unsigned short u16;
+// On a lambda that the compiler might call instead (a call keeps its captured
+// tiles in memory: 9 times the time).
+#define KGWE_INLINE __attribute__((always_inline))
+
 constexpr int kRows = 128;    // rows of a job (packed_plan.hip)
 constexpr int kTile = 64;     // keys per tile
 constexpr float kLog2e = 1.4426950408889634f;
@@ -331,6 +336,19 @@ struct BwdArgs {
   float c, scale;
 };
 
+// What the rounding of two values to the pair `w` dropped, rounded in turn.
+template <class T>
+__device__ __forceinline__ unsigned pack2_low(float lo, float hi, unsigned w) {
+  return pack2<T>(lo - T::up(static_cast<u16>(w)), hi - T::up(static_cast<u16>(w >> 16)));
+}
+
+// Sequences of up to this many rows.  A row of two or three keys has nothing
+// for the roundings to average out over: with dS as one 16-bit value and D from
+// an o whose P was rounded, dQ and dK were up to 1.8 times the rounding of the
+// result off there (1.45 times in longer sequences).  These few take D as the
+// sum of P dP, and dS as two 16-bit values.
+constexpr int kShort = kTile;
+
 // dQ: the forward's geometry (query on the lane).  Recomputes S^T and dP^T and
 // accumulates dQ^T += K^T dS^T, K^T read transposed from the K image.  dQ and
 // dK / dV are two kernels, 7 products where one kernel would need 5: that one
@@ -374,8 +392,7 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(BwdArgs a) {
   }
   const int64_t li = static_cast<int64_t>(h) * a.b.T + row;
   const float lse = ok ? a.lse[li] : 0.f;
-  const float delta = half_add(dsum);
-  if (hh == 0 && ok) a.delta[li] = -delta;
+  float delta = half_add(dsum);
   f32x16 acc[NB];
 #pragma unroll
   for (int i = 0; i < NB; ++i) acc[i] = f32x16{};
@@ -387,12 +404,23 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(BwdArgs a) {
   const u16* kb = a.k.p + static_cast<int64_t>(row0) * a.k.row + hkv * a.k.head;
   const u16* vb = a.v.p + static_cast<int64_t>(row0) * a.v.row + hkv * a.v.head;
   const int kbytes = static_cast<int>(2 * a.k.row), vbytes = static_cast<int>(2 * a.v.row);
-  auto load = [&](char* Kd, char* Vd, int t) {
+  auto load = [&](char* Kd, char* Vd, int t) KGWE_INLINE {
     const int k0 = t * kTile, rows = min(kTile, klen - k0);
     dma.load(row_buffer(kb + k0 * a.k.row, rows, kbytes), kbytes, Kd);
     dma.load(row_buffer(vb + k0 * a.v.row, rows, vbytes), vbytes, Vd);
   };
-  auto tile = [&](const char* Kc, const char* Vc, char* Kn, char* Vn, int t) {
+  // S^T and dP^T + d of 32 keys.
+  auto scores = [&](const char* Kc, const char* Vc, int st, float d, f32x16& s, f32x16& p) KGWE_INLINE {
+    s = f32x16{};
+#pragma unroll
+    for (int r = 0; r < 16; ++r) p[r] = d;  // dP - D without a subtraction
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      s = mfma32<T>(ad.rows(Kc, 32 * st, u), qf[u], s);
+      p = mfma32<T>(ad.rows(Vc, 32 * st, u), df[u], p);
+    }
+  };
+  auto tile = [&](auto brief_c, const char* Kc, const char* Vc, char* Kn, char* Vn, int t) KGWE_INLINE {
     if (t + 1 < nt) load(Kn, Vn, t + 1);
     const int k0 = t * kTile;
     if (mine && (!a.causal || k0 <= q0 + 31)) {
@@ -401,14 +429,8 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(BwdArgs a) {
       // Two 32-key halves in turn: one S^T / dP^T pair live at a time.
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
-        f32x16 s = f32x16{}, p;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) p[r] = -delta;  // dP - D without a subtraction
-#pragma unroll
-        for (int u = 0; u < NT; ++u) {
-          s = mfma32<T>(ad.rows(Kc, 32 * st, u), qf[u], s);
-          p = mfma32<T>(ad.rows(Vc, 32 * st, u), df[u], p);
-        }
+        f32x16 s, p;
+        scores(Kc, Vc, st, -delta, s, p);
 #pragma unroll
         for (int r = 0; r < 16; ++r) p[r] *= exp2_fast(fmaf(s[r], a.c, -lse));
         if (edge) {
@@ -424,6 +446,13 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(BwdArgs a) {
 #pragma unroll
           for (int db = 0; db < NB; ++db)
             acc[db] = mfma32<T>(ad.cols(Kc, 32 * st + 16 * u, db), as_op(sw), acc[db]);
+          if constexpr (brief_c.value) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sw[j] = pack2_low<T>(p[8 * u + 2 * j], p[8 * u + 2 * j + 1], sw[j]);
+#pragma unroll
+            for (int db = 0; db < NB; ++db)
+              acc[db] = mfma32<T>(ad.cols(Kc, 32 * st + 16 * u, db), as_op(sw), acc[db]);
+          }
         }
       }
     }
@@ -435,11 +464,29 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(BwdArgs a) {
     for (int t = 0; t < NT; ++t) asm volatile("" ::"v"(qf[t]), "v"(df[t]));
     asm volatile("" ::"v"(lse), "v"(delta));
     dma_join();
-    for (int t = 0; t < nt; t += 2) {
-      tile(K0, V0, K1, V1, t);
-      if (t + 1 < nt) tile(K1, V1, K0, V0, t + 1);
+    if (klen <= kShort) {  // one tile
+      if (mine) {
+        const int last = a.causal ? min(klen - 1, qrow) : klen - 1;
+        float d = 0.f;
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          f32x16 s, p;
+          scores(K0, V0, st, 0.f, s, p);
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (32 * st + tile_row(r, hh) <= last) d = fmaf(exp2_fast(fmaf(s[r], a.c, -lse)), p[r], d);
+        }
+        delta = half_add(d);
+      }
+      tile(std::true_type{}, K0, V0, K1, V1, 0);
+    } else {
+      for (int t = 0; t < nt; t += 2) {
+        tile(std::false_type{}, K0, V0, K1, V1, t);
+        if (t + 1 < nt) tile(std::false_type{}, K1, V1, K0, V0, t + 1);
+      }
     }
   }
+  if (hh == 0 && ok) a.delta[li] = -delta;
   store_row<T, NB>(a.dq + (row * a.b.Hq + h) * D, acc, a.scale, hh, ok);
 }
 
@@ -498,7 +545,7 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(BwdArgs a) {
   const int nq = (qlen + kQt - 1) / kQt;
   const int first = a.causal ? kb * (kRows / kQt) : 0;
   const int total = max(0, nq - first) * (g_end - g_begin);
-  auto load = [&](char* Qd, char* Od, float* Ld, int qt, int g) {
+  auto load = [&](char* Qd, char* Od, float* Ld, int qt, int g) KGWE_INLINE {
     const int h = hkv * G + g, s0 = qt * kQt, rows = min(kQt, qlen - s0);
     const int64_t r = static_cast<int64_t>(row0) + s0;
     dma.load(row_buffer(a.q.p + r * a.q.row + h * a.q.head, rows, qbytes), qbytes, Qd);
@@ -509,7 +556,8 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(BwdArgs a) {
     }
   };
   int qt = nq - 1, g = g_begin;
-  auto step = [&](const char* Qc, const char* Oc, const float* Lc, char* Qn, char* On, float* Ln, bool more) {
+  auto step = [&](auto brief_c, const char* Qc, const char* Oc, const float* Lc, char* Qn, char* On, float* Ln,
+                  bool more) KGWE_INLINE {
     const bool wrap = g + 1 == g_end;
     const int g2 = wrap ? g_begin : g + 1, qt2 = wrap ? qt - 1 : qt;
     if (more) load(Qn, On, Ln, qt2, g2);
@@ -558,6 +606,12 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(BwdArgs a) {
           dva[db] = mfma32<T>(ad.cols(Oc, 16 * u, db), as_op(pw), dva[db]);
           dka[db] = mfma32<T>(ad.cols(Qc, 16 * u, db), as_op(sw), dka[db]);
         }
+        if constexpr (brief_c.value) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sw[j] = pack2_low<T>(p[8 * u + 2 * j], p[8 * u + 2 * j + 1], sw[j]);
+#pragma unroll
+          for (int db = 0; db < NB; ++db) dka[db] = mfma32<T>(ad.cols(Qc, 16 * u, db), as_op(sw), dka[db]);
+        }
       }
     }
     dma_join();
@@ -569,10 +623,14 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(BwdArgs a) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) asm volatile("" ::"v"(kf[t]));
     dma_join();
-    for (int it = 0; it < total; it += 2) {
-      step(Q0, O0, L0, Q1, O1, L1, it + 1 < total);
-      if (it + 1 < total) step(Q1, O1, L1, Q0, O0, L0, it + 2 < total);
-    }
+    auto sweep = [&](auto brief_c) KGWE_INLINE {
+      for (int it = 0; it < total; it += 2) {
+        step(brief_c, Q0, O0, L0, Q1, O1, L1, it + 1 < total);
+        if (it + 1 < total) step(brief_c, Q1, O1, L1, Q0, O0, L0, it + 2 < total);
+      }
+    };
+    if (qlen <= kShort) sweep(std::true_type{});
+    else sweep(std::false_type{});
   } else {
     dma_join();  // the V image's DMA ends before the workgroup does
   }

@@ -276,6 +276,38 @@ def test_long_sweeps_of_few_workgroups(lengths, pad, P, hq, hkv, causal, d, dtyp
             _within(got, *exact[name], name)
 
 
+@pytest.mark.parametrize("n", [2, 3, 17, 64])
+@pytest.mark.parametrize("d,dtype", [(64, torch.bfloat16), (128, torch.bfloat16), (128, torch.float16)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_gradients_of_short_sequences_are_rounded_once(n, d, dtype, causal):
+    """dQ and dK of sequences of up to 64 rows: dS is two 16-bit values (h^2 of it is lost, or half an fp16 step) and D the sum of P dP in
+    fp32, so but for fp32's own roundings the error is that of the result, h."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    hq, hkv, reps = 6, 3, 5
+    lengths, h, tiny, sc = [n] * reps, HALF[dtype], TINY[dtype], 1 / math.sqrt(d)
+    q, k, v, do = (_rnd(g, n * reps, x, d, dtype=dtype) for x in (hq, hkv, hkv, hq))
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    dq, dk, _ = torch.autograd.grad(attention_packed(*leaves, PackedBatch(lengths), causal=causal), leaves, do)
+    seen = torch.ones(n, n, device="cuda", dtype=torch.bool).tril() if causal else torch.ones(
+        n, n, device="cuda", dtype=torch.bool)
+    want = [torch.zeros_like(t, dtype=torch.float64) for t in (dq, dk)]
+    tol = [torch.zeros_like(t) for t in want]
+    for i in range(reps):
+        r = slice(i * n, i * n + n)
+        for hd in range(hq):
+            j = hd // (hq // hkv)
+            qq, kk, vv, gg = (t.detach().double() for t in (q[r, hd], k[r, j], v[r, j], do[r, hd]))
+            p = torch.softmax((qq @ kk.T * sc).masked_fill(~seen, -math.inf), 1)
+            dp, mag = gg @ vv.T, gg.abs() @ vv.abs().T
+            ds = p * (dp - (p * dp).sum(1, keepdim=True))
+            eds = (h * h + SLOP) * ds.abs() + SLOP * p * (mag + (p * mag).sum(1, keepdim=True)) + tiny * seen
+            want[0][r, hd], tol[0][r, hd] = ds @ kk * sc, (eds + SLOP * ds.abs()) @ kk.abs() * sc
+            want[1][r, j] += ds.T @ qq * sc
+            tol[1][r, j] += (eds + SLOP * ds.abs()).T @ qq.abs() * sc
+    for got, val, t, name in zip((dq, dk), want, tol, ("dq", "dk")):
+        _within(got, val, t + h * val.abs() + tiny, name)
+
+
 def test_gradient_matches_differences():
     g = torch.Generator(device="cuda").manual_seed(7)
     lengths, hq, hkv, d = [37, 80], 4, 2, 64
