@@ -57,6 +57,14 @@ constexpr int kRows = 128;    // rows of a job (packed_plan.hip)
 constexpr int kTile = 64;     // keys per tile
 constexpr float kLog2e = 1.4426950408889634f;
 
+// Sequences of up to this many rows.  A row of two or three keys has nothing
+// for the roundings to average out over: with dS as one 16-bit value and D from
+// an o whose P was rounded, dQ and dK were up to 1.8 times the rounding of the
+// result off there (1.45 times in longer sequences).  These few take D as the
+// sum of P dP, and dS as two 16-bit values; o is not read again, nor its low part
+// written.
+constexpr int kShort = kTile;
+
 struct View {
   const u16* p;
   int64_t row, head;  // strides in elements
@@ -308,7 +316,7 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 1 : TWO_V ? 2 : 3) void
   const float inv = lt == 0.f ? 0.f : 1.f / lt;
   const int64_t off = (orow * a.b.Hq + h) * D;
   store_row<T, NB>(a.o + off, oacc, inv, hh, ok);
-  if (a.o_low != nullptr) {
+  if (a.o_low != nullptr && klen > kShort) {
 #pragma unroll
     for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -341,13 +349,6 @@ template <class T>
 __device__ __forceinline__ unsigned pack2_low(float lo, float hi, unsigned w) {
   return pack2<T>(lo - T::up(static_cast<u16>(w)), hi - T::up(static_cast<u16>(w >> 16)));
 }
-
-// Sequences of up to this many rows.  A row of two or three keys has nothing
-// for the roundings to average out over: with dS as one 16-bit value and D from
-// an o whose P was rounded, dQ and dK were up to 1.8 times the rounding of the
-// result off there (1.45 times in longer sequences).  These few take D as the
-// sum of P dP, and dS as two 16-bit values.
-constexpr int kShort = kTile;
 
 // dQ: the forward's geometry (query on the lane).  Recomputes S^T and dP^T and
 // accumulates dQ^T += K^T dS^T, K^T read transposed from the K image.  dQ and
@@ -382,12 +383,14 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(BwdArgs a) {
       qf[t] = ok ? *reinterpret_cast<const bf16x8*>(qp + 16 * t + 8 * hh) : bf16x8{};
       df[t] = ok ? *reinterpret_cast<const bf16x8*>(a.dout + off + 16 * t + 8 * hh) : bf16x8{};
     }
+    if (klen > kShort) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const bf16x8 ov = ok ? *reinterpret_cast<const bf16x8*>(a.o + off + 16 * t + 8 * hh) : bf16x8{};
-      const bf16x8 lv = ok ? *reinterpret_cast<const bf16x8*>(a.o_low + off + 16 * t + 8 * hh) : bf16x8{};
+      for (int t = 0; t < NT; ++t) {
+        const bf16x8 ov = ok ? *reinterpret_cast<const bf16x8*>(a.o + off + 16 * t + 8 * hh) : bf16x8{};
+        const bf16x8 lv = ok ? *reinterpret_cast<const bf16x8*>(a.o_low + off + 16 * t + 8 * hh) : bf16x8{};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) dsum = fmaf(T::up(df[t][e]), T::up(ov[e]) + T::up(lv[e]), dsum);
+        for (int e = 0; e < 8; ++e) dsum = fmaf(T::up(df[t][e]), T::up(ov[e]) + T::up(lv[e]), dsum);
+      }
     }
   }
   const int64_t li = static_cast<int64_t>(h) * a.b.T + row;
