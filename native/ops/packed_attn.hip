@@ -22,8 +22,8 @@
 // nothing) holds there never enters.
 //
 // Bounds, measured in bf16 with 32 / 8 heads: one sequence of 16,384 rows,
-// causal, D 128, runs at 1.16 PF/s forward (1.90 ms), 1.24 in dQ (2.65 ms) and
-// 1.11 in dK / dV (3.95 ms), a plain matrix product of 8,192^3 at 1.37; the
+// causal, D 128, runs at 1.15 PF/s forward (1.92 ms), 1.24 in dQ (2.65 ms) and
+// 1.13 in dK / dV (3.89 ms), a plain matrix product of 8,192^3 at 1.37; the
 // clock is then down to 1.77 GHz at the card's power limit (operands of zeros
 // run 25 % faster), so fewer operations would help, a better schedule does
 // not.  At D 64 the softmax weighs twice as much: 32 exponentials and as many
