@@ -17,6 +17,7 @@ import struct
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 # KGWE_OPS_LIB: load another build of the kernels (same-box A/B runs only).
 _LIB_PATH = (Path(os.environ["KGWE_OPS_LIB"]) if os.environ.get("KGWE_OPS_LIB")
@@ -229,6 +230,15 @@ def launch(name: str, device: torch.device, *fields) -> None:
 def addr(t: torch.Tensor | None) -> int:
     """Address for a record field: 0 for no tensor."""
     return 0 if t is None else t.data_ptr()
+
+
+def no_tangents(what: str, *tensors: torch.Tensor | None) -> None:
+    """Refuse tensors with a forward-mode derivative: the kernels have none, and to reverse mode such a tensor looks
+    like one that wants no gradient.  Holds under torch.no_grad() too, which leaves forward mode on.  (Outside a
+    dual level there are no tangents: one comparison.)"""
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f"{what} has no forward-mode derivative")
 
 
 def use_hip(*tensors: torch.Tensor) -> bool:

@@ -18,7 +18,8 @@ import torch
 import torch.nn.functional as F
 
 from . import reference as ref
-from ._lib import HALF_TYPES, addr, check, dense16, has_symbol, launch, lib, ptr, rows16, stream, token_view, use_hip
+from ._lib import (HALF_TYPES, addr, check, dense16, has_symbol, launch, lib, no_tangents, ptr, rows16, stream,
+                   token_view, use_hip)
 from .packed import PackedBatch
 
 
@@ -182,6 +183,7 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: P
         return ref.attention_packed(q, k, v, batch.lengths.tolist(), causal, prefix)
     if dtype not in HALF_TYPES or qs[2] not in (64, 128):
         raise ValueError("attention_packed: bf16 or fp16 with head_dim 64 or 128")
+    no_tangents("attention_packed", q, k, v, *(prefix or ()))
     if batch.total == 0:
         return q.clone()
     if grad:

@@ -25,7 +25,7 @@ import math
 import torch
 
 from . import reference as ref
-from ._lib import HALF_TYPES, addr, check, dense16, launch, lib, ptr, rows16, stream, use_hip
+from ._lib import HALF_TYPES, addr, check, dense16, launch, lib, no_tangents, ptr, rows16, stream, use_hip
 from .functional import check_norm_rope
 
 
@@ -35,6 +35,7 @@ def _require(cond: bool, msg: str) -> None:
 
 
 def _forward_only(what: str, *tensors) -> None:
+    no_tangents(what, *tensors)
     if not torch.is_grad_enabled():
         return
     if any([t is not None and t.requires_grad for t in tensors]):

@@ -11,7 +11,7 @@ import os
 import torch
 
 from . import reference as ref
-from ._lib import HALF_TYPES, addr, check, dense16, launch, lib, ptr, rows16, stream, use_hip
+from ._lib import HALF_TYPES, addr, check, dense16, launch, lib, no_tangents, ptr, rows16, stream, use_hip
 from .gemm import wgrad, wgrad_supported
 
 
@@ -293,6 +293,7 @@ def norm_rope_qkv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, posit
     check_norm_rope("norm_rope_qkv", qkv, positions, cos, sin, hq, hkv, d, q_weight, k_weight, offset, 1)
     if not qkv.is_cuda:
         return ref.norm_rope_qkv(qkv, cos, sin, positions, hq, hkv, d, q_weight, k_weight, eps, offset)
+    no_tangents("norm_rope_qkv", qkv, cos, sin, q_weight, k_weight)
     if qkv.shape[0] == 0:
         q, k, v = qkv.reshape(0, hq + 2 * hkv, d).split((hq, hkv, hkv), dim=1)
         return q, k, v

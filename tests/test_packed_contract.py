@@ -1,0 +1,59 @@
+"""What the operators on packed and prefix-sharing batches refuse rather than answer wrongly."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from kgwe.ops import attention_packed, norm_rope_qkv
+from kgwe.ops import decode as dec
+from kgwe.ops import reference as ref
+from kgwe.ops.packed import PackedBatch
+
+
+def _dual(t):
+    return forward_ad.make_dual(t, torch.ones_like(t))
+
+
+# ------------------------------------------------------------------ forward-mode derivatives
+def test_forward_only_calls_refuse_tangents():
+    att = dec.PrefixDecodeAttention(1, 4, 2, 16, 8, 5, "cpu", dtype=torch.float32)
+    q, p, c = torch.zeros(1, 4, 16), torch.zeros(2, 5, 16), torch.zeros(1, 2, 8, 16)
+    lens = torch.zeros(1, dtype=torch.int32)
+    hq, hkv, d = 2, 1, 32
+    qkv = torch.randn(3, (hq + 2 * hkv) * d)
+    cos, sin = ref.rope_tables(8, d)
+    pos, w = torch.zeros(3, dtype=torch.int32), torch.ones(d)
+    kc, vc = torch.zeros(3, hkv, 8, d), torch.zeros(3, hkv, 8, d)
+    with forward_ad.dual_level():
+        att(q, p, p, c, c, lens)  # a level alone is nothing to refuse
+        for bad in (lambda: att(_dual(q), p, p, c, c, lens), lambda: att(q, p, _dual(p), c, c, lens),
+                    lambda: dec.norm_rope_append(_dual(qkv), pos, cos, sin, kc, vc, hq, hkv, d),
+                    lambda: dec.norm_rope_append(qkv, pos, cos, sin, kc, vc, hq, hkv, d, _dual(w), w)):
+            with pytest.raises(ValueError):
+                bad()
+            with pytest.raises(ValueError), torch.no_grad():  # which leaves forward mode as it is
+                bad()
+
+
+@pytest.mark.gpu
+def test_gpu_kernels_refuse_tangents():
+    """A tensor with a tangent does not require a gradient; the kernels would drop the tangent."""
+    hq, hkv, d = 4, 2, 64
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q, k, v, pk = (torch.randn(s, h, d, device="cuda", generator=g).bfloat16()
+                   for s, h in ((5, hq), (5, hkv), (5, hkv), (hkv, 3)))
+    qkv, w = torch.randn(5, (hq + 2 * hkv) * d, device="cuda", generator=g).bfloat16(), torch.ones(
+        d, device="cuda", dtype=torch.bfloat16)
+    batch = PackedBatch([5])
+    cos, sin = ref.rope_tables(5, d, device="cuda")
+    with forward_ad.dual_level():
+        for bad in (lambda: attention_packed(_dual(q), k, v, batch), lambda: attention_packed(q, k, _dual(v), batch),
+                    lambda: attention_packed(q, k.clone().requires_grad_(), _dual(v), batch),
+                    lambda: attention_packed(q, k, v, batch, prefix=(pk, _dual(pk))),
+                    lambda: norm_rope_qkv(_dual(qkv), cos, sin, 5, hq, hkv, d),
+                    lambda: norm_rope_qkv(qkv, cos, sin, 5, hq, hkv, d, w, _dual(w)),
+                    lambda: norm_rope_qkv(qkv, _dual(cos), sin, 5, hq, hkv, d)):
+            with pytest.raises(ValueError):
+                bad()
+            with pytest.raises(ValueError), torch.no_grad():
+                bad()
+        attention_packed(q, k, v, batch)
