@@ -13,6 +13,8 @@
 // go through a buffer descriptor whose extent ends with the tile's last valid
 // row: rows past it arrive as zeros, whatever memory holds there.
 #pragma once
+#include <type_traits>
+
 #include "half_types.h"
 
 namespace kgwe {
@@ -51,9 +53,18 @@ __device__ __forceinline__ unsigned pack2<Fp16>(float lo, float hi) {
 
 __device__ __forceinline__ bf16x8 as_op(const u32x4& w) { return __builtin_bit_cast(bf16x8, w); }
 
-// 2^x as one v_exp_f32: arguments here are at most a few units, and a result
-// below 2^-126 is zero to any 16-bit output.
+// 2^x as one v_exp_f32: arguments here are far below 128, and a result below
+// 2^-126 is zero to any 16-bit output.
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// log2 of what a probability against a running maximum is multiplied by before
+// it is rounded to T: fp16 has steps of 2^-24 below 2^-14, and what many keys
+// far from the maximum add up to would be lost (65,536 keys at 2^-26 of it:
+// all).  The sum of the probabilities carries the same factor, so the output
+// does not; it costs nothing, the exponent takes it.  Running maxima lag by up
+// to 2^4 (kDefer): 2^15 at most, and fp16 ends at 65,504.
+template <class T>
+constexpr float kLift = std::is_same<T, Fp16>::value ? 11.f : 0.f;
 
 // Row of a 32x32 accumulator tile that register r of this lane half holds.
 __device__ __forceinline__ int tile_row(int r, int half) { return (r & 3) + 8 * (r >> 2) + 4 * half; }

@@ -111,7 +111,7 @@ __device__ __forceinline__ int wave_rows(const Batch& b, const Job& job, int wav
 }
 
 // Running max kept until a tile's max passes it by this much (log2 units), so
-// P stays below 2^4 and O is rescaled on few tiles.
+// P stays below 2^4 (kLift counts on it) and O is rescaled on few tiles.
 constexpr float kDefer = 4.f;
 
 struct FwdArgs {
@@ -236,14 +236,15 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 1 : TWO_V ? 2 : 3) void
           for (int r = 0; r < 16; ++r) oacc[i][r] *= alpha;
       }
       m = m_new;
-      // P = 2^(S c - m) in pairs; the accumulator tile is the next product's operand as it is
+      const float m_p = m_use - kLift<T>;
+      // P = 2^(S c - m), in fp16 2^11 times that, in pairs; the accumulator tile is the next product's operand as it is
       float r0 = 0.f, r1 = 0.f;
 #pragma unroll
       for (int st = 0; st < 2; ++st)
 #pragma unroll
         for (int r = 0; r < 16; r += 2) {
-          const float p0 = exp2_fast(fmaf(s[st][r], a.c, -m_use));
-          const float p1 = exp2_fast(fmaf(s[st][r + 1], a.c, -m_use));
+          const float p0 = exp2_fast(fmaf(s[st][r], a.c, -m_p));
+          const float p1 = exp2_fast(fmaf(s[st][r + 1], a.c, -m_p));
           r0 += p0;
           r1 += p1;
           pb[2 * st + (r >> 3)][(r & 7) >> 1] = pack2<T>(p0, p1);
@@ -324,7 +325,7 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 1 : TWO_V ? 2 : 3) void
     store_row<T, NB>(a.o_low + off, oacc, 1.f, hh, ok);
   }
   if (a.lse != nullptr && ok && hh == 0)
-    a.lse[static_cast<int64_t>(h) * a.b.T + orow] = lt == 0.f ? -INFINITY : m + log2f(lt);
+    a.lse[static_cast<int64_t>(h) * a.b.T + orow] = lt == 0.f ? -INFINITY : m + log2f(lt) - kLift<T>;
 }
 
 struct BwdArgs {
