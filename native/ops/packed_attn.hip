@@ -114,12 +114,49 @@ __device__ __forceinline__ int wave_rows(const Batch& b, const Job& job, int wav
 // P stays below 2^4 (kLift counts on it) and O is rescaled on few tiles.
 constexpr float kDefer = 4.f;
 
+// The gradient's 16-bit operands, P and dS, in fp16.  At their natural size P =
+// 1 / n and dS = P (dP - D) of long rows fall among fp16's steps of 2^-24 (dQ for
+// incoming gradients of 1e-3 was off by 1.1e-2 of its norm at 12,000 keys, by
+// 3.7e-2 at 40,000; it is 1.2e-3 and 2.1e-3, of which the result's own rounding
+// 1.1e-3 and 2.1e-3), and dS of large incoming gradients passes its largest
+// value, 65,504, where dQ and dK do not.  bf16 has fp32's range.
+//   P is at most 1: it is lifted by 2^14, by way of the stored row sums.
+//   dS has no bound that is worth having, so every accumulated row (of dQ or
+//   dK) has a factor of its own, a power of two from 2^60 down: where a tile's
+//   dS would pass 2^15 the factor and the sums so far are scaled down together,
+//   the largest to 2^13 .. 2^14.  What is 2^28 below a row's largest dS still
+//   counts in full.
+// Factors are powers of two and leave the accumulators through the result's own
+// multiplier, so they round nothing.  The maxima cost 3 to 6 % of a training
+// call (16,384 rows, 32 / 8 heads x 128: 8.91 -> 9.19 ms, 300 sequences of 10 to
+// 60 rows 269 -> 285 us).
+template <class T>
+constexpr bool kScaled = std::is_same<T, Fp16>::value;
+template <class T>
+constexpr int kLiftP = kScaled<T> ? 14 : 0;  // log2; stored row sums are lse - kLiftP
+constexpr int kFirst = 60;  // log2 of the first factor: times any dS of fp16 inputs far below fp32's largest
+constexpr float kTop = 32768.f;
+
+// Largest magnitude in the accumulator row that this lane and its partner hold.
+__device__ __forceinline__ float row_top(const f32x16& p) {
+  float top = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(p[r]));
+  return half_max(top);
+}
+
+// log2 of what brings a row's largest dS back to 2^13 .. 2^14, 0 where it has
+// room (and for infinity, which nothing brings back).
+__device__ __forceinline__ int fit(float top) {
+  return top > kTop && top < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(top) : 0;
+}
+
 struct FwdArgs {
   Batch b;
   View q, k, v, pk, pv;
   u16* o;      // [T, Hq, D]
   u16* o_low;  // what the rounding of o dropped, rounded in turn; null: not wanted
-  float* lse;  // [Hq, T], log2 units; null: not wanted
+  float* lse;  // [Hq, T], log2 units, less kLiftP; null: not wanted
   int P, causal;
   float c;     // scale * log2 e
 };
@@ -325,7 +362,7 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 1 : TWO_V ? 2 : 3) void
     store_row<T, NB>(a.o_low + off, oacc, 1.f, hh, ok);
   }
   if (a.lse != nullptr && ok && hh == 0)
-    a.lse[static_cast<int64_t>(h) * a.b.T + orow] = lt == 0.f ? -INFINITY : m + log2f(lt) - kLift<T>;
+    a.lse[static_cast<int64_t>(h) * a.b.T + orow] = lt == 0.f ? -INFINITY : m + log2f(lt) - kLift<T> - kLiftP<T>;
 }
 
 struct BwdArgs {
@@ -395,8 +432,12 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(BwdArgs a) {
     }
   }
   const int64_t li = static_cast<int64_t>(h) * a.b.T + row;
-  const float lse = ok ? a.lse[li] : 0.f;
+  float lse = ok ? a.lse[li] : 0.f;
+  if constexpr (kScaled<T>) lse += kLiftP<T>;
   float delta = half_add(dsum);
+  int factor = kFirst;   // log2 of this row's
+  float shift = -lse;    // of the exponents
+  if constexpr (kScaled<T>) shift = factor - lse;
   f32x16 acc[NB];
 #pragma unroll
   for (int i = 0; i < NB; ++i) acc[i] = f32x16{};
@@ -436,11 +477,23 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(BwdArgs a) {
         f32x16 s, p;
         scores(Kc, Vc, st, -delta, s, p);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) p[r] *= exp2_fast(fmaf(s[r], a.c, -lse));
+        for (int r = 0; r < 16; ++r) p[r] *= exp2_fast(fmaf(s[r], a.c, shift));
         if (edge) {
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if (32 * st + tile_row(r, 0) > last) p[r] = 0.f;
+        }
+        if constexpr (kScaled<T>) {
+          const float top = row_top(p);
+          if (__any(top > kTop)) {
+            const int n = fit(top);
+            const float f = ldexpf(1.f, n);
+            factor += n;
+            shift = factor - lse;
+            p *= f;
+#pragma unroll
+            for (int db = 0; db < NB; ++db) acc[db] *= f;
+          }
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -491,7 +544,9 @@ __global__ __launch_bounds__(256, 2) void packed_dq_kernel(BwdArgs a) {
     }
   }
   if (hh == 0 && ok) a.delta[li] = -delta;
-  store_row<T, NB>(a.dq + (row * a.b.Hq + h) * D, acc, a.scale, hh, ok);
+  float mul = a.scale;
+  if constexpr (kScaled<T>) mul = ldexpf(mul, -factor);
+  store_row<T, NB>(a.dq + (row * a.b.Hq + h) * D, acc, mul, hh, ok);
 }
 
 constexpr int kQt = 32;  // query rows per step of the dK / dV sweep
@@ -545,6 +600,7 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(BwdArgs a) {
   f32x16 dka[NB], dva[NB];
 #pragma unroll
   for (int i = 0; i < NB; ++i) dka[i] = dva[i] = f32x16{};
+  float factor = ldexpf(1.f, kFirst - kLiftP<T>);  // this key's, besides P's
 
   const int nq = (qlen + kQt - 1) / kQt;
   const int first = a.causal ? kb * (kRows / kQt) : 0;
@@ -597,6 +653,16 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(BwdArgs a) {
         for (int r = 0; r < 16; ++r)
           if (tile_row(r, 0) < before) s[r] = p[r] = 0.f;
       }
+      if constexpr (kScaled<T>) {
+        const float top = row_top(p) * factor;
+        if (__any(top > kTop)) {
+          const float f = ldexpf(1.f, fit(top));
+          factor *= f;
+#pragma unroll
+          for (int db = 0; db < NB; ++db) dka[db] *= f;
+        }
+        p *= factor;
+      }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         u32x4 pw, sw;
@@ -639,9 +705,14 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(BwdArgs a) {
     dma_join();  // the V image's DMA ends before the workgroup does
   }
   const int64_t off = (krow * a.b.Hkv + hkv) * D;
+  float mul_k = 1.f, mul_v = 1.f;
+  if constexpr (kScaled<T>) {
+    mul_v = ldexpf(1.f, -kLiftP<T>);
+    mul_k = mul_v / factor;
+  }
   if (a.parts == 1) {
-    store_row<T, NB>(a.dk + off, dka, a.scale, hh, ok);
-    store_row<T, NB>(a.dv + off, dva, 1.f, hh, ok);
+    store_row<T, NB>(a.dk + off, dka, a.scale * mul_k, hh, ok);
+    store_row<T, NB>(a.dv + off, dva, mul_v, hh, ok);
   } else if (ok) {
     const int64_t all = static_cast<int64_t>(a.b.T) * a.b.Hkv * D;
     float* pk = a.part + part * all + off + 4 * hh;
@@ -653,8 +724,8 @@ __global__ __launch_bounds__(256, 2) void packed_dkv_kernel(BwdArgs a) {
         f32x4 x, y;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          x[j] = dka[db][4 * g4 + j];
-          y[j] = dva[db][4 * g4 + j];
+          x[j] = dka[db][4 * g4 + j] * mul_k;
+          y[j] = dva[db][4 * g4 + j] * mul_v;
         }
         *reinterpret_cast<f32x4*>(pk + 32 * db + 8 * g4) = x;
         *reinterpret_cast<f32x4*>(pv + 32 * db + 8 * g4) = y;

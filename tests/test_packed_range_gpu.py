@@ -70,3 +70,51 @@ def test_many_far_keys_keep_their_weight(d, dtype):
             att = dec.PrefixDecodeAttention(B, 1, 1, d, 300, P, "cuda", dtype=dtype)
             lens = torch.zeros(B, dtype=torch.int32, device="cuda")
             _check_far(att(q.expand(B, 1, d).contiguous(), k, v, own, own, lens)[:, 0], q, k, v)
+
+
+# ------------------------------------------------------------------ incoming gradients of any size
+def _exact_gradients(q, k, v, do, n, causal):
+    """Of sequences of n rows each, in 64 bits."""
+    T, hq, d = q.shape
+    G, sc = hq // k.shape[1], 1 / math.sqrt(d)
+    out = [torch.zeros_like(t, dtype=torch.float64) for t in (q, k, v)]
+    hidden = torch.ones(n, n, dtype=torch.bool, device="cuda").triu(1) if causal else None
+    for at in range(0, T, n):
+        r = slice(at, at + n)
+        for h in range(hq):
+            qq, kk, vv, gg = (t.detach().double() for t in (q[r, h], k[r, h // G], v[r, h // G], do[r, h]))
+            s = qq @ kk.T * sc
+            p = torch.softmax(s if hidden is None else s.masked_fill_(hidden, -math.inf), 1)
+            del s
+            ds = gg @ vv.T
+            ds = ds.sub_((p * ds).sum(1, keepdim=True)).mul_(p).mul_(sc)
+            out[0][r, h] = ds @ kk
+            out[1][r, h // G] += ds.T @ qq
+            out[2][r, h // G] += p.T @ gg
+    return out
+
+
+@pytest.mark.parametrize("n,reps,do_scale,q_scale,k_scale,v_scale", [
+    (12000, 1, 1e-2, 1, 1, 1), (12000, 1, 1e-3, 1, 1, 1),  # dS about 1 / n: below what fp16 holds well
+    (40, 30, 2.0 ** -15, 1 / 16, 16, 1), (40, 30, 2.0 ** -15, 16, 1 / 16, 1),  # the same in short sequences
+    (300, 2, 2.0 ** 12, 1 / 16, 1 / 16, 4), (50, 9, 2.0 ** 12, 1 / 16, 1 / 16, 4),  # dS past fp16's largest
+])
+@pytest.mark.parametrize("hq,hkv", [(2, 1), (2, 2)])  # the group's heads shared out, and not
+@pytest.mark.parametrize("d,causal", [(64, True), (128, False)])
+def test_fp16_gradients_of_small_and_large_incoming_gradients(n, reps, do_scale, q_scale, k_scale, v_scale, hq, hkv, d,
+                                                              causal):
+    """P, dS and the result are rounded once each, whatever the size of dS: three errors of h / sqrt(3)."""
+    g = torch.Generator(device="cuda").manual_seed(n + d)
+    T, f16 = n * reps, torch.float16
+    q, k, v, do = (_rnd(g, T, x, d, dtype=f16, scale=s)
+                   for x, s in ((hq, q_scale), (hkv, k_scale), (hkv, v_scale), (hq, do_scale)))
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad(attention_packed(*leaves, PackedBatch([n] * reps), causal=causal), leaves, do)
+    h = HALF[f16]
+    late = torch.arange(T, device="cuda") % n >= n // 2  # rows of many keys, which early rows would hide
+    for name, got, want in zip(("dq", "dk", "dv"), grads, _exact_gradients(q, k, v, do, n, causal)):
+        assert got.isfinite().all(), name
+        for rows in (late, ~late):
+            err, norm = (got[rows].double() - want[rows]).norm().item(), want[rows].norm().item()
+            allowed = 1.5 * math.sqrt((h * norm) ** 2 + want[rows].numel() * STEP[f16] ** 2 / 12)
+            assert err <= allowed, (name, err, norm, allowed)
