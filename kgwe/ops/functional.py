@@ -223,6 +223,8 @@ def check_norm_rope(what, qkv, positions, cos, sin, hq, hkv, d, q_weight, k_weig
         raise ValueError(f"{what}: qkv must be [T, (hq+2hkv)*d]")
     if isinstance(positions, int):
         _require(positions > 0, f"{what}: a sequence length must be positive")
+        _require(shape[0] % positions == 0, f"{what}: rows must be a multiple of the sequence length")
+        reach = positions + offset
     elif not (positions.dtype == torch.int32 and positions.shape == shape[:1] and positions.device == device):
         raise ValueError(f"{what}: positions int32 [T] on qkv's device")
     if (q_weight is None) != (k_weight is None):
@@ -286,10 +288,11 @@ def norm_rope_qkv(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, posit
     """qkv [T, (hq+2hkv)d] -> q [T,hq,d], k [T,hkv,d], v [T,hkv,d]: every q and k
     head RMS-normed with its weight [d] (no weights: no norm), then rotated at
     ``positions[t] + offset`` (int32 [T], as a PackedBatch has them; or the
-    sequence length S of a rectangular batch: row t is at t % S), in one pass
-    and with one rounding; v is copied.  A row whose position is negative
-    or outside the tables gives zeros and takes no gradient.  Differentiable
-    with regard to qkv and the weights."""
+    sequence length S of a rectangular batch: row t is at t % S, T is a multiple
+    of S and the tables hold S + offset rows), in one pass and with one
+    rounding; v is copied.  A row whose given position is negative or outside
+    the tables gives zeros and takes no gradient.  Differentiable with regard to
+    qkv and the weights."""
     check_norm_rope("norm_rope_qkv", qkv, positions, cos, sin, hq, hkv, d, q_weight, k_weight, offset, 1)
     if not qkv.is_cuda:
         return ref.norm_rope_qkv(qkv, cos, sin, positions, hq, hkv, d, q_weight, k_weight, eps, offset)

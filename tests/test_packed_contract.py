@@ -57,3 +57,18 @@ def test_gpu_kernels_refuse_tangents():
             with pytest.raises(ValueError), torch.no_grad():
                 bad()
         attention_packed(q, k, v, batch)
+
+
+# ------------------------------------------------------------------ a rectangular batch
+def test_a_rectangular_batch_fits_its_tables():
+    """A sequence length in the place of positions is known on the host: rows past the tables are an undersized table,
+    not padding, and the rows are whole sequences (as rope_qkv has it)."""
+    hq, hkv, d = 2, 1, 32
+    qkv = torch.randn(12, (hq + 2 * hkv) * d)
+    cos, sin = ref.rope_tables(8, d)
+    for S, offset in ((12, 0), (6, 3), (9, 0), (5, 0), (8, 0)):
+        with pytest.raises(ValueError):
+            norm_rope_qkv(qkv, cos, sin, S, hq, hkv, d, offset=offset)
+    for S, offset in ((6, 2), (4, 0), (1, 7)):
+        assert all(t.any(-1).all() for t in norm_rope_qkv(qkv, cos, sin, S, hq, hkv, d, offset=offset))
+    assert norm_rope_qkv(qkv[:0], cos, sin, 8, hq, hkv, d)[0].shape == (0, hq, d)
