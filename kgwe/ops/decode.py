@@ -127,8 +127,9 @@ def norm_rope_append(qkv: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, si
     Returns q [T,hq,d], with ``keep_kv`` (q, k, v).  One new token per row in a
     decode step, or all rows of a packed prompt.  A row of qkv whose place is
     outside the cache (position -1: padding) writes nothing; two rows must not
-    name one place.  Forward only."""
+    name one place, and a cache without any place is refused.  Forward only."""
     T, dtype, device, cache = qkv.shape[0], qkv.dtype, qkv.device, kc.shape
+    _require(kc.numel() > 0, "norm_rope_append: the caches have no room")
     if not (len(cache) == 4 and vc.shape == cache and cache[1] == hkv and cache[3] == d and kc.dtype == vc.dtype == dtype
             and kc.is_contiguous() and vc.is_contiguous() and kc.device == vc.device == device
             and kc.data_ptr() != vc.data_ptr()):
@@ -152,7 +153,7 @@ def norm_rope_append(qkv: torch.Tensor, pos: torch.Tensor, cos: torch.Tensor, si
     k = v = None
     if keep_kv:
         k, v = qkv.new_empty((T, hkv, d)), qkv.new_empty((T, hkv, d))
-    if T > 0 and kc.numel() > 0:
+    if T > 0:
         if (kc.data_ptr() | vc.data_ptr()) & 15:
             raise ValueError("norm_rope_append: caches must be 16-byte aligned")
         qkv, cos, sin, pos = rows16(qkv), dense16(cos), dense16(sin), pos.contiguous()

@@ -72,3 +72,25 @@ def test_a_rectangular_batch_fits_its_tables():
     for S, offset in ((6, 2), (4, 0), (1, 7)):
         assert all(t.any(-1).all() for t in norm_rope_qkv(qkv, cos, sin, S, hq, hkv, d, offset=offset))
     assert norm_rope_qkv(qkv[:0], cos, sin, 8, hq, hkv, d)[0].shape == (0, hq, d)
+
+
+# ------------------------------------------------------------------ caches without room
+@pytest.mark.parametrize("T,R,smax", [(3, 3, 0), (3, 0, 8), (0, 0, 8), (0, 3, 0)])
+def test_an_empty_cache_is_refused_as_such(T, R, smax):
+    hq, hkv, d = 2, 1, 32
+    cos, sin = ref.rope_tables(8, d)
+    kc, vc = torch.zeros(R, hkv, smax, d), torch.zeros(R, hkv, smax, d)
+    ints = torch.zeros(T, dtype=torch.int32)
+    with pytest.raises(ValueError, match="no room"):
+        dec.norm_rope_append(torch.randn(T, (hq + 2 * hkv) * d), ints, cos, sin, kc, vc, hq, hkv, d, rows=ints)
+
+
+@pytest.mark.gpu
+def test_gpu_append_of_no_rows():
+    hq, hkv, d = 2, 1, 64
+    cos, sin = ref.rope_tables(8, d, device="cuda")
+    kc, vc = torch.ones(2, 3, hkv, 8, d, device="cuda", dtype=torch.bfloat16).unbind()
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    out = dec.norm_rope_append(torch.zeros(0, (hq + 2 * hkv) * d, device="cuda", dtype=torch.bfloat16), none, cos, sin,
+                               kc, vc, hq, hkv, d, rows=none, keep_kv=True)
+    assert [t.shape for t in out] == [(0, hq, d), (0, hkv, d), (0, hkv, d)] and (kc == 1).all() and (vc == 1).all()
