@@ -228,6 +228,9 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(Args a) {
     return;
   }
 
+  // (Own chunks outside the one-workgroup form are always joined with something:
+  // the entry sees to it, so a sequence without keys needs no workgroup here.)
+  //
   // At most 32 rows: every wave walks tiles of its own (tile index = wave mod
   // 4) with its own K and V buffer and no barrier: the next K tile is on its
   // way from the S product on, the next V tile from the O product on.
@@ -250,8 +253,7 @@ __global__ __launch_bounds__(256, 2) void prefix_attn_kernel(Args a) {
           int left = unit - scan_chunks, b0 = scan_b, found = 0;
           for (; b0 < a.B; b0 += 64) {
             const int n = b0 + lane < a.B ? min(max(a.lens[b0 + lane], 0), a.Smax) : 0;
-            // where nothing is joined an empty row's zeros have to be written, too
-            const int chunks = final ? (b0 + lane < a.B ? 1 : 0) : (n + a.o_chunk - 1) / a.o_chunk;
+            const int chunks = (n + a.o_chunk - 1) / a.o_chunk;
             int upto = chunks;
 #pragma unroll
             for (int off = 1; off < kWave; off <<= 1) {
@@ -585,6 +587,7 @@ KGWE_API int kgwe_prefix_attn(const PrefixCall* c, hipStream_t s) {
     return -1;
   const Plan p = make_plan(B, Hq, Hkv, P, Smax);
   const int slots = p.p_splits + p.o_splits;
+  if (!p.direct && p.o_splits > 0 && slots < 2) return -1;  // a sequence without keys would stay unwritten
   if (!p.direct && slots > 1 && !c->work) return -2;
   float* ml = c->work + static_cast<int64_t>(B) * Hq * slots * D;
   const Args a{static_cast<const u16*>(c->q), static_cast<const u16*>(c->pk), static_cast<const u16*>(c->pv),

@@ -118,3 +118,34 @@ def test_fp16_gradients_of_small_and_large_incoming_gradients(n, reps, do_scale,
             err, norm = (got[rows].double() - want[rows]).norm().item(), want[rows].norm().item()
             allowed = 1.5 * math.sqrt((h * norm) ** 2 + want[rows].numel() * STEP[f16] ** 2 / 12)
             assert err <= allowed, (name, err, norm, allowed)
+
+
+# ------------------------------------------------------------------ one chunk of a prefix, nothing to join
+@pytest.mark.parametrize("B,h", [(130, 128), (2, 256)])  # tiles that 128 rows share; a wave's own tiles
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_single_chunk_of_a_prefix_is_written_without_a_join(B, h, dtype):
+    g = torch.Generator(device="cuda").manual_seed(B)
+    P, d = 600, 64
+    q, k, v = (_rnd(g, *s, dtype=dtype) for s in ((B, h, d), (h, P, d), (h, P, d)))
+    own = torch.zeros(B, h, 0, d, device="cuda", dtype=dtype)
+    att = dec.PrefixDecodeAttention(B, h, h, d, 0, P, "cuda", dtype=dtype)
+    assert att.words == 0
+    o = att(q, k, v, own, own, torch.zeros(B, device="cuda", dtype=torch.int32)).double()
+    p = torch.softmax(torch.matmul(q.double().transpose(0, 1), k.double().transpose(1, 2).contiguous()) / 8, -1)
+    want, mass = (torch.matmul(p, x).transpose(0, 1) for x in (v.double(), v.double().abs()))
+    hf = HALF[dtype]
+    assert ((o - want).abs() <= hf * want.abs() + (hf + 2.0 ** -14) * mass + STEP[dtype]).all()
+
+
+def test_sequences_without_keys_are_written_where_chunks_are_joined():
+    """Own chunks outside the one-workgroup form: whatever the cache's length, an empty sequence's zeros come from the
+    join."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for smax in (513, 700, 1025):
+        q, kc, vc = (_rnd(g, *s, dtype=torch.bfloat16) for s in ((3, 4, 64), (3, 2, smax, 64), (3, 2, smax, 64)))
+        none = kc[0, :, :0]
+        for B in (3, 1):
+            att = dec.PrefixDecodeAttention(B, 4, 2, 64, smax, 0, "cuda")
+            o = att(q[:B], none, none, kc[:B], vc[:B], torch.tensor([0, 1, 0][:B], dtype=torch.int32, device="cuda"))
+            assert not o[0].any() and not o[2:].any()
+            assert B == 1 or torch.equal(o[1], vc[1, :, 0].repeat_interleave(2, 0))
