@@ -149,3 +149,41 @@ def test_sequences_without_keys_are_written_where_chunks_are_joined():
             o = att(q[:B], none, none, kc[:B], vc[:B], torch.tensor([0, 1, 0][:B], dtype=torch.int32, device="cuda"))
             assert not o[0].any() and not o[2:].any()
             assert B == 1 or torch.equal(o[1], vc[1, :, 0].repeat_interleave(2, 0))
+
+
+# ------------------------------------------------------------------ D from the unrounded output
+@pytest.mark.parametrize("n,reps", [(65, 8), (130, 4), (300, 2)])
+@pytest.mark.parametrize("d,dtype", [(64, torch.bfloat16), (128, torch.bfloat16), (128, torch.float16)])
+def test_gradients_take_d_from_the_unrounded_output(n, reps, d, dtype):
+    """Values and keys around a common mean: an error of D_i moves all dS of the row one way, where the errors of the
+    roundings of P and dS cancel.  The kernel's dQ and dK are within 1.5 times those roundings' root mean square; with
+    D = dO . round(o) they would not be, which is computed beside it.  Not causal: every row has n keys."""
+    g = torch.Generator(device="cuda").manual_seed(n + d)
+    hq, hkv, T, sc, h = 2, 1, n * reps, 1 / math.sqrt(d), HALF[dtype]
+    q, do = _rnd(g, T, hq, d, dtype=dtype), _rnd(g, T, hq, d, dtype=dtype)
+    k, v = ((torch.randn(T, hkv, d, device="cuda", generator=g) + m).to(dtype) for m in (2, 4))
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    dq, dk, _ = torch.autograd.grad(attention_packed(*leaves, PackedBatch([n] * reps), causal=False), leaves, do)
+    shape = [torch.zeros(T, x, d, device="cuda", dtype=torch.float64) for x in (hq, hkv)]
+    want, off = [t.clone() for t in shape], [t.clone() for t in shape]  # the gradient; what D = dO . round(o) would add
+    square = [torch.zeros_like(t[..., 0]) for t in shape]  # expected squared error of a row
+    for at in range(0, T, n):
+        r = slice(at, at + n)
+        for hd in range(hq):
+            qq, kk, vv, gg = (t.detach().double() for t in (q[r, hd], k[r, 0], v[r, 0], do[r, hd]))
+            p = torch.softmax(qq @ kk.T * sc, 1)
+            dp, o = gg @ vv.T, p @ vv
+            ds = p * (dp - (gg * o).sum(1, keepdim=True))
+            moved = p * -(gg * (o.to(dtype).double() - o)).sum(1, keepdim=True)
+            want[0][r, hd], off[0][r, hd] = ds @ kk * sc, moved @ kk * sc
+            want[1][r, 0] += ds.T @ qq * sc
+            off[1][r, 0] += moved.T @ qq * sc
+            # squared errors of D: P's roundings, that of o's low part, and fp32's (2^-20 of the summed magnitudes)
+            d2 = h * h / 3 * (p * dp).pow(2).sum(1) + h ** 4 / 3 * (gg * o).pow(2).sum(1)
+            d2 = d2 + (2.0 ** -20 * (gg.abs() * vv.abs().amax(0)).sum(1)) ** 2
+            square[0][r, hd] = (h * h / 3 * (ds * ds) @ kk.pow(2).sum(1) + d2 * (p @ kk).pow(2).sum(1)) * sc * sc
+            square[1][r, 0] += (h * h / 3 * (ds * ds).T @ qq.pow(2).sum(1) + (p * p).T @ (d2 * qq.pow(2).sum(1))) * sc * sc
+    for name, got, val, var, sq in zip(("dq", "dk"), (dq, dk), want, off, square):
+        allowed = 1.5 * math.sqrt(sq.sum().item() + h * h / 3 * val.pow(2).sum().item() + val.numel() * STEP[dtype] ** 2 / 12)
+        err = (got.double() - val).norm().item()
+        assert err <= allowed < var.norm().item(), (name, err, allowed, var.norm().item())
