@@ -187,3 +187,29 @@ def test_gradients_take_d_from_the_unrounded_output(n, reps, d, dtype):
         allowed = 1.5 * math.sqrt(sq.sum().item() + h * h / 3 * val.pow(2).sum().item() + val.numel() * STEP[dtype] ** 2 / 12)
         err = (got.double() - val).norm().item()
         assert err <= allowed < var.norm().item(), (name, err, allowed, var.norm().item())
+
+
+# ------------------------------------------------------------------ a plan dropped under a waiting launch
+def test_a_dropped_plan_is_not_handed_out_before_its_launch_has_run():
+    """The side stream is held back by a bounded spin, so the job table is certainly still to be read when the batch
+    goes and tensors of its size are made on the main stream."""
+    g = torch.Generator(device="cuda").manual_seed(14)
+    lengths = [3000, 2000, 1]
+    q, k, v = (_rnd(g, sum(lengths), x, 64, dtype=torch.bfloat16) for x in (16, 4, 4))
+    want = attention_packed(q, k, v, PackedBatch(lengths))
+    side, main = torch.cuda.Stream(), torch.cuda.current_stream()
+    with torch.cuda.stream(side):
+        attention_packed(q, k, v, PackedBatch(lengths))  # the stream's first call is not the one that counts
+    torch.cuda.synchronize()
+    batch = PackedBatch(lengths)
+    at, slots = batch.jobs.data_ptr(), batch.jobs.shape[0]
+    side.wait_stream(main)
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        got = attention_packed(q, k, v, batch)
+    del batch
+    other = [torch.zeros(slots, 4, dtype=torch.int32, device="cuda") for _ in range(8)]
+    assert not side.query()  # the launch is still to come
+    assert at not in [t.data_ptr() for t in other]
+    main.wait_stream(side)
+    assert torch.equal(got, want)
