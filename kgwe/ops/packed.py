@@ -33,7 +33,9 @@ class PackedBatch:
     ``positions`` [total] and ``seq_ids`` [total] (both -1 for padding rows),
     ``last_rows`` [n] (last row of every sequence; the row before it for an
     empty one).  The tables belong to the stream they were built on, like any
-    tensor; built inside a graph capture they belong to that graph.
+    tensor; built inside a graph capture (lengths on the GPU only) they belong
+    to that graph, and a batch built before a capture that uses it has to be
+    kept, like any input, as long as the graph is replayed.
     """
 
     def __init__(self, lengths, total: int | None = None, device=None):
@@ -77,6 +79,8 @@ class PackedBatch:
             if on_gpu:
                 self.lengths = lengths.detach().clamp(0, self.total).to(torch.int32).contiguous()
             else:
+                if torch.cuda.is_current_stream_capturing():  # the copy below would end the capture with an error
+                    raise ValueError("PackedBatch: inside a graph capture lengths have to be on the GPU, with total")
                 self.lengths = torch.tensor(values, dtype=torch.int32).to(device)
             self._plan_on_gpu()
 

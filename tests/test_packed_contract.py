@@ -94,3 +94,22 @@ def test_gpu_append_of_no_rows():
     out = dec.norm_rope_append(torch.zeros(0, (hq + 2 * hkv) * d, device="cuda", dtype=torch.bfloat16), none, cos, sin,
                                kc, vc, hq, hkv, d, rows=none, keep_kv=True)
     assert [t.shape for t in out] == [(0, hq, d), (0, hkv, d), (0, hkv, d)] and (kc == 1).all() and (vc == 1).all()
+
+
+# ------------------------------------------------------------------ plans and captures
+@pytest.mark.gpu
+def test_host_lengths_are_refused_inside_a_capture():
+    """Their copy would break the capture; the refusal leaves it whole."""
+    lengths = torch.tensor([3, 2], dtype=torch.int32, device="cuda")
+    q = torch.randn(5, 2, 64, device="cuda").bfloat16()
+    want = attention_packed(q, q, q, PackedBatch([3, 2]))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(ValueError):
+            PackedBatch([3, 2])
+        got = attention_packed(q, q, q, PackedBatch(lengths, total=5))
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
