@@ -159,8 +159,14 @@ def attention_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: P
     (behind the last sequence) give zeros and get zero gradients, whatever they
     hold.  On a GPU: bf16 or fp16, D 64 or 128; q / k / v may be views with
     dense 16-byte aligned rows (slices of a fused projection), others are
-    copied.  Never does anything of one sequence enter another, NaN and infinities
-    included.  Inside its own sequence a non-finite value (in v; for gradients
+    copied.  A call that will be differentiated keeps its inputs, the result,
+    what the result's rounding dropped (a second [T, Hq, D]) and row sums (fp32
+    [Hq, T]) for the gradient.  Forward-mode derivatives are refused on a GPU.
+
+    How the work is split depends on the whole batch (its rows and its number of
+    sequences), so a sequence may round differently in another batch; one call
+    repeated gives the same bits.  Never does anything of one sequence enter
+    another, NaN and infinities included.  Inside its own sequence a non-finite value (in v; for gradients
     also in q, k or the incoming gradient) reaches what depends on it, and may
     also reach up to 63 rows on its other side of the causal diagonal."""
     qs, ks = q.shape, k.shape

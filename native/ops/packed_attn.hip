@@ -8,11 +8,18 @@
 //   dV_j = sum_i p_ij dO_i          dP_ij = dO_i v_j      D_i = dO_i o_i
 //   dS = p (dP - D)   dQ_i = s sum_j dS_ij k_j   dK_j = s sum_i dS_ij q_i
 //
+// P is rounded to 16 bits once in the forward, P and dS once each in the
+// gradient: the matrix instructions take 16-bit operands, and a second one for
+// what the rounding dropped would be half as many products again.  It shows as
+// an error of up to 2.2e-3 (o) and 2.4e-3 (o and gradients) of the norm in bf16,
+// where the rounding of the result alone is 1.7e-3.  Sums, row statistics and
+// states are fp32.
+//
 // D comes from the unrounded o: the forward also stores what its rounding
-// dropped (one more 16-bit value), since D is subtracted from every dP of the
-// row and an error of o's rounding would show in dQ and dK (2.6e-3 of the
-// gradient's norm in bf16, against 2.3e-3 for the roundings of dS and of the
-// result alone).
+// dropped (one more 16-bit value per element of o, 134 MB at 16,384 rows of 32
+// heads x 128), since D is subtracted from every dP of the row and an error of
+// o's rounding would move them all one way: 2.6e-3 in bf16 with centred values,
+// far more where keys and values have a common mean.
 //
 // One workgroup = 4 waves = 128 rows of one sequence and head (a job of the
 // batch's plan, longest sweep first); q, k, v are read through their strides,
@@ -22,14 +29,18 @@
 // nothing) holds there never enters.
 //
 // Bounds, measured in bf16 with 32 / 8 heads: one sequence of 16,384 rows,
-// causal, D 128, runs at 1.15 PF/s forward (1.92 ms), 1.24 in dQ (2.65 ms) and
-// 1.13 in dK / dV (3.89 ms), a plain matrix product of 8,192^3 at 1.37; the
-// clock is then down to 1.77 GHz at the card's power limit (operands of zeros
-// run 25 % faster), so fewer operations would help, a better schedule does
-// not.  At D 64 the softmax weighs twice as much: 32 exponentials and as many
-// multiply-adds per 16 matrix instructions: 0.94 PF/s at 8,000 rows.  Ragged batches
-// lose to blocks of few rows and to the last workgroups (24 documents of 64 to
-// 4,096 rows: 0.23 + 0.35 + 0.39 ms, 618 TF/s over all three).
+// causal, D 128, runs at 1.09 to 1.15 PF/s forward (1.92 to 2.02 ms, by the
+// card), 1.18 to 1.24 in dQ (2.65 to 2.79 ms) and 1.08 to 1.13 in dK / dV (3.89
+// to 4.06 ms), a plain matrix product of 8,192^3 at 1.37; the matrix cores are
+// busy 63, 67 and 57 % of the time and the clock is down to 1.77 GHz at the
+// card's power limit (operands of zeros run 25 % faster), so fewer operations
+// would help, a better schedule does not.  At D 64 the softmax weighs twice as
+// much: 32 exponentials and as many multiply-adds per 16 matrix instructions,
+// 0.94 PF/s at 8,000 rows.  Ragged batches (24 documents of 64 to 4,096 rows:
+// 0.23 + 0.35 + 0.41 ms, 580 TF/s over all three) keep the matrix cores busy 36,
+// 36 and 41 %: the SIMDs hold 2.3, 1.7 and 1.3 waves of 3, 2 and 2 on average
+// (2.7, 1.9 and 1.7 at 16,384 rows), which wait for loads and barriers 25 to 32
+// % of their time (19 to 27).  Masked and empty keys are 8 % of the products.
 //
 // Tried and slower: 8 waves and 256 rows per tile (documents 210 -> 235 us),
 // two workgroup halves on alternate tiles where there are workgroups enough (32
@@ -124,7 +135,7 @@ constexpr float kDefer = 4.f;
 //   dS has no bound that is worth having, so every accumulated row (of dQ or
 //   dK) has a factor of its own, a power of two from 2^60 down: where a tile's
 //   dS would pass 2^15 the factor and the sums so far are scaled down together,
-//   the largest to 2^13 .. 2^14.  What is 2^28 below a row's largest dS still
+//   the largest to 2^13 .. 2^14.  What is 2^27 below a row's largest dS still
 //   counts in full.
 // Factors are powers of two and leave the accumulators through the result's own
 // multiplier, so they round nothing.  The maxima cost 3 to 6 % of a training

@@ -18,10 +18,12 @@
 // own keys count the chunks that hold keys from lens and take every o_wgs-th.
 //
 // Measured (32 / 8 heads, bf16, GPU time of a call): 64 rows, 32,768 shared
-// keys and up to 1,500 own ones, D 128: 52.5 us, of which the join 7 us; the
-// 184 MB alone take 37 us at the card's copy rate, 3.5 TB/s is reached while
-// every prefix key is also multiplied with 256 rows.  32 rows, 2,048 + up to
-// 1,000 keys, D 64: 10.4 us for 14 MB, two launches' latency.  4 rows, 200 +
+// keys and up to 1,500 own ones, D 128: 54 + 7.6 us, the second for the join
+// (52.5 in all where the call repeats on the same inputs, which the last-level
+// cache can hold); the 184 MB alone take 37 us at the card's copy rate, 3.4 TB/s
+// is reached while every prefix key is also multiplied with 256 rows, by 1.2
+// waves per SIMD.  32 rows, 2,048 + up to 1,000 keys, D 64: 8.2 + 3.9 us for 14
+// MB, two launches whose waves wait 63 and 71 % of their time.  4 rows, 200 +
 // up to 60 keys: 4.8 us, one launch.  1,024 rows, 500 + up to 1,000 keys,
 // D 64: 123 us.
 #include <algorithm>
