@@ -57,14 +57,24 @@ __device__ __forceinline__ bf16x8 as_op(const u32x4& w) { return __builtin_bit_c
 // 2^-126 is zero to any 16-bit output.
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// log2 of what a probability against a running maximum is multiplied by before
-// it is rounded to T: fp16 has steps of 2^-24 below 2^-14, and what many keys
-// far from the maximum add up to would be lost (65,536 keys at 2^-26 of it:
-// all).  The sum of the probabilities carries the same factor, so the output
-// does not; it costs nothing, the exponent takes it.  Running maxima lag by up
-// to 2^4 (kDefer): 2^15 at most, and fp16 ends at 65,504.
+// Running maximum (log2 units) kept until a tile's largest score passes it by
+// this much, so outputs are rescaled on few tiles.
+constexpr float kDefer = 4.f;
+
+// The reference that exponents are taken against, after a tile whose largest
+// score is `top`: the running maximum, in fp16 less 11, which multiplies all
+// probabilities and their sum by 2^11 before they are rounded to T.  fp16 has
+// steps of 2^-24 below 2^-14, and what many keys far from the maximum add up to
+// would be lost (65,536 keys at 2^-26 of it: all).  With kDefer that is 2^15 at
+// most, and fp16 ends at 65,504.  Scores past 2^20 are not lifted: the rounding
+// of top * c, which the exponents do not share, needs the room there.
 template <class T>
-constexpr float kLift = std::is_same<T, Fp16>::value ? 11.f : 0.f;
+__device__ __forceinline__ float next_max(float top, float c, float m) {
+  const float x = top * c;
+  float lift = 0.f;
+  if constexpr (std::is_same<T, Fp16>::value) lift = fabsf(x) < 0x1p20f ? 11.f : 0.f;
+  return x > m + (kDefer + lift) ? x - lift : m;
+}
 
 // Row of a 32x32 accumulator tile that register r of this lane half holds.
 __device__ __forceinline__ int tile_row(int r, int half) { return (r & 3) + 8 * (r >> 2) + 4 * half; }

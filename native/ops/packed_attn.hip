@@ -121,10 +121,6 @@ __device__ __forceinline__ int wave_rows(const Batch& b, const Job& job, int wav
   return job.blk * kRows + 32 * (wave & ((1 << per) - 1));
 }
 
-// Running max kept until a tile's max passes it by this much (log2 units), so
-// P stays below 2^4 (kLift counts on it) and O is rescaled on few tiles.
-constexpr float kDefer = 4.f;
-
 // The gradient's 16-bit operands, P and dS, in fp16.  At their natural size P =
 // 1 / n and dS = P (dP - D) of long rows fall among fp16's steps of 2^-24 (dQ for
 // incoming gradients of 1e-3 was off by 1.1e-2 of its norm at 12,000 keys, by
@@ -138,7 +134,7 @@ constexpr float kDefer = 4.f;
 //   the largest to 2^13 .. 2^14.  What is 2^27 below a row's largest dS still
 //   counts in full.
 // Factors are powers of two and leave the accumulators through the result's own
-// multiplier, so they round nothing.  The maxima cost 3 to 6 % of a training
+// multiplier, so they round nothing.  The maxima cost 3 to 8 % of a training
 // call (16,384 rows, 32 / 8 heads x 128: 8.91 -> 9.19 ms, 300 sequences of 10 to
 // 60 rows 269 -> 285 us).
 template <class T>
@@ -272,8 +268,7 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 1 : TWO_V ? 2 : 3) void
       for (int st = 0; st < 2; ++st)
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[st][r]);
-      mx = half_max(mx) * a.c;
-      const float m_new = mx > m + kDefer ? mx : m;
+      const float m_new = next_max<T>(half_max(mx), a.c, m);
       const float m_use = m_new == -INFINITY ? 0.f : m_new;
       if (__any(m_new > m && m > -INFINITY)) {  // before a row's first max there is nothing to rescale
         const float alpha = exp2_fast(m - m_use);
@@ -284,15 +279,14 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 1 : TWO_V ? 2 : 3) void
           for (int r = 0; r < 16; ++r) oacc[i][r] *= alpha;
       }
       m = m_new;
-      const float m_p = m_use - kLift<T>;
-      // P = 2^(S c - m), in fp16 2^11 times that, in pairs; the accumulator tile is the next product's operand as it is
+      // P = 2^(S c - m) in pairs; the accumulator tile is the next product's operand as it is
       float r0 = 0.f, r1 = 0.f;
 #pragma unroll
       for (int st = 0; st < 2; ++st)
 #pragma unroll
         for (int r = 0; r < 16; r += 2) {
-          const float p0 = exp2_fast(fmaf(s[st][r], a.c, -m_p));
-          const float p1 = exp2_fast(fmaf(s[st][r + 1], a.c, -m_p));
+          const float p0 = exp2_fast(fmaf(s[st][r], a.c, -m_use));
+          const float p1 = exp2_fast(fmaf(s[st][r + 1], a.c, -m_use));
           r0 += p0;
           r1 += p1;
           pb[2 * st + (r >> 3)][(r & 7) >> 1] = pack2<T>(p0, p1);
@@ -372,8 +366,12 @@ __global__ __launch_bounds__(256 * HALVES, HALVES == 2 ? 1 : TWO_V ? 2 : 3) void
       for (int r = 0; r < 16; ++r) oacc[i][r] = oacc[i][r] * inv - T::up(T::down(oacc[i][r] * inv));
     store_row<T, NB>(a.o_low + off, oacc, 1.f, hh, ok);
   }
-  if (a.lse != nullptr && ok && hh == 0)
-    a.lse[static_cast<int64_t>(h) * a.b.T + orow] = lt == 0.f ? -INFINITY : m + log2f(lt) - kLift<T> - kLiftP<T>;
+  if (a.lse != nullptr && ok && hh == 0) {
+    float z = lt == 0.f ? -INFINITY : m + log2f(lt) - kLiftP<T>;
+    // Where a step of it is 1 and more it is rounded up, or P might pass its 2^14 by more than fp16 holds.
+    if constexpr (kScaled<T>) z += fabsf(z) > 0x1p23f && lt != 0.f ? fabsf(z) * 0x1p-22f : 0.f;
+    a.lse[static_cast<int64_t>(h) * a.b.T + orow] = z;
+  }
 }
 
 struct BwdArgs {

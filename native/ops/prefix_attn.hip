@@ -36,7 +36,6 @@ namespace {
 
 typedef unsigned short u16;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kDefer = 4.f;  // as in packed_attn.hip (kLift counts on it)
 constexpr int kWide = 64;      // keys per tile of the 128-row form, shared by 4 waves
 constexpr int kSlim = 32;      // keys per tile of the 32-row form, one wave's own
 
@@ -67,7 +66,7 @@ struct State {
     for (int i = 0; i < NB; ++i) o[i] = f32x16{};
   }
   // Scores of NS x 32 keys (key on the accumulator's rows), of which the first
-  // `valid` count -> P (in fp16 2^11 times P, as is l) as the next product's operand.
+  // `valid` count -> P as the next product's operand.
   template <int NS>
   __device__ __forceinline__ void soften(f32x16 (&s)[NS], int valid, float c, int hh, u32x4 (&pb)[2 * NS]) {
     if (valid < 32 * NS) {
@@ -82,8 +81,7 @@ struct State {
     for (int st = 0; st < NS; ++st)
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[st][r]);
-    mx = half_max(mx) * c;
-    const float m_new = mx > m + kDefer ? mx : m;
+    const float m_new = next_max<T>(half_max(mx), c, m);
     const float m_use = m_new == -INFINITY ? 0.f : m_new;
     if (__any(m_new > m && m > -INFINITY)) {  // before a row's first max there is nothing to rescale
       const float alpha = exp2_fast(m - m_use);
@@ -94,13 +92,12 @@ struct State {
         for (int r = 0; r < 16; ++r) o[i][r] *= alpha;
     }
     m = m_new;
-    const float m_p = m_use - kLift<T>;
     float r0 = 0.f, r1 = 0.f;
 #pragma unroll
     for (int st = 0; st < NS; ++st)
 #pragma unroll
       for (int r = 0; r < 16; r += 2) {
-        const float p0 = exp2_fast(fmaf(s[st][r], c, -m_p)), p1 = exp2_fast(fmaf(s[st][r + 1], c, -m_p));
+        const float p0 = exp2_fast(fmaf(s[st][r], c, -m_use)), p1 = exp2_fast(fmaf(s[st][r + 1], c, -m_use));
         r0 += p0;
         r1 += p1;
         pb[2 * st + (r >> 3)][(r & 7) >> 1] = pack2<T>(p0, p1);

@@ -213,3 +213,50 @@ def test_a_dropped_plan_is_not_handed_out_before_its_launch_has_run():
     assert at not in [t.data_ptr() for t in other]
     main.wait_stream(side)
     assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------ scores past 2^24
+@pytest.mark.parametrize("scale", [300.0, 3000.0, 6000.0])
+@pytest.mark.parametrize("d,dtype", [(64, torch.float16), (128, torch.float16), (128, torch.bfloat16)])
+def test_huge_scores_choose_their_key(scale, d, dtype):
+    """Scores of 1e5 to 1e8: an fp32 exponent is off by up to several units there, which must not carry a lifted
+    probability past fp16's largest value.  Rows whose best key leads by far (2^-18 of the scores' size and 60 units,
+    well past every rounding) give its value; gradients are finite."""
+    g = torch.Generator(device="cuda").manual_seed(d)
+    n, hq, hkv = 700, 4, 2
+    q, k = _rnd(g, n, hq, d, dtype=dtype, scale=scale), _rnd(g, n, hkv, d, dtype=dtype, scale=scale)
+    k[:200] *= 0.1  # maxima that rise
+    v, do = _rnd(g, n, hkv, d, dtype=dtype), _rnd(g, n, hq, d, dtype=dtype)
+    batch = PackedBatch([n])
+
+    def check(o, keys, vals, seen=None):
+        for h in range(hq):
+            s = q[:, h].double() @ keys[h // 2].double().T / math.sqrt(d)
+            s = s if seen is None else s.masked_fill(~seen, -math.inf)
+            best = s.topk(2, 1)
+            led = best.values[:, 0] - best.values[:, 1] > 60 + 2.0 ** -18 * s.masked_fill(s == -math.inf, 0).abs().amax(1)
+            assert led.sum() > n // 2
+            want = vals[h // 2][best.indices[led, 0]].double()
+            # the one probability left is 2^x for some x <= 4, rounded once and divided by its unrounded self: 1 + h at
+            # most; then the result's own rounding, and 2^-20 for fp32's
+            assert ((o[led, h].double() - want).abs() <= (2 * HALF[dtype] + HALF[dtype] ** 2 + 2.0 ** -20) * want.abs()
+                    + STEP[dtype]).all()
+
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    for causal in (True, False):
+        o = attention_packed(*leaves, batch, causal=causal)
+        assert all(t.isfinite().all() for t in (o, *torch.autograd.grad(o, leaves, do)))
+        if not causal:
+            check(o.detach(), k.detach().transpose(0, 1), v.detach().transpose(0, 1))
+    with torch.no_grad():
+        # each row as the single token of a sequence behind the others' keys
+        pk, pv = k.transpose(0, 1).contiguous(), v.transpose(0, 1).contiguous()
+        own = torch.zeros(n, hkv, 8, d, device="cuda", dtype=dtype)
+        att = dec.PrefixDecodeAttention(n, hq, hkv, d, 8, n, "cuda", dtype=dtype)
+        check(att(q, pk, pv, own, own, torch.zeros(n, dtype=torch.int32, device="cuda")), pk, pv)
+        few = dec.PrefixDecodeAttention(8, hq, hkv, d, 8, n, "cuda", dtype=dtype)
+        o = torch.cat([few(q[i:i + 8].contiguous(), pk, pv, own[:8], own[:8], torch.zeros(8, dtype=torch.int32, device="cuda"))
+                       for i in range(0, n - 4, 8)] + [torch.zeros_like(q[:n % 8])])
+        keep = n - n % 8
+        q, n = q[:keep], keep
+        check(o[:keep], pk, pv)
